@@ -77,6 +77,9 @@ def build_torch_binding(force: bool = False) -> str:
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     cmd += [f"-I{p}" for p in ext.include_paths("cuda")]
     cmd += [f"-L{p}" for p in ext.library_paths("cuda")] + [f"-L{LIB_DIR}"]
+    # the shared C++ runtime, also where the compiler's default is a static one: torch's exceptions carry text formatted by
+    # streams, and two copies of the runtime in one process do not share their locales (formatting a number then crashes)
+    cmd += ["-l:libstdc++.so.6"]
     cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lquant_cast_cuda", "-lcudart",
             "-Wl,-rpath,$ORIGIN", "-Wl,--no-as-needed"]
     r = subprocess.run(cmd, capture_output=True, text=True)
