@@ -280,6 +280,29 @@ int qcc_fp8_block128x128(const void *x, int64_t M, int64_t N, int flags /* 0 or 
 int qcc_amax_block128x128(const void *x, int64_t M, int64_t N, int mode, float *out, void *stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * 8-bit integer linear layer (no counterpart in the reference: the sibling of its rowwise fp8 cast, and the product that
+ * consumes it)
+ * ------------------------------------------------------------------------------------------- */
+
+/* One scale per row: scale[r] = max(amax_r, bf16(1e-12)) / 127, q = int8(rne(x * (1 / scale[r]))), |q| <= 127: the recipe
+ * of rowwise_fp8_f (G:301-307) with 127 for the fp8 maximum.  A row that holds a NaN gets a NaN scale, one that holds an
+ * infinity an infinite scale; its codes then mean nothing.  Any N >= 1; M may be 0.  flags: 0 or QCC_RECIP_DIV. */
+int qcc_int8_rowwise(const void *x, int64_t M, int64_t N, int flags, void *q, float *scale, void *stream);
+
+/* element type of an output */
+#define QCC_OUT_BF16 0
+#define QCC_OUT_F16 1
+#define QCC_OUT_F32 2
+
+/* out (M, N) = (sum_k a[m][k] * b[n][k]) * scale_a[m] * scale_b[n] + bias[n]: a (M, K) and b (N, K) contiguous int8, the sum
+ * exact in 32-bit integers, the scales applied in fp32, one rounding to the output type.  bias: bf16 (N) or NULL.
+ * K % 16 == 0 (TMA rows), 16 <= K <= QCC_INT8_MAX_K (128 * 128 * K stays below 2^31); M and N are free, 0 included.  a, b and
+ * out 16-byte aligned. */
+#define QCC_INT8_MAX_K 131056
+int qcc_int8_scaled_mm(const void *a, const void *b, int64_t M, int64_t N, int64_t K, const float *scale_a, const float *scale_b,
+                       const void *bias, int out_dtype, void *out, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
  * mxfp8: 32-element blocks, e8m0 scales, e4m3 elements
  * ------------------------------------------------------------------------------------------- */
 
@@ -431,6 +454,89 @@ int qcc_nvfp4_transposed(const void *x, int64_t M, int64_t N, const float *outer
  */
 int qcc_nvfp4_both(const void *x, int64_t M, int64_t N, const float *outer, int flags, void *qk, void *sk,
                    void *qm, void *sm, void *stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * paged nvfp4 key/value cache (no counterpart in the reference: its nvfp4 cast with a cache's pages for destination, and the
+ * operators that read them)
+ *
+ * cache: (num_pages, kv_heads, 2, page * 9 * head_dim / 16) bytes, 16-byte aligned.  For keys (0) and values (1) of a page and
+ * head: the e2m1 codes of its tokens, (page, head_dim / 2) bytes with the even element in the low nibble, then their e4m3
+ * block scales, (page, head_dim / 16) bytes.  value = code * scale * outer, with one fp32 outer scale for keys and one for
+ * values (device; finite and > 0).  head_dim 64 or 128; page 16, 32, 64 or 128 tokens.  Nothing needs to be initialised:
+ * a slot is read only once a sequence's length says that it holds a token.
+ *
+ * Sequences are rows of a block table of int32 page numbers: token i of sequence b is token i % page of page
+ * table[b * table_stride + i / page].  Slot numbers are page * page_number + offset.  Page, slot and position numbers live on
+ * the device and are checked there: one outside its range sets code 20 (page, slot, or a length beyond the table row) or 21
+ * (position) in the word qcc_device_error reads; a token with a bad slot or position is not written, one on a bad page is read
+ * back as zeros.
+ * ------------------------------------------------------------------------------------------- */
+
+/* Bytes of one page (0 for an unsupported geometry). */
+size_t qcc_nvfp4_kv_page_bytes(int kv_heads, int page, int head_dim);
+
+#define QCC_ROPE_INTERLEAVED 0x2000 /* rotate neighbouring elements (2i, 2i+1) instead of (i, i + rot/2) */
+
+/* Appends `tokens` keys and values, bf16 (tokens, kv_heads, head_dim), to the cache: the first `rot` elements of each key are
+ * rotated by its position, then keys and values are cast to nvfp4 (the recipe of nvfp4_gs_f, G:1494-1517) into slot
+ * slots[t]; a negative slot skips the token (a padded row of a batch).  The non-negative slots of a call must differ.
+ * q (tokens, q_heads, head_dim), if q_heads > 0, is rotated the same way into q_out (contiguous bf16); rows whose position is
+ * outside the table become zero.  cos_sin (max_pos, rot) fp32: rot/2 cosines, then rot/2 sines of a position.  rot is 0 (no
+ * rotation) or a multiple of 32 up to head_dim.  Rotation in fp32, each product and sum rounded on its own; the cast takes the
+ * fp32 result.  A block that holds a NaN reads back as NaN. */
+typedef struct qcc_kv_append_args {
+    const void *k, *v, *q;               /* 16-byte aligned; rows contiguous                                   */
+    void *q_out;
+    int64_t k_stride[2], v_stride[2], q_stride[2]; /* elements from a token, and from a head, to the next; multiples of 8 */
+    int64_t tokens;
+    void *cache;
+    int64_t num_pages;
+    const int64_t *slots, *positions;    /* (tokens); positions may be NULL when rot == 0                      */
+    const float *cos_sin;                /* 16-byte aligned                                                    */
+    int64_t max_pos;
+    const float *k_outer, *v_outer;
+    int kv_heads, q_heads, head_dim, page, rot;
+    int flags;                           /* QCC_ROPE_INTERLEAVED, QCC_RECIP_DIV                                */
+} qcc_kv_append_args;
+int qcc_nvfp4_kv_append(const qcc_kv_append_args *args, void *stream);
+
+/* Reads sequences back: k, v (total, kv_heads, head_dim) bf16 = bf16(code * scale * outer); rows cu_kv[b] .. cu_kv[b+1] - 1
+ * are the tokens of sequence b (cu_kv: device int32[seqs + 1], ascending from 0); rows from cu_kv[seqs] on become zero. */
+int qcc_nvfp4_kv_gather(const void *cache, int64_t num_pages, int kv_heads, int page, int head_dim, const int32_t *table,
+                        int64_t table_stride, int table_width, const int32_t *cu_kv, int seqs, int64_t total,
+                        const float *k_outer, const float *v_outer, void *k, void *v, void *stream);
+
+/* Attention over the cache.  q (rows, q_heads, head_dim) bf16, already rotated; kv_lens[b] (device int32): tokens that the cache
+ * holds of sequence b.  Without cu_q every sequence has one query (rows == seqs); with it rows cu_q[b] .. cu_q[b+1] - 1 are the
+ * queries of sequence b, its LAST tokens: query i of n sees the keys j <= kv_lens[b] - n + i.  max_q: at least the most
+ * queries of a sequence.  q head h reads kv head h / (q_heads / kv_heads).
+ *   out (rows, q_heads, head_dim) bf16 = sum_j softmax_j(scale * q . k_j) v_j;  lse (rows, q_heads) fp32, may be NULL, =
+ *   log sum_j exp(scale * q . k_j).  A query that sees no key, and every row behind the last sequence: out = 0, lse = -inf.
+ * Sums, maxima and the softmax in fp32; the probabilities are rounded to fp16 before they multiply the values.
+ * The result does not depend on what the slots behind a sequence's last token hold.  Two runs on the same inputs give the
+ * same bits.  A sequence whose query offsets descend, leave the rows of q or hold more than max_q rows sets code 22 in the word
+ * qcc_device_error reads, and its rows are not written; one that reaches a bad page (code 20) gets a result without meaning.
+ * workspace: scratch of qcc_nvfp4_kv_attention_workspace_bytes, 16-byte aligned, any contents; calls that may overlap on the
+ * GPU need one each.  At most 4096 sequences. */
+typedef struct qcc_kv_attention_args {
+    const void *q;               /* 16-byte aligned, rows contiguous                              */
+    int64_t q_stride[2];         /* elements from a row, and from a head, to the next; multiples of 8 */
+    int64_t rows;
+    const void *cache;
+    int64_t num_pages;
+    const int32_t *table;        /* (seqs, table_width), rows table_stride apart                   */
+    int64_t table_stride;
+    int table_width;
+    const int32_t *kv_lens, *cu_q;
+    int seqs, max_q;
+    const float *k_outer, *v_outer;
+    float scale;
+    int q_heads, kv_heads, head_dim, page;
+    void *out;
+    float *lse;
+} qcc_kv_attention_args;
+size_t qcc_nvfp4_kv_attention_workspace_bytes(int seqs, int max_q, int q_heads, int kv_heads, int head_dim);
+int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------------------------
  * 16-point randomised Hadamard transform (RHT) and the nvfp4 casts built on it

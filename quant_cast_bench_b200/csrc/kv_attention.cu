@@ -1,0 +1,623 @@
+// Attention over the paged nvfp4 key/value cache, sm_100a.
+//
+//   o = sum_j softmax_j(scale * q . k_j) v_j,   lse = log sum_j exp(scale * q . k_j)
+//
+// over the keys j that a query sees: query i of the n of a sequence with L cached tokens sees j <= L - n + i.  A query that
+// sees none gets o = 0 and lse = -inf.  One pass over the cache with the running maximum and sum of the softmax in fp32.
+#include "kv_cache.cuh"
+
+#include "host_util.h"
+
+namespace qcc {
+
+constexpr unsigned int QCC_DEVERR_QUERIES = 22u;    // query offsets that are not ascending within the rows of q
+constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ran out
+constexpr int KV_MAX_SEQS = 4096;
+constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+
+struct AttnArgs {
+    const uint16_t *q;
+    const uint8_t *cache;
+    const int32_t *table, *kv_lens, *cu_q;
+    const float *k_outer, *v_outer;
+    uint16_t *out;
+    float *lse, *part;      // part: 2 slots per CTA of NT * 8 rows x (D + 2) floats
+    int32_t *prefix;        // seqs + 1
+    int64_t q_token, q_head, table_stride, num_pages, rows;
+    float scale_log2;
+    int seqs, width, q_heads, kv_heads, group, page, max_q;
+};
+
+__device__ __forceinline__ float ex2(float x)
+{
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+    return r;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
+{
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
+{
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t a)
+{
+    uint32_t r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
+    return r;
+}
+__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
+                 "r"(bytes), "r"(smem_u32(bar))
+                 : "memory");
+}
+
+// queries and cached tokens of sequence b, checked against what the caller's tensors hold
+__device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n, int &L)
+{
+    if (g.cu_q) {
+        q0 = __ldg(g.cu_q + b);
+        n = __ldg(g.cu_q + b + 1) - q0;
+        if (q0 < 0 || n < 0 || n > g.max_q || (int64_t)q0 + n > g.rows) {
+            atomicMax(&g_qcc_error, QCC_DEVERR_QUERIES);
+            q0 = 0;
+            n = 0;
+        }
+    } else {
+        q0 = b;
+        n = 1;
+    }
+    L = max(__ldg(g.kv_lens + b), 0);
+    if (L > (int64_t)g.width * g.page) {
+        atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
+        L = g.width * g.page;
+    }
+}
+
+// -------------------------------------------------------------------------------------------------------------------
+// Few queries: work split over the cached tokens
+//
+// The rows of a sequence and kv head (its queries times the heads of the group) are at most a few, so the time is that of
+// reading the cache: 9/16 byte an element, and every element has to be widened before a matrix instruction takes it.  That
+// widening is what competes with HBM (41 elements a clock and SM at full bandwidth), so codes go from shared memory straight
+// into the registers that mma.sync m16n8k16 wants, with no second trip through shared memory:
+//   S^T = K Q^T    A: 16 tokens x 16 elements.  A thread's fragment rows are tokens, and the order of the contracted elements
+//                  is free as long as Q has the same, so a thread reads 16 contiguous bytes (32 elements) of a token.
+//   O^T = V^T P^T  A: 16 elements x 16 tokens.  A thread reads one 16-element block of four tokens; the nibbles of two tokens
+//                  are brought side by side before they are widened, which gives the token pairs of the fragment.
+// The queries are on the N side, 8 at a time: no row of the instruction is spent on padding when a group has 8 heads.
+// Codes times block scales are exact in fp16 (2 + 4 significant bits); q is brought to fp16 by a power of two for its row,
+// exact for all elements above 2^-22 of the row's largest; P is rounded to fp16, half a step of 2^-11.  The tensor cores are
+// far from busy (tcgen05 would need the widened tiles in shared memory, whose bandwidth that alone would use up).
+//
+// A tile is 128 tokens of one sequence and head, 16 for each warp.  A warp fetches its own tokens by bulk copies into a ring of
+// its own, so the warps of a CTA meet only where a unit ends.  All tiles of the batch are numbered and dealt out evenly,
+// whatever the lengths; a unit (sequence, head, row tile) that spans CTAs leaves partial sums which a second kernel joins in a
+// fixed order.
+// -------------------------------------------------------------------------------------------------------------------
+constexpr int SP_WARPS = 8, SP_THREADS = SP_WARPS * 32, SP_TOK = 16 * SP_WARPS;
+
+template <int D, int NT> struct SplitCfg {
+    static constexpr int TILE = 16 * 2 * (D / 2 + D / 16);          // bytes of one warp's 16 tokens, keys and values
+    static constexpr int CTAS = NT == 1 ? 2 : 1;
+    static constexpr int STAGES = (NT == 1 ? 5 : 8) * (D == 64 ? 2 : 1);
+    static constexpr int RED = SP_WARPS * NT * 8 * (D / 4) * 4;
+    static constexpr int ML = SP_WARPS * NT * 8 * 2 * 4;
+    static constexpr int FIXED = SP_WARPS * (TILE * STAGES + STAGES * 8) + RED + ML;
+};
+
+template <int D, int NT> __host__ __device__ constexpr int part_floats() { return NT * 8 * (D + 2); }
+
+struct Segment {
+    int b, q0, n, L, head, rt, first, last, unit_last;   // first, last: tiles of the unit; unit_last: flat number of the tile behind it
+};
+
+// the segment that starts at flat tile t: its unit's tiles [first, last) within hi
+template <int NT>
+__device__ __forceinline__ void find_segment(const AttnArgs &g, const int32_t *prefix, int t, int hi, Segment &s)
+{
+    int lo = 0, up = g.seqs - 1;      // last b with prefix[b] <= t (t < total, so it has tiles)
+    while (lo < up) {
+        const int mid = (lo + up + 1) >> 1;
+        if (prefix[mid] <= t) lo = mid; else up = mid - 1;
+    }
+    s.b = lo;
+    seq_of(g, lo, s.q0, s.n, s.L);
+    const int kvt = (s.L + SP_TOK - 1) / SP_TOK, rts = (s.n * g.group + NT * 8 - 1) / (NT * 8);
+    const int local = t - prefix[lo], unit = local / kvt;
+    s.head = unit / rts;
+    s.rt = unit - s.head * rts;
+    s.first = local - unit * kvt;
+    s.last = min(kvt, s.first + hi - t);
+    s.unit_last = prefix[lo] + (unit + 1) * kvt;
+}
+// tiles that some row of the row tile sees
+template <int NT>
+__device__ __forceinline__ int seen_tiles(const AttnArgs &g, const Segment &s)
+{
+    const int i = min(s.n - 1, ((s.rt + 1) * NT * 8 - 1) / g.group);
+    const int end = s.L - s.n + i + 1;
+    return min(s.last, (max(end, 0) + SP_TOK - 1) / SP_TOK);
+}
+
+template <int D, int NT>
+__global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_split_kernel(const AttnArgs g)
+{
+    using C = SplitCfg<D, NT>;
+    constexpr int KW = D / 32, VW = D / 64, MT = D / 16, RB = D / 2 + D / 16;    // words of a thread per token: keys, values; m tiles
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t *ring = smem + warp * (C::TILE * C::STAGES);
+    float *red = reinterpret_cast<float *>(smem + SP_WARPS * C::TILE * C::STAGES);
+    float2 *ml = reinterpret_cast<float2 *>(red + C::RED / 4);
+    uint64_t *full = reinterpret_cast<uint64_t *>(ml + C::ML / 8) + warp * C::STAGES;
+    int32_t *prefix = reinterpret_cast<int32_t *>(reinterpret_cast<uint64_t *>(ml + C::ML / 8) + SP_WARPS * C::STAGES);
+    __shared__ int32_t wsum[SP_WARPS];
+
+    if (lane == 0)
+        for (int i = 0; i < C::STAGES; i++) mbar_init(full + i, 1);
+    if (threadIdx.x == 0) prefix[0] = 0;
+    fence_barrier_init();
+    // tiles of each sequence, summed up
+    int carry = 0;
+    for (int b0 = 0; b0 < g.seqs; b0 += SP_THREADS) {
+        const int b = b0 + threadIdx.x;
+        int v = 0;
+        if (b < g.seqs) {
+            int q0, n, L;
+            seq_of(g, b, q0, n, L);
+            v = g.kv_heads * ((n * g.group + NT * 8 - 1) / (NT * 8)) * ((L + SP_TOK - 1) / SP_TOK);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+            if (lane >= o) v += u;
+        }
+        if (lane == 31) wsum[warp] = v;
+        __syncthreads();
+        int before = carry, all = carry;
+        for (int w = 0; w < SP_WARPS; w++) {
+            if (w < warp) before += wsum[w];
+            all += wsum[w];
+        }
+        if (b < g.seqs) prefix[b + 1] = before + v;
+        carry = all;
+        __syncthreads();
+    }
+    const int total = carry, ctas = min((int)gridDim.x, total);
+    if (blockIdx.x == 0)
+        for (int i = threadIdx.x; i <= g.seqs; i += SP_THREADS) g.prefix[i] = prefix[i];
+    if ((int)blockIdx.x >= ctas) return;
+    const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
+
+    // ---- fetching: the warp's 16 tokens of tile after tile, C::STAGES ahead of their use.  The page of the next fetch is looked
+    // up one fetch early.
+    struct { Segment s; int t, tile, end; int64_t page; } f;
+    uint32_t fetched = 0;
+    f.t = lo;
+    const uint32_t tok_bytes = 2 * RB * 16;
+    // moves the cursor to the next tile that exists (f.t < hi), and asks for its page
+    auto seek = [&](bool fresh) {
+        for (;;) {
+            if (!fresh) {
+                if (++f.tile < f.end) break;
+                f.t += f.s.last - f.s.first;
+            }
+            if (f.t >= hi) return;
+            find_segment<NT>(g, prefix, f.t, hi, f.s);
+            f.tile = f.s.first - 1;
+            f.end = seen_tiles<NT>(g, f.s);
+            fresh = false;
+        }
+        const int tok = f.tile * SP_TOK + warp * 16;
+        f.page = tok < f.s.L ? (int64_t)__ldg(g.table + f.s.b * g.table_stride + tok / g.page) : -1;
+    };
+    auto fetch = [&]() {
+        if (f.t >= hi) return;
+        const uint32_t st = fetched++ % C::STAGES;
+        const int tok = f.tile * SP_TOK + warp * 16;
+        const bool some = tok < f.s.L, ok = f.page >= 0 && f.page < g.num_pages;
+        if (lane == 0) {
+            if (some && !ok) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
+            mbar_expect_tx(full + st, ok ? tok_bytes : 0);
+        }
+        __syncwarp();
+        if (ok) {
+            const uint8_t *src = g.cache + (f.page * g.kv_heads + f.s.head) * (int64_t)(g.page * 2 * RB);
+            uint8_t *dst = ring + st * C::TILE;
+            if (g.page == 16) {
+                if (lane == 0) bulk_load(dst, src, tok_bytes, full + st);
+            } else if (lane < 4) {       // codes and scales of keys, codes and scales of values
+                const int off = tok % g.page, scales = lane & 1;
+                bulk_load(dst + (lane >> 1) * (16 * RB) + scales * (8 * D), src + (lane >> 1) * (g.page * RB) + (scales ? g.page * (D / 2) + off * (D / 16) : off * (D / 2)),
+                          scales ? D : 8 * D, full + st);
+            }
+        }
+        seek(false);
+    };
+    seek(true);
+#pragma unroll 1
+    for (int i = 0; i < C::STAGES; i++) fetch();
+
+    // ---- 16 tokens of every tile each
+    const int gr = lane >> 2, c = lane & 3;
+    const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
+    uint32_t it = 0;
+    for (int t = lo; t < hi;) {
+        Segment s;
+        find_segment<NT>(g, prefix, t, hi, s);
+        const int end = seen_tiles<NT>(g, s);
+        const int rows = s.n * g.group;
+
+        uint32_t qf[NT][2 * KW * 2];    // row gr of each n tile, elements of this thread
+        float factor[NT][2];            // score -> log2 units, columns 2c and 2c + 1
+        int limit[NT][2];               // keys that the column sees
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int r = s.rt * NT * 8 + nt * 8 + gr;
+            const int i = r / g.group, h = s.head * g.group + r - i * g.group;
+            uint4 w[KW];
+            uint32_t acc = 0;
+#pragma unroll
+            for (int j = 0; j < KW; j++) {
+                w[j] = r < rows ? ld_v4(g.q + (int64_t)(s.q0 + i) * g.q_token + h * g.q_head + c * (D / 4) + j * 8) : make_uint4(0, 0, 0, 0);
+                acc = absmax2_acc(absmax2_acc(absmax2_acc(absmax2_acc(acc, w[j].x), w[j].y), w[j].z), w[j].w);
+            }
+            uint32_t m = f2u(hmax_halves_f32(acc));
+            m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
+            m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
+            uint32_t e = m >> 23;
+            e = e == 255u ? 134u : max(e, 8u);
+            const float mult = u2f((261u - e) << 23), back = u2f((e - 7u) << 23);
+#pragma unroll
+            for (int j = 0; j < KW; j++) {
+                qf[nt][4 * j] = pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult);
+                qf[nt][4 * j + 1] = pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult);
+                qf[nt][4 * j + 2] = pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult);
+                qf[nt][4 * j + 3] = pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult);
+            }
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                factor[nt][x] = __shfl_sync(0xFFFFFFFFu, back, (2 * c + x) * 4) * (g.scale_log2 * k_outer);
+                const int rc = s.rt * NT * 8 + nt * 8 + 2 * c + x;
+                limit[nt][x] = rc < rows ? s.L - s.n + rc / g.group + 1 : 0;
+            }
+        }
+
+        float o[NT][MT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int i = 0; i < MT; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+            m[nt][0] = m[nt][1] = -INFINITY;
+            l[nt][0] = l[nt][1] = 0.0f;
+        }
+        for (int tile = s.first; tile < end; tile++, it++) {
+            const uint32_t st = it % C::STAGES;
+            mbar_wait(full + st, (it / C::STAGES) & 1, KV_ATTN_ERR);
+            const int tok = tile * SP_TOK + warp * 16;
+            if (tok < s.L) {
+                const uint8_t *kc = ring + st * C::TILE, *ks = kc + 8 * D, *vc = kc + 16 * RB, *vs = vc + 8 * D;
+                float sc[NT][4];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+                {
+                    uint32_t wa[KW], wb[KW], sa[2], sb[2];     // tokens gr and gr + 8
+                    if (D == 128) {
+                        const uint4 a = lds_v4(smem_u32(kc + gr * 64 + c * 16)), b = lds_v4(smem_u32(kc + (gr + 8) * 64 + c * 16));
+                        wa[0] = a.x; wa[1] = a.y; wa[2 % KW] = a.z; wa[3 % KW] = a.w;
+                        wb[0] = b.x; wb[1] = b.y; wb[2 % KW] = b.z; wb[3 % KW] = b.w;
+                        const uint32_t u = *reinterpret_cast<const uint16_t *>(ks + gr * 8 + 2 * c), v = *reinterpret_cast<const uint16_t *>(ks + (gr + 8) * 8 + 2 * c);
+                        sa[0] = e4m3_to_half2(u & 0xFFu); sa[1] = e4m3_to_half2(u >> 8);
+                        sb[0] = e4m3_to_half2(v & 0xFFu); sb[1] = e4m3_to_half2(v >> 8);
+                    } else {
+                        const uint2 a = lds_v2(smem_u32(kc + gr * 32 + c * 8)), b = lds_v2(smem_u32(kc + (gr + 8) * 32 + c * 8));
+                        wa[0] = a.x; wa[1] = a.y;
+                        wb[0] = b.x; wb[1] = b.y;
+                        sa[0] = sa[1] = e4m3_to_half2(ks[gr * 4 + c]);
+                        sb[0] = sb[1] = e4m3_to_half2(ks[(gr + 8) * 4 + c]);
+                    }
+#pragma unroll
+                    for (int j = 0; j < KW; j++) {
+                        uint32_t ha[4], hb[4];
+                        e2m1x8_to_half(wa[j], ha);
+                        e2m1x8_to_half(wb[j], hb);
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            ha[u] = hmul2_bits(ha[u], sa[j * 2 / KW]);
+                            hb[u] = hmul2_bits(hb[u], sb[j * 2 / KW]);
+                        }
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) {
+                            mma16816(sc[nt], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * j], qf[nt][4 * j + 1]);
+                            mma16816(sc[nt], ha[2], hb[2], ha[3], hb[3], qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
+                        }
+                    }
+                }
+                // scores in log2 units; the running maximum moves only when a score is 2^8 above it, so that P stays below 2^8
+                bool grow = false;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int x = 0; x < 4; x++) {
+                        const int key = tok + gr + (x >> 1) * 8;
+                        sc[nt][x] = key < limit[nt][x & 1] ? sc[nt][x] * factor[nt][x & 1] : -INFINITY;
+                        grow |= sc[nt][x] - m[nt][x & 1] > 8.0f;
+                    }
+                }
+                if (__any_sync(0xFFFFFFFFu, grow)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                        for (int x = 0; x < 2; x++) {
+                            float v = fmaxf(sc[nt][x], sc[nt][x + 2]);
+#pragma unroll
+                            for (int sh = 4; sh < 32; sh <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, sh));
+                            v = fmaxf(m[nt][x], v);
+                            const float a = v == -INFINITY ? 1.0f : ex2(m[nt][x] - v);
+                            m[nt][x] = v;
+                            l[nt][x] *= a;
+#pragma unroll
+                            for (int i = 0; i < MT; i++) {
+                                o[nt][i][x] *= a;
+                                o[nt][i][x + 2] *= a;
+                            }
+                        }
+                    }
+                }
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
+                    const float p0 = ex2(sc[nt][0] - m0), p1 = ex2(sc[nt][1] - m1), p2 = ex2(sc[nt][2] - m0), p3 = ex2(sc[nt][3] - m1);
+                    l[nt][0] += p0 + p2;
+                    l[nt][1] += p1 + p3;
+                    pb[nt][0] = transpose8x8(pack_half2(p0, p1));
+                    pb[nt][1] = transpose8x8(pack_half2(p2, p3));
+                }
+                // values of tokens 2c, 2c + 1 and 2c + 8, 2c + 9
+                uint32_t vs2[2], vw[4][VW];
+#pragma unroll
+                for (int x = 0; x < 2; x++) {
+                    const int t0 = 2 * c + 8 * x;
+                    uint32_t s0 = D == 128 ? vs[t0 * 8 + gr] : vs[t0 * 4 + (gr >> 1)], s1 = D == 128 ? vs[t0 * 8 + 8 + gr] : vs[t0 * 4 + 4 + (gr >> 1)];
+                    if (tok + t0 >= s.L) s0 = 0;           // whatever the slots behind the last token hold, it counts as zero
+                    if (tok + t0 + 1 >= s.L) s1 = 0;
+                    const uint32_t two = s0 | (s1 << 8);
+                    asm("{\n.reg .b16 b;\ncvt.u16.u32 b, %1;\ncvt.rn.f16x2.e4m3x2 %0, b;\n}\n" : "=r"(vs2[x]) : "r"(two));
+                    if (D == 128) {
+                        const uint2 a = lds_v2(smem_u32(vc + t0 * 64 + gr * 8)), b = lds_v2(smem_u32(vc + t0 * 64 + 64 + gr * 8));
+                        vw[2 * x][0] = a.x; vw[2 * x][1 % VW] = a.y;
+                        vw[2 * x + 1][0] = b.x; vw[2 * x + 1][1 % VW] = b.y;
+                    } else {
+                        vw[2 * x][0] = *reinterpret_cast<const uint32_t *>(vc + t0 * 32 + gr * 4);
+                        vw[2 * x + 1][0] = *reinterpret_cast<const uint32_t *>(vc + t0 * 32 + 32 + gr * 4);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < VW; j++) {
+                    uint32_t ev[2][4], od[2][4];      // even and odd elements, token pairs
+#pragma unroll
+                    for (int x = 0; x < 2; x++) {
+                        const uint32_t w0 = vw[2 * x][j], w1 = vw[2 * x + 1][j];
+                        e2m1x8_to_half((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), ev[x]);
+                        e2m1x8_to_half(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), od[x]);
+#pragma unroll
+                        for (int u = 0; u < 4; u++) {
+                            ev[x][u] = hmul2_bits(ev[x][u], vs2[x]);
+                            od[x][u] = hmul2_bits(od[x][u], vs2[x]);
+                        }
+                    }
+#pragma unroll
+                    for (int u = 0; u < 4; u++)
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) mma16816(o[nt][4 * j + u], ev[0][u], od[0][u], ev[1][u], od[1][u], pb[nt][0], pb[nt][1]);
+                }
+            }
+            __syncwarp();      // all lanes have read the stage that the next fetch overwrites
+            fetch();
+        }
+
+        // ---- join the warps, then write the unit's result or this CTA's partial sums
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+#pragma unroll
+                for (int sh = 4; sh < 32; sh <<= 1) l[nt][x] += __shfl_xor_sync(0xFFFFFFFFu, l[nt][x], sh);
+                if (gr == 0) ml[warp * NT * 8 + nt * 8 + 2 * c + x] = make_float2(m[nt][x], l[nt][x]);
+            }
+        named_barrier(1, SP_WARPS * 32);
+        const bool whole = s.first == 0 && t + s.last - s.first == s.unit_last;
+        float *slot = g.part + (size_t)(2 * blockIdx.x + (t == lo ? 0 : 1)) * part_floats<D, NT>();
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int x = 0; x < 2; x++) {
+                float top = -INFINITY;
+                for (int w = 0; w < SP_WARPS; w++) top = fmaxf(top, ml[w * NT * 8 + nt * 8 + 2 * c + x].x);
+                const float a = m[nt][x] == -INFINITY ? 1.0f : ex2(m[nt][x] - top);      // an empty warp holds zeros (or NaN, which stays)
+#pragma unroll
+                for (int i = 0; i < MT; i++) {
+                    o[nt][i][x] *= a;
+                    o[nt][i][x + 2] *= a;
+                }
+            }
+        constexpr int DQ = D / 4, PER = MT / 4;        // elements and m tiles of one round
+#pragma unroll
+        for (int round = 0; round < 4; round++) {
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int i = 0; i < PER; i++)
+#pragma unroll
+                    for (int x = 0; x < 4; x++)
+                        red[(warp * NT * 8 + nt * 8 + 2 * c + (x & 1)) * DQ + gr * (2 * PER) + 2 * i + (x >> 1)] = o[nt][round * PER + i][x];
+            named_barrier(1, SP_WARPS * 32);
+            for (int e = threadIdx.x; e < NT * 8 * DQ; e += SP_WARPS * 32) {
+                const int qi = e / DQ, x = e - qi * DQ;
+                const int d = (x / (2 * PER)) * (4 * 2 * PER) + round * 2 * PER + x % (2 * PER);
+                float sum = 0.0f, top = -INFINITY, den = 0.0f;
+                for (int w = 0; w < SP_WARPS; w++) {
+                    sum += red[(w * NT * 8 + qi) * DQ + x];
+                    top = fmaxf(top, ml[w * NT * 8 + qi].x);
+                }
+                for (int w = 0; w < SP_WARPS; w++) {
+                    const float2 v = ml[w * NT * 8 + qi];
+                    den += v.y * (v.x == -INFINITY ? 1.0f : ex2(v.x - top));
+                }
+                if (whole) {
+                    const int r = s.rt * NT * 8 + qi;
+                    if (r < rows) {
+                        const int i = r / g.group;
+                        const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + s.head * g.group + r - i * g.group;
+                        const __nv_bfloat16 y = __float2bfloat16_rn(den == 0.0f ? 0.0f : __fdividef(sum * v_outer, den));
+                        g.out[at * D + d] = *reinterpret_cast<const uint16_t *>(&y);
+                        if (round == 0 && x == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
+                    }
+                } else {
+                    slot[qi * (D + 2) + 2 + d] = sum;
+                    if (round == 0 && x == 0) {
+                        slot[qi * (D + 2)] = top;
+                        slot[qi * (D + 2) + 1] = den;
+                    }
+                }
+            }
+            named_barrier(1, SP_WARPS * 32);
+        }
+        t += s.last - s.first;
+    }
+}
+
+// One CTA per unit (sequence, head, row tile): joins the partial sums of a unit that several CTAs worked on, in the order of
+// its tokens, and fills the rows of a unit without tokens.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) kv_attn_join_kernel(const AttnArgs g, int grid, int max_rts, int units)
+{
+    pdl_wait();
+    if ((int)blockIdx.x >= units) {
+        // rows behind the last sequence
+        const int64_t first = (int64_t)max(__ldg(g.cu_q + g.seqs), 0) * g.q_heads, n = g.rows * g.q_heads;
+        for (int64_t r = first + blockIdx.x - units; r < n; r += gridDim.x - units) {
+            for (int d = threadIdx.x; d < D; d += 128) g.out[r * D + d] = 0;
+            if (threadIdx.x == 0 && g.lse) g.lse[r] = -INFINITY;
+        }
+        return;
+    }
+    const int rt = blockIdx.x % max_rts, head = blockIdx.x / max_rts % g.kv_heads, b = blockIdx.x / max_rts / g.kv_heads;
+    int q0, n, L;
+    seq_of(g, b, q0, n, L);
+    const int rows = n * g.group, rts = (rows + NT * 8 - 1) / (NT * 8), kvt = (L + SP_TOK - 1) / SP_TOK;
+    if (rt >= rts) return;
+    const int total = g.prefix[g.seqs], ctas = min(grid, total);
+    const float v_outer = __ldg(g.v_outer);
+    int i0 = 0, i1 = -1, first = 0;
+    if (kvt > 0) {
+        first = g.prefix[b] + (head * rts + rt) * kvt;
+        // CTA i works on tiles [total * i / ctas, total * (i + 1) / ctas): tile t belongs to ((t + 1) * ctas - 1) / total
+        i0 = (int)((((int64_t)first + 1) * ctas - 1) / total);
+        i1 = (int)((((int64_t)first + kvt) * ctas - 1) / total);
+        if (i0 == i1) return;
+    }
+    const int slot0 = kvt > 0 && (int)((int64_t)total * i0 / ctas) < first ? 1 : 0;    // the unit is not the first of its first CTA
+    for (int e = threadIdx.x; e < NT * 8 * D; e += 128) {
+        const int qi = e / D, d = e - qi * D, r = rt * NT * 8 + qi;
+        if (r >= rows) break;
+        float top = -INFINITY, den = 0.0f, sum = 0.0f;
+        for (int i = i0; i <= i1; i++)
+            top = fmaxf(top, g.part[(size_t)(2 * i + (i == i0 ? slot0 : 0)) * part_floats<D, NT>() + qi * (D + 2)]);
+        for (int i = i0; i <= i1; i++) {
+            const float *p = g.part + (size_t)(2 * i + (i == i0 ? slot0 : 0)) * part_floats<D, NT>() + qi * (D + 2);
+            const float a = p[0] == -INFINITY ? 1.0f : ex2(p[0] - top);
+            den += p[1] * a;
+            sum += p[2 + d] * a;
+        }
+        const int i = r / g.group;
+        const int64_t at = (int64_t)(q0 + i) * g.q_heads + head * g.group + r - i * g.group;
+        const __nv_bfloat16 y = __float2bfloat16_rn(den == 0.0f ? 0.0f : __fdividef(sum * v_outer, den));
+        g.out[at * D + d] = *reinterpret_cast<const uint16_t *>(&y);
+        if (d == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
+    }
+}
+
+template <int D, int NT>
+static int split_launch(const AttnArgs &g, int max_q, cudaStream_t st)
+{
+    using C = SplitCfg<D, NT>;
+    static PerDeviceFlag done;
+    const int dev = current_device_slot();
+    if (dev < 0) return QCC_ERR_ARG;
+    if (!done.get(dev)) {
+        cudaError_t e = cudaFuncSetAttribute(kv_attn_split_kernel<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::FIXED + (KV_MAX_SEQS + 1) * 4);
+        if (e != cudaSuccess) return (int)e;
+        done.set(dev);
+    }
+    const int grid = sm_count() * C::CTAS;
+    kv_attn_split_kernel<D, NT><<<grid, SP_THREADS, C::FIXED + (g.seqs + 1) * 4, st>>>(g);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    const int max_rts = (int)(((int64_t)max_q * g.group + NT * 8 - 1) / (NT * 8));
+    const int units = g.seqs * g.kv_heads * max_rts;
+    const int behind = g.cu_q ? 32 : 0;      // CTAs for the rows behind the last sequence
+    return (int)launch_maybe_pdl(kv_attn_join_kernel<D, NT>, dim3((unsigned)(units + behind)), dim3(128), 0, st, true, g, grid, max_rts, units);
+}
+
+// how the rows of a sequence and kv head are tiled: 8 * nt rows
+static int row_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+
+}  // namespace qcc
+
+using namespace qcc;
+
+extern "C" int qcc_kv_attention_device_error(unsigned int *out) { return read_clear_device_error(out); }
+
+extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int seqs, int max_q, int q_heads, int kv_heads, int head_dim)
+{
+    if (seqs < 0 || max_q < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+    const int nt = row_tiles_of((int64_t)max_q * (q_heads / kv_heads));
+    const size_t prefix = (((size_t)seqs + 1) * 4 + 15) / 16 * 16;
+    return prefix + (size_t)2 * sm_count() * (nt == 1 ? 2 : 1) * nt * 8 * (head_dim + 2) * 4;
+}
+
+extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *workspace, size_t workspace_bytes, void *stream)
+{
+    if (!p) return QCC_ERR_ARG;
+    if ((p->head_dim != 64 && p->head_dim != 128) || p->kv_heads < 1 || p->q_heads < p->kv_heads || p->q_heads % p->kv_heads || p->q_heads > 4096)
+        return QCC_ERR_SHAPE;
+    if ((p->page != 16 && p->page != 32 && p->page != 64 && p->page != 128) || p->seqs < 0 || p->seqs > KV_MAX_SEQS || p->rows < 0 || p->max_q < 1 ||
+        p->num_pages < 0 || p->table_width < 0 || p->table_stride < 0 || (int64_t)p->table_width * p->page > 0x40000000)
+        return QCC_ERR_SHAPE;
+    if (p->seqs == 0 || p->rows == 0) return 0;
+    if (!p->cu_q && p->rows != p->seqs) return QCC_ERR_SHAPE;
+    if (!p->q || !p->cache || !p->kv_lens || !p->k_outer || !p->v_outer || !p->out || (!p->table && p->table_width > 0)) return QCC_ERR_ARG;
+    if (!aligned16(p->q) || !aligned16(p->cache) || !aligned16(p->out) || (p->q_stride[0] | p->q_stride[1]) % 8 != 0) return QCC_ERR_ALIGN;
+    const int group = p->q_heads / p->kv_heads, max_q = p->cu_q ? p->max_q : 1, nt = row_tiles_of((int64_t)max_q * group);
+    const int64_t rts = ((int64_t)max_q * group + nt * 8 - 1) / (nt * 8), kvt = ((int64_t)p->table_width * p->page + SP_TOK - 1) / SP_TOK;
+    if (rts * p->kv_heads * p->seqs > 0x7FFFFF00 || rts * p->kv_heads * p->seqs * (kvt + 1) > 0x7FFFFFFF) return QCC_ERR_SHAPE;
+    if (!workspace || workspace_bytes < qcc_nvfp4_kv_attention_workspace_bytes(p->seqs, max_q, p->q_heads, p->kv_heads, p->head_dim)) return QCC_ERR_WORKSPACE;
+    if (!aligned16(workspace)) return QCC_ERR_ALIGN;
+    AttnArgs g;
+    g.q = static_cast<const uint16_t *>(p->q);
+    g.cache = static_cast<const uint8_t *>(p->cache);
+    g.table = p->table; g.kv_lens = p->kv_lens; g.cu_q = p->cu_q;
+    g.k_outer = p->k_outer; g.v_outer = p->v_outer;
+    g.out = static_cast<uint16_t *>(p->out);
+    g.lse = p->lse;
+    g.prefix = static_cast<int32_t *>(workspace);
+    g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + (((size_t)p->seqs + 1) * 4 + 15) / 16 * 16);
+    g.q_token = p->q_stride[0]; g.q_head = p->q_stride[1];
+    g.table_stride = p->table_stride; g.num_pages = p->num_pages; g.rows = p->rows;
+    g.scale_log2 = p->scale * LOG2E;
+    g.seqs = p->seqs; g.width = p->table_width; g.q_heads = p->q_heads; g.kv_heads = p->kv_heads; g.group = group; g.page = p->page; g.max_q = max_q;
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (p->head_dim == 128)
+        return nt == 1 ? split_launch<128, 1>(g, max_q, st) : nt == 2 ? split_launch<128, 2>(g, max_q, st) : split_launch<128, 4>(g, max_q, st);
+    return nt == 1 ? split_launch<64, 1>(g, max_q, st) : nt == 2 ? split_launch<64, 2>(g, max_q, st) : split_launch<64, 4>(g, max_q, st);
+}

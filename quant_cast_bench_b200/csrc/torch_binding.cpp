@@ -22,6 +22,12 @@
 //   mxfp4(x, swizzle)                                       -> (q (M, N/2), scale)
 //   nvfp4_per_token_scale(x, recip_div)                     -> (M, 1) fp32 outer scales
 //   sr_f32_to_bf16(x, key, global_row, global_col, num_col) -> bf16       fp32 input, stochastic rounding
+//   int8_rowwise(x, recip_div)                              -> (q int8, scale (M, 1))
+//   int8_scaled_mm(a, b, scale_a, scale_b, bias, out_dtype) -> (a @ b.T) * scale_a * scale_b.T + bias   exact int32 sums
+//   nvfp4_kv_append(k, v, cache, slots, k_outer, v_outer, positions, cos_sin, interleaved, q, recip_div) -> rotated q (empty
+//                                                               without q); writes the cache
+//   nvfp4_kv_gather(cache, block_table, cu_kv, total, head_dim, k_outer, v_outer) -> (k, v) bf16
+//   nvfp4_kv_attention(q, cache, block_table, kv_lens, k_outer, v_outer, cu_q, max_q, scale) -> (out, lse)
 //
 // recip_div: QCC_RECIP_DIV (divisions by a constant as eager PyTorch computes them on a CUDA device).
 // Built by quant_cast_bench_b200/build.py into lib/libquant_cast_torch.so, which links against libquant_cast_cuda.so.
@@ -30,6 +36,10 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <cmath>
+#include <limits>
+#include <optional>
 #include <string>
 #include <tuple>
 #include <vector>
@@ -339,6 +349,222 @@ at::Tensor sr_f32_to_bf16_cuda(const at::Tensor &x, const at::Tensor &key, int64
     return out;
 }
 
+// ---- int8 linear layer
+void check_codes(const at::Tensor &t, const char *what)
+{
+    TORCH_CHECK(t.dim() == 2 && t.scalar_type() == at::kChar, "quant_cast_cuda: ", what, " must be 2-D int8");
+}
+void check_product(const at::Tensor &a, const at::Tensor &b)
+{
+    check_codes(a, "a");
+    check_codes(b, "b");
+    const int64_t K = a.size(1);
+    TORCH_CHECK(b.size(1) == K, "quant_cast_cuda: a has ", K, " columns, b ", b.size(1));
+    TORCH_CHECK(K % 16 == 0 && K >= 16 && K <= QCC_INT8_MAX_K, "quant_cast_cuda: int8_scaled_mm needs K % 16 == 0 and 16 <= K <= ", QCC_INT8_MAX_K, ", got ", K);
+}
+int out_kind(at::ScalarType t)
+{
+    TORCH_CHECK(t == at::kBFloat16 || t == at::kHalf || t == at::kFloat, "quant_cast_cuda: out_dtype must be bfloat16, float16 or float32");
+    return t == at::kBFloat16 ? QCC_OUT_BF16 : t == at::kHalf ? QCC_OUT_F16 : QCC_OUT_F32;
+}
+
+std::tuple<at::Tensor, at::Tensor> int8_rowwise_cuda(const at::Tensor &x, bool recip_div)
+{
+    check_x_cuda(x);
+    TORCH_CHECK(x.size(1) >= 1, "quant_cast_cuda: int8_rowwise needs at least one column");
+    const c10::cuda::CUDAGuard guard(x.device());
+    at::Tensor q = at::empty(x.sizes(), x.options().dtype(at::kChar)), s = at::empty({x.size(0), 1}, x.options().dtype(at::kFloat));
+    ok(qcc_int8_rowwise(x.data_ptr(), x.size(0), x.size(1), recip_div ? QCC_RECIP_DIV : 0, q.data_ptr(), s.data_ptr<float>(), stream_of(x)), "int8_rowwise");
+    return {q, s};
+}
+
+at::Tensor int8_scaled_mm_cuda(const at::Tensor &a, const at::Tensor &b, const at::Tensor &scale_a, const at::Tensor &scale_b,
+                               const std::optional<at::Tensor> &bias, at::ScalarType out_dtype)
+{
+    check_product(a, b);
+    TORCH_CHECK(a.is_cuda() && a.is_contiguous() && b.is_contiguous(), "quant_cast_cuda: a and b must be contiguous CUDA tensors (there is no CPU implementation)");
+    const int64_t M = a.size(0), K = a.size(1), N = b.size(0);
+    TORCH_CHECK(scale_a.scalar_type() == at::kFloat && scale_a.numel() == M && scale_a.is_contiguous() && scale_b.scalar_type() == at::kFloat &&
+                    scale_b.numel() == N && scale_b.is_contiguous(),
+                "quant_cast_cuda: scale_a and scale_b must be contiguous fp32, one value a row of a and of b");
+    same_device(a, b, "b");
+    same_device(a, scale_a, "scale_a");
+    same_device(a, scale_b, "scale_b");
+    if (bias) {
+        TORCH_CHECK(bias->scalar_type() == at::kBFloat16 && bias->numel() == N && bias->is_contiguous(), "quant_cast_cuda: bias must be N contiguous bfloat16 values");
+        same_device(a, *bias, "bias");
+    }
+    const int kind = out_kind(out_dtype);
+    const c10::cuda::CUDAGuard guard(a.device());
+    at::Tensor out = at::empty({M, N}, a.options().dtype(out_dtype));
+    ok(qcc_int8_scaled_mm(a.data_ptr(), b.data_ptr(), M, N, K, scale_a.data_ptr<float>(), scale_b.data_ptr<float>(), bias ? bias->data_ptr() : nullptr, kind,
+                          out.data_ptr(), stream_of(a)),
+       "int8_scaled_mm");
+    return out;
+}
+
+// ---- paged nvfp4 key/value cache
+struct CacheShape {
+    int heads, page;
+};
+CacheShape check_cache(const at::Tensor &cache, int64_t head_dim)
+{
+    TORCH_CHECK(head_dim == 64 || head_dim == 128, "quant_cast_cuda: head_dim must be 64 or 128");
+    TORCH_CHECK(cache.is_cuda() && cache.scalar_type() == at::kByte && cache.dim() == 4 && cache.size(2) == 2 && cache.is_contiguous(),
+                "quant_cast_cuda: cache must be a contiguous CUDA uint8 tensor (pages, kv_heads, 2, page * 9 * head_dim / 16)");
+    const int64_t unit = 9 * head_dim / 16, page = cache.size(3) / unit;
+    TORCH_CHECK(cache.size(3) % unit == 0 && (page == 16 || page == 32 || page == 64 || page == 128) && cache.size(1) >= 1 && cache.size(1) <= 4096,
+                "quant_cast_cuda: a page block of ", cache.size(3), " bytes is no page of 16, 32, 64 or 128 tokens");
+    return {(int)cache.size(1), (int)page};
+}
+void check_rows(const at::Tensor &t, const at::Tensor &cache, const char *what)
+{
+    TORCH_CHECK(t.dim() == 3 && t.scalar_type() == at::kBFloat16, "quant_cast_cuda: ", what, " must be 3-D bfloat16");
+    same_device(cache, t, what);
+    TORCH_CHECK(t.stride(2) == 1 && (t.numel() == 0 || (t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0)),
+                "quant_cast_cuda: rows of ", what, " must be contiguous and 16-byte aligned");
+}
+const float *outer_of(const at::Tensor &t, const at::Tensor &cache, const char *what)
+{
+    TORCH_CHECK(t.scalar_type() == at::kFloat && t.numel() == 1, "quant_cast_cuda: ", what, " must be one fp32 value");
+    same_device(cache, t, what);
+    return t.data_ptr<float>();
+}
+void check_numbers(const at::Tensor &t, at::ScalarType dt, int64_t n, const at::Tensor &cache, const char *what)
+{
+    TORCH_CHECK(t.scalar_type() == dt && t.dim() == 1 && t.size(0) == n && t.is_contiguous(), "quant_cast_cuda: ", what, " must be ", n, " contiguous ", dt, " values");
+    same_device(cache, t, what);
+}
+void check_table(const at::Tensor &t, const at::Tensor &cache)
+{
+    TORCH_CHECK(t.scalar_type() == at::kInt && t.dim() == 2 && (t.size(1) <= 1 || t.stride(1) == 1) && t.stride(0) >= 0 && t.size(1) <= 0x7FFFFFFF && t.size(0) <= 0x7FFFFFFE,
+                "quant_cast_cuda: block_table must be int32 (seqs, pages) with contiguous rows");
+    same_device(cache, t, "block_table");
+}
+
+at::Tensor nvfp4_kv_append_cuda(const at::Tensor &k, const at::Tensor &v, at::Tensor cache, const at::Tensor &slots, const at::Tensor &k_outer,
+                                const at::Tensor &v_outer, const std::optional<at::Tensor> &positions, const std::optional<at::Tensor> &cos_sin,
+                                bool interleaved, const std::optional<at::Tensor> &q, bool recip_div)
+{
+    TORCH_CHECK(k.dim() == 3, "quant_cast_cuda: k must be (tokens, kv_heads, head_dim)");
+    const int64_t T = k.size(0), D = k.size(2);
+    const CacheShape c = check_cache(cache, D);
+    check_rows(k, cache, "k");
+    check_rows(v, cache, "v");
+    TORCH_CHECK(v.sizes() == k.sizes() && k.size(1) == c.heads, "quant_cast_cuda: k and v must have the cache's heads and one shape");
+    check_numbers(slots, at::kLong, T, cache, "slots");
+    qcc_kv_append_args a = {};
+    a.k_outer = outer_of(k_outer, cache, "k_outer");
+    a.v_outer = outer_of(v_outer, cache, "v_outer");
+    if (cos_sin) {
+        TORCH_CHECK(cos_sin->scalar_type() == at::kFloat && cos_sin->dim() == 2 && cos_sin->is_contiguous() && cos_sin->size(0) > 0 && cos_sin->size(1) > 0 &&
+                        cos_sin->size(1) <= D && cos_sin->size(1) % 32 == 0,
+                    "quant_cast_cuda: cos_sin must be contiguous fp32 (max_pos, rot) with rot a multiple of 32 up to ", D);
+        same_device(cache, *cos_sin, "cos_sin");
+        TORCH_CHECK(positions.has_value(), "quant_cast_cuda: a rotation needs positions");
+        check_numbers(*positions, at::kLong, T, cache, "positions");
+        a.cos_sin = cos_sin->data_ptr<float>();
+        a.positions = positions->data_ptr<int64_t>();
+        a.max_pos = cos_sin->size(0);
+        a.rot = (int)cos_sin->size(1);
+    }
+    const c10::cuda::CUDAGuard guard(cache.device());
+    at::Tensor out = at::empty({q ? T : 0, q ? q->size(1) : 0, D}, k.options());
+    if (q) {
+        check_rows(*q, cache, "q");
+        TORCH_CHECK(q->size(0) == T && q->size(2) == D && q->size(1) <= 4096, "quant_cast_cuda: q must have k's tokens and head_dim");
+        a.q = q->data_ptr();
+        a.q_out = out.data_ptr();
+        a.q_heads = (int)q->size(1);
+        a.q_stride[0] = q->stride(0);
+        a.q_stride[1] = q->stride(1);
+    }
+    if (T == 0) return out;
+    a.k = k.data_ptr();
+    a.v = v.data_ptr();
+    a.k_stride[0] = k.stride(0); a.k_stride[1] = k.stride(1);
+    a.v_stride[0] = v.stride(0); a.v_stride[1] = v.stride(1);
+    a.tokens = T;
+    a.cache = cache.data_ptr();
+    a.num_pages = cache.size(0);
+    a.slots = slots.data_ptr<int64_t>();
+    a.kv_heads = c.heads;
+    a.head_dim = (int)D;
+    a.page = c.page;
+    a.flags = (interleaved ? QCC_ROPE_INTERLEAVED : 0) | (recip_div ? QCC_RECIP_DIV : 0);
+    ok(qcc_nvfp4_kv_append(&a, stream_of(cache)), "nvfp4_kv_append");
+    return out;
+}
+
+std::tuple<at::Tensor, at::Tensor> nvfp4_kv_gather_cuda(const at::Tensor &cache, const at::Tensor &block_table, const at::Tensor &cu_kv, int64_t total,
+                                                        int64_t head_dim, const at::Tensor &k_outer, const at::Tensor &v_outer)
+{
+    const CacheShape c = check_cache(cache, head_dim);
+    check_table(block_table, cache);
+    check_numbers(cu_kv, at::kInt, block_table.size(0) + 1, cache, "cu_kv");
+    const float *ko = outer_of(k_outer, cache, "k_outer"), *vo = outer_of(v_outer, cache, "v_outer");
+    TORCH_CHECK(total >= 0, "quant_cast_cuda: total must not be negative");
+    const c10::cuda::CUDAGuard guard(cache.device());
+    at::Tensor k = at::empty({total, c.heads, head_dim}, cache.options().dtype(at::kBFloat16)), v = at::empty_like(k);
+    ok(qcc_nvfp4_kv_gather(cache.data_ptr(), cache.size(0), c.heads, c.page, (int)head_dim, block_table.data_ptr<int32_t>(), block_table.stride(0),
+                           (int)block_table.size(1), cu_kv.data_ptr<int32_t>(), (int)block_table.size(0), total, ko, vo, k.data_ptr(), v.data_ptr(), stream_of(cache)),
+       "nvfp4_kv_gather");
+    return {k, v};
+}
+
+std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_cuda(const at::Tensor &q, const at::Tensor &cache, const at::Tensor &block_table, const at::Tensor &kv_lens,
+                                                           const at::Tensor &k_outer, const at::Tensor &v_outer, const std::optional<at::Tensor> &cu_q,
+                                                           int64_t max_q, double scale)
+{
+    TORCH_CHECK(q.dim() == 3, "quant_cast_cuda: q must be (rows, q_heads, head_dim)");
+    const int64_t rows = q.size(0), hq = q.size(1), D = q.size(2), seqs = block_table.size(0);
+    const CacheShape c = check_cache(cache, D);
+    check_rows(q, cache, "q");
+    TORCH_CHECK(hq >= c.heads && hq % c.heads == 0 && hq <= 4096, "quant_cast_cuda: ", hq, " query heads do not divide among ", c.heads, " kv heads");
+    check_table(block_table, cache);
+    check_numbers(kv_lens, at::kInt, seqs, cache, "kv_lens");
+    qcc_kv_attention_args a = {};
+    a.k_outer = outer_of(k_outer, cache, "k_outer");
+    a.v_outer = outer_of(v_outer, cache, "v_outer");
+    if (cu_q) {
+        check_numbers(*cu_q, at::kInt, seqs + 1, cache, "cu_q");
+        TORCH_CHECK(max_q >= 1 && max_q <= 0x7FFFFFFF, "quant_cast_cuda: cu_q needs max_q >= 1");
+    } else {
+        TORCH_CHECK(rows == seqs, "quant_cast_cuda: ", rows, " query rows for ", seqs, " sequences: several queries a sequence need cu_q");
+        max_q = 1;
+    }
+    const c10::cuda::CUDAGuard guard(cache.device());
+    at::Tensor out = at::empty({rows, hq, D}, q.options()), lse = at::empty({rows, hq}, q.options().dtype(at::kFloat));
+    if (rows == 0 || seqs == 0) {
+        out.zero_();
+        lse.fill_(-std::numeric_limits<float>::infinity());
+        return {out, lse};
+    }
+    const size_t ws_bytes = qcc_nvfp4_kv_attention_workspace_bytes((int)std::min<int64_t>(seqs, 1 << 20), (int)max_q, (int)hq, c.heads, (int)D);
+    at::Tensor ws = at::empty({(int64_t)ws_bytes}, cache.options());
+    a.q = q.data_ptr();
+    a.q_stride[0] = q.stride(0); a.q_stride[1] = q.stride(1);
+    a.rows = rows;
+    a.cache = cache.data_ptr();
+    a.num_pages = cache.size(0);
+    a.table = block_table.data_ptr<int32_t>();
+    a.table_stride = block_table.stride(0);
+    a.table_width = (int)block_table.size(1);
+    a.kv_lens = kv_lens.data_ptr<int32_t>();
+    a.cu_q = cu_q ? cu_q->data_ptr<int32_t>() : nullptr;
+    a.seqs = (int)std::min<int64_t>(seqs, 1 << 20);
+    a.max_q = (int)max_q;
+    a.scale = scale > 0 ? (float)scale : (float)(1.0 / std::sqrt((double)D));
+    a.q_heads = (int)hq;
+    a.kv_heads = c.heads;
+    a.head_dim = (int)D;
+    a.page = c.page;
+    a.out = out.data_ptr();
+    a.lse = lse.data_ptr<float>();
+    ok(qcc_nvfp4_kv_attention(&a, ws.data_ptr(), ws_bytes, stream_of(cache)), "nvfp4_kv_attention");
+    return {out, lse};
+}
+
 // ---------------------------------------------------------------------------------------- Meta (shape) implementations
 at::Tensor like(const at::Tensor &x, std::vector<int64_t> shape, at::ScalarType dt) { return at::empty(shape, x.options().dtype(dt)); }
 
@@ -444,6 +670,36 @@ at::Tensor sr_f32_to_bf16_meta(const at::Tensor &x, const at::Tensor &, int64_t,
     return like(x, x.sizes().vec(), at::kBFloat16);
 }
 
+std::tuple<at::Tensor, at::Tensor> int8_rowwise_meta(const at::Tensor &x, bool)
+{
+    check_x(x);
+    return {like(x, {x.size(0), x.size(1)}, at::kChar), like(x, {x.size(0), 1}, at::kFloat)};
+}
+at::Tensor int8_scaled_mm_meta(const at::Tensor &a, const at::Tensor &b, const at::Tensor &, const at::Tensor &, const std::optional<at::Tensor> &, at::ScalarType out_dtype)
+{
+    check_product(a, b);
+    out_kind(out_dtype);
+    return like(a, {a.size(0), b.size(0)}, out_dtype);
+}
+at::Tensor nvfp4_kv_append_meta(const at::Tensor &k, const at::Tensor &, at::Tensor, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                const std::optional<at::Tensor> &, const std::optional<at::Tensor> &, bool, const std::optional<at::Tensor> &q, bool)
+{
+    TORCH_CHECK(k.dim() == 3 && (!q || q->dim() == 3), "quant_cast_cuda: k and q must be 3-D");
+    return like(k, {q ? k.size(0) : 0, q ? q->size(1) : 0, k.size(2)}, at::kBFloat16);
+}
+std::tuple<at::Tensor, at::Tensor> nvfp4_kv_gather_meta(const at::Tensor &cache, const at::Tensor &, const at::Tensor &, int64_t total, int64_t head_dim,
+                                                        const at::Tensor &, const at::Tensor &)
+{
+    TORCH_CHECK(cache.dim() == 4, "quant_cast_cuda: cache must be 4-D");
+    return {like(cache, {total, cache.size(1), head_dim}, at::kBFloat16), like(cache, {total, cache.size(1), head_dim}, at::kBFloat16)};
+}
+std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_meta(const at::Tensor &q, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
+                                                           const at::Tensor &, const std::optional<at::Tensor> &, int64_t, double)
+{
+    TORCH_CHECK(q.dim() == 3, "quant_cast_cuda: q must be (rows, q_heads, head_dim)");
+    return {like(q, q.sizes().vec(), at::kBFloat16), like(q, {q.size(0), q.size(1)}, at::kFloat)};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(quant_cast_cuda_native, m)
@@ -463,6 +719,13 @@ TORCH_LIBRARY(quant_cast_cuda_native, m)
     m.def("mxfp8_32x32(Tensor x, bool rowwise, bool colwise, bool swizzle, bool transposed_data=True) -> Tensor[]");
     m.def("mxfp4(Tensor x, bool swizzle) -> (Tensor, Tensor)");
     m.def("nvfp4_per_token_scale(Tensor x, bool recip_div=False) -> Tensor");
+    m.def("int8_rowwise(Tensor x, bool recip_div=False) -> (Tensor, Tensor)");
+    m.def("int8_scaled_mm(Tensor a, Tensor b, Tensor scale_a, Tensor scale_b, Tensor? bias=None, ScalarType out_dtype=bfloat16) -> Tensor");
+    m.def("nvfp4_kv_append(Tensor k, Tensor v, Tensor(a!) cache, Tensor slots, Tensor k_outer, Tensor v_outer, Tensor? positions=None, "
+          "Tensor? cos_sin=None, bool interleaved=False, Tensor? q=None, bool recip_div=False) -> Tensor");
+    m.def("nvfp4_kv_gather(Tensor cache, Tensor block_table, Tensor cu_kv, int total, int head_dim, Tensor k_outer, Tensor v_outer) -> (Tensor, Tensor)");
+    m.def("nvfp4_kv_attention(Tensor q, Tensor cache, Tensor block_table, Tensor kv_lens, Tensor k_outer, Tensor v_outer, Tensor? cu_q=None, "
+          "int max_q=1, float scale=0.) -> (Tensor, Tensor)");
     m.def("sr_f32_to_bf16(Tensor x, Tensor key, int global_row=0, int global_col=0, int num_col=-1) -> Tensor");
 }
 
@@ -483,6 +746,11 @@ TORCH_LIBRARY_IMPL(quant_cast_cuda_native, CUDA, m)
     m.impl("mxfp8_32x32", mxfp8_32x32_cuda);
     m.impl("mxfp4", mxfp4_cuda);
     m.impl("nvfp4_per_token_scale", nvfp4_per_token_scale_cuda);
+    m.impl("int8_rowwise", int8_rowwise_cuda);
+    m.impl("int8_scaled_mm", int8_scaled_mm_cuda);
+    m.impl("nvfp4_kv_append", nvfp4_kv_append_cuda);
+    m.impl("nvfp4_kv_gather", nvfp4_kv_gather_cuda);
+    m.impl("nvfp4_kv_attention", nvfp4_kv_attention_cuda);
     m.impl("sr_f32_to_bf16", sr_f32_to_bf16_cuda);
 }
 
@@ -503,5 +771,10 @@ TORCH_LIBRARY_IMPL(quant_cast_cuda_native, Meta, m)
     m.impl("mxfp8_32x32", mxfp8_32x32_meta);
     m.impl("mxfp4", mxfp4_meta);
     m.impl("nvfp4_per_token_scale", nvfp4_per_token_scale_meta);
+    m.impl("int8_rowwise", int8_rowwise_meta);
+    m.impl("int8_scaled_mm", int8_scaled_mm_meta);
+    m.impl("nvfp4_kv_append", nvfp4_kv_append_meta);
+    m.impl("nvfp4_kv_gather", nvfp4_kv_gather_meta);
+    m.impl("nvfp4_kv_attention", nvfp4_kv_attention_meta);
     m.impl("sr_f32_to_bf16", sr_f32_to_bf16_meta);
 }

@@ -13,6 +13,9 @@ LIB_PATH = os.path.join(os.path.dirname(_HERE), "lib", "libquant_cast_cuda.so")
 FMT_E4M3, FMT_E5M2 = 0, 1
 ROWWISE, COLWISE, SWIZZLE, FLOOR, SR, BLOCK32 = 1, 2, 4, 8, 16, 32
 PDL, REVERSE = 0x200, 0x400
+ROPE_INTERLEAVED = 0x2000
+OUT_BF16, OUT_F16, OUT_F32 = 0, 1, 2
+INT8_MAX_K = 131056
 XCHG_PUBLISH, XCHG_PDL = 1, 2
 AMAX_RAW, AMAX_FP8_SCALE, AMAX_NVFP4_SCALE = 0, 1, 2
 AMAX_ONE_LAUNCH = 0x100
@@ -77,6 +80,13 @@ SIGNATURES = {
     "qcc_nvfp4_per_token_scale": (_int, [_vp, _i64, _i64, _int, _vp, _vp]),
     "qcc_fp8_block128x128": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _vp]),
     "qcc_amax_block128x128": (_int, [_vp, _i64, _i64, _int, _vp, _vp]),
+    "qcc_int8_rowwise": (_int, [_vp, _i64, _i64, _int, _vp, _vp, _vp]),
+    "qcc_int8_scaled_mm": (_int, [_vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp]),
+    "qcc_nvfp4_kv_page_bytes": (_sz, [_int, _int, _int]),
+    "qcc_nvfp4_kv_append": (_int, [_vp, _vp]),
+    "qcc_nvfp4_kv_gather": (_int, [_vp, _i64, _int, _int, _int, _vp, _i64, _int, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp]),
+    "qcc_nvfp4_kv_attention_workspace_bytes": (_sz, [_int, _int, _int, _int, _int]),
+    "qcc_nvfp4_kv_attention": (_int, [_vp, _vp, _sz, _vp]),
     "qcc_hadamard_rht": (_int, [_vp, _i64, _i64, _vp, _vp, _vp]),
     "qcc_nvfp4_rht_amax": (_int, [_vp, _i64, _i64, _vp, _int, _vp, _vp]),
     "qcc_nvfp4_rht": (_int, [_vp, _i64, _i64, _vp, _vp, _vp, _int, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
@@ -90,6 +100,21 @@ class XchgRef(ctypes.Structure):
     """qcc_xchg_ref of include/quant_cast_cuda.h"""
     _fields_ = [("states", ctypes.POINTER(ctypes.c_void_p)), ("world", ctypes.c_int), ("rank", ctypes.c_int),
                 ("publish", ctypes.c_int)]
+
+
+class KvAppendArgs(ctypes.Structure):
+    """qcc_kv_append_args of include/quant_cast_cuda.h"""
+    _fields_ = [("k", _vp), ("v", _vp), ("q", _vp), ("q_out", _vp), ("k_stride", _i64 * 2), ("v_stride", _i64 * 2), ("q_stride", _i64 * 2),
+                ("tokens", _i64), ("cache", _vp), ("num_pages", _i64), ("slots", _vp), ("positions", _vp), ("cos_sin", _vp), ("max_pos", _i64),
+                ("k_outer", _vp), ("v_outer", _vp), ("kv_heads", _int), ("q_heads", _int), ("head_dim", _int), ("page", _int), ("rot", _int),
+                ("flags", _int)]
+
+
+class KvAttentionArgs(ctypes.Structure):
+    """qcc_kv_attention_args of include/quant_cast_cuda.h"""
+    _fields_ = [("q", _vp), ("q_stride", _i64 * 2), ("rows", _i64), ("cache", _vp), ("num_pages", _i64), ("table", _vp), ("table_stride", _i64),
+                ("table_width", _int), ("kv_lens", _vp), ("cu_q", _vp), ("seqs", _int), ("max_q", _int), ("k_outer", _vp), ("v_outer", _vp),
+                ("scale", ctypes.c_float), ("q_heads", _int), ("kv_heads", _int), ("head_dim", _int), ("page", _int), ("out", _vp), ("lse", _vp)]
 
 
 _lib = None
@@ -174,13 +199,17 @@ DEVICE_ERRORS = {
     17: "the transform matrix is not diag(+-1) @ H16 / 4",
     18: "a colwise fp8 cast gave up waiting for the column maxima of a panel",
     19: "a wait for another rank's amax (amax exchange) ran out",
+    20: "a page or slot number outside the cache, or a sequence longer than its row of the block table",
+    21: "a position outside the rotation table",
+    22: "query offsets that descend, leave the rows of q or exceed max_q",
 }
 
 
 def device_error():
     """Reads and clears the device-side error word of the current CUDA device (synchronises): 0 when no kernel
     reported anything, 1..15 a TMA barrier wait that ran out, 16 invalid token-group offsets, 17 an unsupported transform matrix, 18 a colwise cast
-    that gave up waiting for the column maxima of a panel, 19 a wait for another rank's amax that ran out."""
+    that gave up waiting for the column maxima of a panel, 19 a wait for another rank's amax that ran out, 20..22 bad page,
+    position or query numbers of a key/value cache call (DEVICE_ERRORS)."""
     v = ctypes.c_uint(0)
     rc = load().qcc_device_error(ctypes.byref(v))       # (not through check(): that is what calls this under QCC_CHECK_DEVICE)
     if rc:
