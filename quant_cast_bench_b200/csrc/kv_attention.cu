@@ -6,6 +6,8 @@
 // sees none gets o = 0 and lse = -inf.  One pass over the cache with the running maximum and sum of the softmax in fp32.
 #include "kv_cache.cuh"
 
+#include <type_traits>
+
 #include "host_util.h"
 
 namespace qcc {
@@ -38,6 +40,24 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
 {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t lds_u8(uint32_t addr)
+{
+    uint32_t r;
+    asm volatile("{\n.reg .u16 t;\nld.shared.u8 t, [%1];\ncvt.u32.u16 %0, t;\n}\n" : "=r"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ uint32_t lds_u16(uint32_t addr)
+{
+    uint16_t r;
+    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(addr));
+    return r;
+}
+__device__ __forceinline__ uint32_t lds_u32(uint32_t addr)
+{
+    uint32_t r;
+    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(addr));
     return r;
 }
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
@@ -97,23 +117,23 @@ __device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n
 // exact for all elements above 2^-22 of the row's largest; P is rounded to fp16, half a step of 2^-11.  The tensor cores are
 // far from busy (tcgen05 would need the widened tiles in shared memory, whose bandwidth that alone would use up).
 //
-// A tile is 128 tokens of one sequence and head, 16 for each warp.  A warp fetches its own tokens by bulk copies into a ring of
+// A tile is 128 tokens of one sequence and head, 32 for each warp.  A warp fetches its own tokens by bulk copies into a ring of
 // its own, so the warps of a CTA meet only where a unit ends.  All tiles of the batch are numbered and dealt out evenly,
 // whatever the lengths; a unit (sequence, head, row tile) that spans CTAs leaves partial sums which a second kernel joins in a
 // fixed order.
 // -------------------------------------------------------------------------------------------------------------------
-constexpr int SP_WARPS = 8, SP_THREADS = SP_WARPS * 32, SP_TOK = 16 * SP_WARPS;
+constexpr int SP_WARPS = 4, SP_THREADS = SP_WARPS * 32, SP_WTOK = 32, SP_TOK = SP_WTOK * SP_WARPS;
 
 template <int D, int NT> struct SplitCfg {
-    static constexpr int TILE = 16 * 2 * (D / 2 + D / 16);          // bytes of one warp's 16 tokens, keys and values
-    static constexpr int CTAS = NT == 1 ? 2 : 1;
-    static constexpr int STAGES = (NT == 1 ? 5 : 8) * (D == 64 ? 2 : 1);
+    static constexpr int TILE = SP_WTOK * 2 * (D / 2 + D / 16);     // bytes of one warp's tokens, keys and values
+    static constexpr int CTAS = NT == 1 ? 4 : 2;
+    static constexpr int STAGES = (NT == 1 ? 2 : 4) * (D == 64 ? 2 : 1);
     static constexpr int RED = SP_WARPS * NT * 8 * (D / 4) * 4;
     static constexpr int ML = SP_WARPS * NT * 8 * 2 * 4;
     static constexpr int FIXED = SP_WARPS * (TILE * STAGES + STAGES * 8) + RED + ML;
 };
 
-template <int D, int NT> __host__ __device__ constexpr int part_floats() { return NT * 8 * (D + 2); }
+template <int D, int NT> __host__ __device__ constexpr int part_floats() { return NT * 8 * (D + 2); }   // sums (NT * 8, D), then (maximum, denominator) of each row
 
 struct Segment {
     int b, q0, n, L, head, rt, first, last, unit_last;   // first, last: tiles of the unit; unit_last: flat number of the tile behind it
@@ -197,13 +217,15 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     if ((int)blockIdx.x >= ctas) return;
     const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
 
-    // ---- fetching: the warp's 16 tokens of tile after tile, C::STAGES ahead of their use.  The page of the next fetch is looked
-    // up one fetch early.
-    struct { Segment s; int t, tile, end; int64_t page; } f;
-    uint32_t fetched = 0;
+    // ---- fetching: the warp's tokens of tile after tile, C::STAGES ahead of their use.  The pages of the next fetch are looked up
+    // one fetch early.  Pages of 32 tokens and more: four copies (codes and scales, keys and values); pages of 16: two of a whole
+    // (page, head) block.
+    const int shift = 31 - __clz(g.page);
+    const uint32_t block_bytes = (uint32_t)g.page * 2 * RB;
+    struct { Segment s; int t, tile, end; int32_t page; } f;     // page: lanes 0 and 1 hold the first and second 16 tokens' page
+    uint32_t f_stage = 0;
     f.t = lo;
-    const uint32_t tok_bytes = 2 * RB * 16;
-    // moves the cursor to the next tile that exists (f.t < hi), and asks for its page
+    // moves the cursor to the next tile that exists (f.t < hi), and asks for its pages
     auto seek = [&](bool fresh) {
         for (;;) {
             if (!fresh) {
@@ -216,40 +238,47 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
             f.end = seen_tiles<NT>(g, f.s);
             fresh = false;
         }
-        const int tok = f.tile * SP_TOK + warp * 16;
-        f.page = tok < f.s.L ? (int64_t)__ldg(g.table + f.s.b * g.table_stride + tok / g.page) : -1;
+        const int tok = f.tile * SP_TOK + warp * SP_WTOK + (lane & 1) * 16;
+        f.page = tok < f.s.L ? __ldg(g.table + f.s.b * g.table_stride + (tok >> shift)) : -1;
     };
     auto fetch = [&]() {
         if (f.t >= hi) return;
-        const uint32_t st = fetched++ % C::STAGES;
-        const int tok = f.tile * SP_TOK + warp * 16;
-        const bool some = tok < f.s.L, ok = f.page >= 0 && f.page < g.num_pages;
-        if (lane == 0) {
-            if (some && !ok) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
-            mbar_expect_tx(full + st, ok ? tok_bytes : 0);
-        }
-        __syncwarp();
-        if (ok) {
-            const uint8_t *src = g.cache + (f.page * g.kv_heads + f.s.head) * (int64_t)(g.page * 2 * RB);
-            uint8_t *dst = ring + st * C::TILE;
-            if (g.page == 16) {
-                if (lane == 0) bulk_load(dst, src, tok_bytes, full + st);
-            } else if (lane < 4) {       // codes and scales of keys, codes and scales of values
-                const int off = tok % g.page, scales = lane & 1;
-                bulk_load(dst + (lane >> 1) * (16 * RB) + scales * (8 * D), src + (lane >> 1) * (g.page * RB) + (scales ? g.page * (D / 2) + off * (D / 16) : off * (D / 2)),
-                          scales ? D : 8 * D, full + st);
+        uint64_t *bar = full + f_stage;
+        uint8_t *dst = ring + f_stage * C::TILE;
+        const int tok = f.tile * SP_TOK + warp * SP_WTOK;
+        const bool ok = f.page >= 0 && f.page < g.num_pages;
+        if (!ok && lane < 2 && tok + lane * 16 < f.s.L) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
+        if (shift == 4) {
+            const uint32_t both = __ballot_sync(0xFFFFFFFFu, ok) & 3u;
+            if (lane == 0) mbar_expect_tx(bar, __popc(both) * (C::TILE / 2));
+            __syncwarp();
+            if (lane < 2 && ok) bulk_load(dst + lane * (C::TILE / 2), g.cache + ((int64_t)f.page * g.kv_heads + f.s.head) * block_bytes, C::TILE / 2, bar);
+        } else {
+            const int32_t pg = __shfl_sync(0xFFFFFFFFu, f.page, 0);
+            const bool good = pg >= 0 && pg < g.num_pages;
+            if (lane == 0) mbar_expect_tx(bar, good ? C::TILE : 0);
+            __syncwarp();
+            if (good && lane < 4) {
+                const int off = tok & (g.page - 1), scales = lane & 1;
+                const uint8_t *src = g.cache + ((int64_t)pg * g.kv_heads + f.s.head) * block_bytes + (lane >> 1) * (g.page * RB);
+                bulk_load(dst + (lane >> 1) * (C::TILE / 2) + scales * (SP_WTOK * D / 2), src + (scales ? g.page * (D / 2) + off * (D / 16) : off * (D / 2)),
+                          scales ? SP_WTOK * D / 16 : SP_WTOK * D / 2, bar);
             }
         }
+        f_stage = f_stage + 1 == C::STAGES ? 0 : f_stage + 1;
         seek(false);
     };
+    // where a stage has codes and scales of keys and values, and the distance from the first 16 tokens to the second
+    const uint32_t k_scales = shift == 4 ? 8 * D : SP_WTOK * D / 2, v_codes = shift == 4 ? 16 * RB : C::TILE / 2, v_scales = v_codes + k_scales;
+    const uint32_t next_codes = shift == 4 ? C::TILE / 2 : 8 * D, next_scales = shift == 4 ? C::TILE / 2 : D;
     seek(true);
 #pragma unroll 1
     for (int i = 0; i < C::STAGES; i++) fetch();
 
-    // ---- 16 tokens of every tile each
+    // ---- 32 tokens of every tile each
     const int gr = lane >> 2, c = lane & 3;
     const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
-    uint32_t it = 0;
+    uint32_t stage = 0, phase = 0;
     for (int t = lo; t < hi;) {
         Segment s;
         find_segment<NT>(g, prefix, t, hi, s);
@@ -299,30 +328,33 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
             m[nt][0] = m[nt][1] = -INFINITY;
             l[nt][0] = l[nt][1] = 0.0f;
         }
-        for (int tile = s.first; tile < end; tile++, it++) {
-            const uint32_t st = it % C::STAGES;
-            mbar_wait(full + st, (it / C::STAGES) & 1, KV_ATTN_ERR);
-            const int tok = tile * SP_TOK + warp * 16;
-            if (tok < s.L) {
-                const uint8_t *kc = ring + st * C::TILE, *ks = kc + 8 * D, *vc = kc + 16 * RB, *vs = vc + 8 * D;
-                float sc[NT][4];
+        // one warp's 32 tokens from `tok` on; MASKED: some of them are behind the last token, or hidden from some row
+        const auto step = [&](auto masked, int tok) {
+            constexpr bool MASKED = decltype(masked)::value;
+            const uint32_t base = smem_u32(ring + stage * C::TILE);
+            constexpr int HB = NT == 4 ? 1 : 2;      // 16-token blocks taken together, as registers allow
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
-                {
+            for (int h0 = 0; h0 < 2; h0 += HB) {
+                float sc[HB][NT][4];
+#pragma unroll
+                for (int h = 0; h < HB; h++) {
+                    const uint32_t kc = base + (h0 + h) * next_codes, ks = base + k_scales + (h0 + h) * next_scales;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) sc[h][nt][0] = sc[h][nt][1] = sc[h][nt][2] = sc[h][nt][3] = 0.0f;
                     uint32_t wa[KW], wb[KW], sa[2], sb[2];     // tokens gr and gr + 8
                     if (D == 128) {
-                        const uint4 a = lds_v4(smem_u32(kc + gr * 64 + c * 16)), b = lds_v4(smem_u32(kc + (gr + 8) * 64 + c * 16));
+                        const uint4 a = lds_v4(kc + gr * 64 + c * 16), b = lds_v4(kc + (gr + 8) * 64 + c * 16);
                         wa[0] = a.x; wa[1] = a.y; wa[2 % KW] = a.z; wa[3 % KW] = a.w;
                         wb[0] = b.x; wb[1] = b.y; wb[2 % KW] = b.z; wb[3 % KW] = b.w;
-                        const uint32_t u = *reinterpret_cast<const uint16_t *>(ks + gr * 8 + 2 * c), v = *reinterpret_cast<const uint16_t *>(ks + (gr + 8) * 8 + 2 * c);
-                        sa[0] = e4m3_to_half2(u & 0xFFu); sa[1] = e4m3_to_half2(u >> 8);
-                        sb[0] = e4m3_to_half2(v & 0xFFu); sb[1] = e4m3_to_half2(v >> 8);
+                        const uint32_t u = e4m3x2_to_half2(lds_u16(ks + gr * 8 + 2 * c)), v = e4m3x2_to_half2(lds_u16(ks + (gr + 8) * 8 + 2 * c));
+                        sa[0] = __byte_perm(u, u, 0x1010); sa[1] = __byte_perm(u, u, 0x3232);
+                        sb[0] = __byte_perm(v, v, 0x1010); sb[1] = __byte_perm(v, v, 0x3232);
                     } else {
-                        const uint2 a = lds_v2(smem_u32(kc + gr * 32 + c * 8)), b = lds_v2(smem_u32(kc + (gr + 8) * 32 + c * 8));
+                        const uint2 a = lds_v2(kc + gr * 32 + c * 8), b = lds_v2(kc + (gr + 8) * 32 + c * 8);
                         wa[0] = a.x; wa[1] = a.y;
                         wb[0] = b.x; wb[1] = b.y;
-                        sa[0] = sa[1] = e4m3_to_half2(ks[gr * 4 + c]);
-                        sb[0] = sb[1] = e4m3_to_half2(ks[(gr + 8) * 4 + c]);
+                        sa[0] = sa[1] = e4m3_to_half2(lds_u8(ks + gr * 4 + c));
+                        sb[0] = sb[1] = e4m3_to_half2(lds_u8(ks + (gr + 8) * 4 + c));
                     }
 #pragma unroll
                     for (int j = 0; j < KW; j++) {
@@ -336,31 +368,36 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            mma16816(sc[nt], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * j], qf[nt][4 * j + 1]);
-                            mma16816(sc[nt], ha[2], hb[2], ha[3], hb[3], qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
+                            mma16816(sc[h][nt], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * j], qf[nt][4 * j + 1]);
+                            mma16816(sc[h][nt], ha[2], hb[2], ha[3], hb[3], qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
                         }
                     }
                 }
-                // scores in log2 units; the running maximum moves only when a score is 2^8 above it, so that P stays below 2^8
-                bool grow = false;
+                // exponents of the probabilities, against the running maximum; it moves only when a score is 2^8 above it, so that P
+                // stays below 2^8
+                const auto seen = [&](int h, int nt, int x) { return !MASKED || tok + (h0 + h) * 16 + gr + (x >> 1) * 8 < limit[nt][x & 1]; };
+                float e[HB][NT][4], most = -INFINITY;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
+                for (int h = 0; h < HB; h++)
 #pragma unroll
-                    for (int x = 0; x < 4; x++) {
-                        const int key = tok + gr + (x >> 1) * 8;
-                        sc[nt][x] = key < limit[nt][x & 1] ? sc[nt][x] * factor[nt][x & 1] : -INFINITY;
-                        grow |= sc[nt][x] - m[nt][x & 1] > 8.0f;
-                    }
-                }
-                if (__any_sync(0xFFFFFFFFu, grow)) {
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
+                        for (int x = 0; x < 4; x++) {
+                            e[h][nt][x] = seen(h, nt, x) ? fmaf(sc[h][nt][x], factor[nt][x & 1], -m[nt][x & 1]) : -INFINITY;
+                            most = fmaxf(most, e[h][nt][x]);
+                        }
+                if (__any_sync(0xFFFFFFFFu, most > 8.0f)) {
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            float v = fmaxf(sc[nt][x], sc[nt][x + 2]);
+                            float v = m[nt][x];
+#pragma unroll
+                            for (int h = 0; h < HB; h++)
+#pragma unroll
+                                for (int y = x; y < 4; y += 2) v = fmaxf(v, seen(h, nt, y) ? sc[h][nt][y] * factor[nt][x] : -INFINITY);
 #pragma unroll
                             for (int sh = 4; sh < 32; sh <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, sh));
-                            v = fmaxf(m[nt][x], v);
                             const float a = v == -INFINITY ? 1.0f : ex2(m[nt][x] - v);
                             m[nt][x] = v;
                             l[nt][x] *= a;
@@ -369,60 +406,79 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                                 o[nt][i][x] *= a;
                                 o[nt][i][x + 2] *= a;
                             }
+#pragma unroll
+                            for (int h = 0; h < HB; h++)
+#pragma unroll
+                                for (int y = x; y < 4; y += 2) e[h][nt][y] = seen(h, nt, y) ? fmaf(sc[h][nt][y], factor[nt][x], -v) : -INFINITY;
                         }
+                }
+#pragma unroll
+                for (int h = 0; h < HB; h++) {
+                    uint32_t pb[NT][2];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        const float p0 = ex2(e[h][nt][0]), p1 = ex2(e[h][nt][1]), p2 = ex2(e[h][nt][2]), p3 = ex2(e[h][nt][3]);
+                        l[nt][0] += p0 + p2;
+                        l[nt][1] += p1 + p3;
+                        pb[nt][0] = transpose8x8(pack_half2(p0, p1));
+                        pb[nt][1] = transpose8x8(pack_half2(p2, p3));
                     }
-                }
-                uint32_t pb[NT][2];
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    const float m0 = m[nt][0] == -INFINITY ? 0.0f : m[nt][0], m1 = m[nt][1] == -INFINITY ? 0.0f : m[nt][1];
-                    const float p0 = ex2(sc[nt][0] - m0), p1 = ex2(sc[nt][1] - m1), p2 = ex2(sc[nt][2] - m0), p3 = ex2(sc[nt][3] - m1);
-                    l[nt][0] += p0 + p2;
-                    l[nt][1] += p1 + p3;
-                    pb[nt][0] = transpose8x8(pack_half2(p0, p1));
-                    pb[nt][1] = transpose8x8(pack_half2(p2, p3));
-                }
-                // values of tokens 2c, 2c + 1 and 2c + 8, 2c + 9
-                uint32_t vs2[2], vw[4][VW];
-#pragma unroll
-                for (int x = 0; x < 2; x++) {
-                    const int t0 = 2 * c + 8 * x;
-                    uint32_t s0 = D == 128 ? vs[t0 * 8 + gr] : vs[t0 * 4 + (gr >> 1)], s1 = D == 128 ? vs[t0 * 8 + 8 + gr] : vs[t0 * 4 + 4 + (gr >> 1)];
-                    if (tok + t0 >= s.L) s0 = 0;           // whatever the slots behind the last token hold, it counts as zero
-                    if (tok + t0 + 1 >= s.L) s1 = 0;
-                    const uint32_t two = s0 | (s1 << 8);
-                    asm("{\n.reg .b16 b;\ncvt.u16.u32 b, %1;\ncvt.rn.f16x2.e4m3x2 %0, b;\n}\n" : "=r"(vs2[x]) : "r"(two));
-                    if (D == 128) {
-                        const uint2 a = lds_v2(smem_u32(vc + t0 * 64 + gr * 8)), b = lds_v2(smem_u32(vc + t0 * 64 + 64 + gr * 8));
-                        vw[2 * x][0] = a.x; vw[2 * x][1 % VW] = a.y;
-                        vw[2 * x + 1][0] = b.x; vw[2 * x + 1][1 % VW] = b.y;
-                    } else {
-                        vw[2 * x][0] = *reinterpret_cast<const uint32_t *>(vc + t0 * 32 + gr * 4);
-                        vw[2 * x + 1][0] = *reinterpret_cast<const uint32_t *>(vc + t0 * 32 + 32 + gr * 4);
-                    }
-                }
-#pragma unroll
-                for (int j = 0; j < VW; j++) {
-                    uint32_t ev[2][4], od[2][4];      // even and odd elements, token pairs
+                    // values of tokens 2c, 2c + 1 and 2c + 8, 2c + 9
+                    const uint32_t vc = base + v_codes + (h0 + h) * next_codes, vs = base + v_scales + (h0 + h) * next_scales;
+                    uint32_t vs2[2], vw[4][VW];
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
-                        const uint32_t w0 = vw[2 * x][j], w1 = vw[2 * x + 1][j];
-                        e2m1x8_to_half((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), ev[x]);
-                        e2m1x8_to_half(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), od[x]);
-#pragma unroll
-                        for (int u = 0; u < 4; u++) {
-                            ev[x][u] = hmul2_bits(ev[x][u], vs2[x]);
-                            od[x][u] = hmul2_bits(od[x][u], vs2[x]);
+                        const int t0 = 2 * c + 8 * x;
+                        uint32_t s0 = D == 128 ? lds_u8(vs + t0 * 8 + gr) : lds_u8(vs + t0 * 4 + (gr >> 1)), s1 = D == 128 ? lds_u8(vs + t0 * 8 + 8 + gr) : lds_u8(vs + t0 * 4 + 4 + (gr >> 1));
+                        if (MASKED) {        // whatever the slots behind the last token hold, it counts as zero
+                            if (tok + (h0 + h) * 16 + t0 >= s.L) s0 = 0;
+                            if (tok + (h0 + h) * 16 + t0 + 1 >= s.L) s1 = 0;
+                        }
+                        vs2[x] = e4m3x2_to_half2(s0 | (s1 << 8));
+                        if (D == 128) {
+                            const uint2 a = lds_v2(vc + t0 * 64 + gr * 8), b = lds_v2(vc + t0 * 64 + 64 + gr * 8);
+                            vw[2 * x][0] = a.x; vw[2 * x][1 % VW] = a.y;
+                            vw[2 * x + 1][0] = b.x; vw[2 * x + 1][1 % VW] = b.y;
+                        } else {
+                            vw[2 * x][0] = lds_u32(vc + t0 * 32 + gr * 4);
+                            vw[2 * x + 1][0] = lds_u32(vc + t0 * 32 + 32 + gr * 4);
                         }
                     }
 #pragma unroll
-                    for (int u = 0; u < 4; u++)
+                    for (int j = 0; j < VW; j++) {
+                        uint32_t ev[2][4], od[2][4];      // even and odd elements, token pairs
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma16816(o[nt][4 * j + u], ev[0][u], od[0][u], ev[1][u], od[1][u], pb[nt][0], pb[nt][1]);
+                        for (int x = 0; x < 2; x++) {
+                            const uint32_t w0 = vw[2 * x][j], w1 = vw[2 * x + 1][j];
+                            e2m1x8_to_half((w0 & 0x0F0F0F0Fu) | ((w1 << 4) & 0xF0F0F0F0u), ev[x]);
+                            e2m1x8_to_half(((w0 >> 4) & 0x0F0F0F0Fu) | (w1 & 0xF0F0F0F0u), od[x]);
+#pragma unroll
+                            for (int u = 0; u < 4; u++) {
+                                ev[x][u] = hmul2_bits(ev[x][u], vs2[x]);
+                                od[x][u] = hmul2_bits(od[x][u], vs2[x]);
+                            }
+                        }
+#pragma unroll
+                        for (int u = 0; u < 4; u++)
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma16816(o[nt][4 * j + u], ev[0][u], od[0][u], ev[1][u], od[1][u], pb[nt][0], pb[nt][1]);
+                    }
                 }
             }
+        };
+        const int clear = s.L - s.n + s.rt * NT * 8 / g.group + 1;      // keys that the row tile's first row, and so every row, sees
+
+        for (int tile = s.first; tile < end; tile++) {
+            mbar_wait(full + stage, phase, KV_ATTN_ERR);
+            const int tok = tile * SP_TOK + warp * SP_WTOK;
+            if (tok + SP_WTOK <= clear) step(std::false_type(), tok);
+            else if (tok < s.L) step(std::true_type(), tok);
             __syncwarp();      // all lanes have read the stage that the next fetch overwrites
             fetch();
+            if (++stage == C::STAGES) {
+                stage = 0;
+                phase ^= 1;
+            }
         }
 
         // ---- join the warps, then write the unit's result or this CTA's partial sums
@@ -483,11 +539,8 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                         if (round == 0 && x == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
                     }
                 } else {
-                    slot[qi * (D + 2) + 2 + d] = sum;
-                    if (round == 0 && x == 0) {
-                        slot[qi * (D + 2)] = top;
-                        slot[qi * (D + 2) + 1] = den;
-                    }
+                    slot[qi * D + d] = sum;
+                    if (round == 0 && x == 0) reinterpret_cast<float2 *>(slot + NT * 8 * D)[qi] = make_float2(top, den);
                 }
             }
             named_barrier(1, SP_WARPS * 32);
@@ -497,16 +550,21 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
 }
 
 // One CTA per unit (sequence, head, row tile): joins the partial sums of a unit that several CTAs worked on, in the order of
-// its tokens, and fills the rows of a unit without tokens.
+// its tokens, and fills the rows of a unit without tokens.  A thread has four neighbouring elements of a row, and the weights of
+// the parts are worked out once, so the loads of the sums do not wait for one another (a thread an element that found the maximum
+// first took 74 us to join 16 units of 19 parts, this takes 5).
+constexpr int JOIN_MAX = 1024;     // parts of a unit: at most one for each CTA of the first kernel
 template <int D, int NT>
-__global__ void __launch_bounds__(128) kv_attn_join_kernel(const AttnArgs g, int grid, int max_rts, int units)
+__global__ void __launch_bounds__(NT * 2 * D) kv_attn_join_kernel(const AttnArgs g, int grid, int max_rts, int units)
 {
+    constexpr int ROWS = NT * 8, THREADS = ROWS * D / 4;
+    __shared__ float2 ml[JOIN_MAX];
     pdl_wait();
     if ((int)blockIdx.x >= units) {
         // rows behind the last sequence
         const int64_t first = (int64_t)max(__ldg(g.cu_q + g.seqs), 0) * g.q_heads, n = g.rows * g.q_heads;
         for (int64_t r = first + blockIdx.x - units; r < n; r += gridDim.x - units) {
-            for (int d = threadIdx.x; d < D; d += 128) g.out[r * D + d] = 0;
+            for (int d = threadIdx.x; d < D; d += THREADS) g.out[r * D + d] = 0;
             if (threadIdx.x == 0 && g.lse) g.lse[r] = -INFINITY;
         }
         return;
@@ -514,37 +572,53 @@ __global__ void __launch_bounds__(128) kv_attn_join_kernel(const AttnArgs g, int
     const int rt = blockIdx.x % max_rts, head = blockIdx.x / max_rts % g.kv_heads, b = blockIdx.x / max_rts / g.kv_heads;
     int q0, n, L;
     seq_of(g, b, q0, n, L);
-    const int rows = n * g.group, rts = (rows + NT * 8 - 1) / (NT * 8), kvt = (L + SP_TOK - 1) / SP_TOK;
+    const int rows = n * g.group, rts = (rows + ROWS - 1) / ROWS, kvt = (L + SP_TOK - 1) / SP_TOK;
     if (rt >= rts) return;
     const int total = g.prefix[g.seqs], ctas = min(grid, total);
-    const float v_outer = __ldg(g.v_outer);
-    int i0 = 0, i1 = -1, first = 0;
+    int i0 = 0, parts = 0, first = 0;
     if (kvt > 0) {
         first = g.prefix[b] + (head * rts + rt) * kvt;
         // CTA i works on tiles [total * i / ctas, total * (i + 1) / ctas): tile t belongs to ((t + 1) * ctas - 1) / total
         i0 = (int)((((int64_t)first + 1) * ctas - 1) / total);
-        i1 = (int)((((int64_t)first + kvt) * ctas - 1) / total);
-        if (i0 == i1) return;
+        parts = (int)((((int64_t)first + kvt) * ctas - 1) / total) - i0 + 1;
+        if (parts == 1) return;
     }
-    const int slot0 = kvt > 0 && (int)((int64_t)total * i0 / ctas) < first ? 1 : 0;    // the unit is not the first of its first CTA
-    for (int e = threadIdx.x; e < NT * 8 * D; e += 128) {
-        const int qi = e / D, d = e - qi * D, r = rt * NT * 8 + qi;
-        if (r >= rows) break;
-        float top = -INFINITY, den = 0.0f, sum = 0.0f;
-        for (int i = i0; i <= i1; i++)
-            top = fmaxf(top, g.part[(size_t)(2 * i + (i == i0 ? slot0 : 0)) * part_floats<D, NT>() + qi * (D + 2)]);
-        for (int i = i0; i <= i1; i++) {
-            const float *p = g.part + (size_t)(2 * i + (i == i0 ? slot0 : 0)) * part_floats<D, NT>() + qi * (D + 2);
-            const float a = p[0] == -INFINITY ? 1.0f : ex2(p[0] - top);
-            den += p[1] * a;
-            sum += p[2 + d] * a;
+    // the slot of part j: the second one of the CTA whose first tile is not this unit's
+    const int second = kvt > 0 && (int)((int64_t)total * i0 / ctas) < first ? 1 : 0;
+    const float *base = g.part + (size_t)2 * i0 * part_floats<D, NT>();
+    const int row = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, r = rt * ROWS + row;
+    float top = -INFINITY, den = 0.0f;
+    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int j0 = 0; j0 < parts; j0 += JOIN_MAX / ROWS) {
+        const int some = min(parts - j0, JOIN_MAX / ROWS);
+        __syncthreads();
+        for (int e = threadIdx.x; e < some * ROWS; e += THREADS) {
+            const int j = j0 + e / ROWS;
+            ml[e] = reinterpret_cast<const float2 *>(base + (size_t)(2 * j + (j == 0 ? second : 0)) * part_floats<D, NT>() + ROWS * D)[e % ROWS];
         }
-        const int i = r / g.group;
-        const int64_t at = (int64_t)(q0 + i) * g.q_heads + head * g.group + r - i * g.group;
-        const __nv_bfloat16 y = __float2bfloat16_rn(den == 0.0f ? 0.0f : __fdividef(sum * v_outer, den));
-        g.out[at * D + d] = *reinterpret_cast<const uint16_t *>(&y);
-        if (d == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
+        __syncthreads();
+        float up = top;
+        for (int j = 0; j < some; j++) up = fmaxf(up, ml[j * ROWS + row].x);
+        const float old = top == -INFINITY ? 1.0f : ex2(top - up);
+        top = up;
+        den *= old; sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
+#pragma unroll 8
+        for (int j = 0; j < some; j++) {
+            const float4 v = *reinterpret_cast<const float4 *>(base + (size_t)(2 * (j0 + j) + (j0 + j == 0 ? second : 0)) * part_floats<D, NT>() + row * D + d);
+            const float2 w = ml[j * ROWS + row];
+            const float a = w.x == -INFINITY ? 1.0f : ex2(w.x - top);     // a part that saw nothing holds zeros (or NaN, which stays)
+            den += w.y * a;
+            sum.x += v.x * a; sum.y += v.y * a; sum.z += v.z * a; sum.w += v.w * a;
+        }
     }
+    if (r >= rows) return;
+    const int i = r / g.group;
+    const int64_t at = (int64_t)(q0 + i) * g.q_heads + head * g.group + r - i * g.group;
+    const float inv = den == 0.0f ? 0.0f : __fdividef(__ldg(g.v_outer), den);
+    const __nv_bfloat162 lo = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.x * inv, den == 0.0f ? 0.0f : sum.y * inv);
+    const __nv_bfloat162 hi = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.z * inv, den == 0.0f ? 0.0f : sum.w * inv);
+    *reinterpret_cast<uint2 *>(g.out + at * D + d) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
+    if (d == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
 }
 
 template <int D, int NT>
@@ -566,7 +640,7 @@ static int split_launch(const AttnArgs &g, int max_q, cudaStream_t st)
     const int max_rts = (int)(((int64_t)max_q * g.group + NT * 8 - 1) / (NT * 8));
     const int units = g.seqs * g.kv_heads * max_rts;
     const int behind = g.cu_q ? 32 : 0;      // CTAs for the rows behind the last sequence
-    return (int)launch_maybe_pdl(kv_attn_join_kernel<D, NT>, dim3((unsigned)(units + behind)), dim3(128), 0, st, true, g, grid, max_rts, units);
+    return (int)launch_maybe_pdl(kv_attn_join_kernel<D, NT>, dim3((unsigned)(units + behind)), dim3(NT * 2 * D), 0, st, true, g, grid, max_rts, units);
 }
 
 // how the rows of a sequence and kv head are tiled: 8 * nt rows
@@ -583,7 +657,7 @@ extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int seqs, int max_q, in
     if (seqs < 0 || max_q < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
     const int nt = row_tiles_of((int64_t)max_q * (q_heads / kv_heads));
     const size_t prefix = (((size_t)seqs + 1) * 4 + 15) / 16 * 16;
-    return prefix + (size_t)2 * sm_count() * (nt == 1 ? 2 : 1) * nt * 8 * (head_dim + 2) * 4;
+    return prefix + (size_t)2 * sm_count() * (nt == 1 ? 4 : 2) * nt * 8 * (head_dim + 2) * 4;
 }
 
 extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *workspace, size_t workspace_bytes, void *stream)

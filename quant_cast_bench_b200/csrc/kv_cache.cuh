@@ -29,12 +29,17 @@ __device__ __forceinline__ void e2m1x8_to_half(uint32_t w, uint32_t (&h)[4])
         : "=r"(h[0]), "=r"(h[1]), "=r"(h[2]), "=r"(h[3])
         : "r"(w));
 }
+// two e4m3 bytes -> half2, the low byte in the low half; exact
+__device__ __forceinline__ uint32_t e4m3x2_to_half2(uint32_t two)
+{
+    uint32_t h;
+    asm("{\n.reg .b16 b;\ncvt.u16.u32 b, %1;\ncvt.rn.f16x2.e4m3x2 %0, b;\n}\n" : "=r"(h) : "r"(two));
+    return h;
+}
 // an e4m3 byte as half2 with both halves its value; exact
 __device__ __forceinline__ uint32_t e4m3_to_half2(uint32_t byte)
 {
-    uint32_t h;
-    asm("{\n.reg .b16 b;\ncvt.u16.u32 b, %1;\ncvt.rn.f16x2.e4m3x2 %0, b;\n}\n" : "=r"(h) : "r"(byte * 0x101u));
-    return h;
+    return e4m3x2_to_half2(byte * 0x101u);
 }
 __device__ __forceinline__ uint32_t hmul2_bits(uint32_t a, uint32_t b)
 {
