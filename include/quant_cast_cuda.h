@@ -535,7 +535,7 @@ typedef struct qcc_kv_attention_args {
     void *out;
     float *lse;
 } qcc_kv_attention_args;
-size_t qcc_nvfp4_kv_attention_workspace_bytes(int seqs, int max_q, int q_heads, int kv_heads, int head_dim);
+size_t qcc_nvfp4_kv_attention_workspace_bytes(int64_t rows, int seqs, int max_q, int q_heads, int kv_heads, int head_dim);
 int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -608,6 +608,7 @@ extern "C" int qcc_colwise_device_error(unsigned int *out);
 extern "C" int qcc_int8_device_error(unsigned int *out);
 extern "C" int qcc_kv_cache_device_error(unsigned int *out);
 extern "C" int qcc_kv_attention_device_error(unsigned int *out);
+extern "C" int qcc_kv_prompt_device_error(unsigned int *out);
 extern "C" int qcc_xchg_device_error(unsigned int *out);
 
 extern "C" {
@@ -633,6 +634,8 @@ int qcc_device_error(unsigned int *out)
     if ((e = qcc_kv_cache_device_error(&d)) != 0) return e;
     c = c > d ? c : d;
     if ((e = qcc_kv_attention_device_error(&d)) != 0) return e;
+    c = c > d ? c : d;
+    if ((e = qcc_kv_prompt_device_error(&d)) != 0) return e;
     c = c > d ? c : d;
     if (out) *out = a > b ? (a > c ? a : c) : (b > c ? b : c);
     return 0;

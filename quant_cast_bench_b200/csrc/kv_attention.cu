@@ -4,7 +4,7 @@
 //
 // over the keys j that a query sees: query i of the n of a sequence with L cached tokens sees j <= L - n + i.  A query that
 // sees none gets o = 0 and lse = -inf.  One pass over the cache with the running maximum and sum of the softmax in fp32.
-#include "kv_cache.cuh"
+#include "kv_attention.cuh"
 
 #include <type_traits>
 
@@ -12,94 +12,7 @@
 
 namespace qcc {
 
-constexpr unsigned int QCC_DEVERR_QUERIES = 22u;    // query offsets that are not ascending within the rows of q
 constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ran out
-constexpr int KV_MAX_SEQS = 4096;
-constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
-
-struct AttnArgs {
-    const uint16_t *q;
-    const uint8_t *cache;
-    const int32_t *table, *kv_lens, *cu_q;
-    const float *k_outer, *v_outer;
-    uint16_t *out;
-    float *lse, *part;      // part: 2 slots per CTA of NT * 8 rows x (D + 2) floats
-    int32_t *prefix;        // seqs + 1
-    int64_t q_token, q_head, table_stride, num_pages, rows;
-    float scale_log2;
-    int seqs, width, q_heads, kv_heads, group, page, max_q;
-};
-
-__device__ __forceinline__ float ex2(float x)
-{
-    float r;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-    return r;
-}
-__device__ __forceinline__ uint32_t pack_half2(float lo, float hi)
-{
-    uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ uint32_t lds_u8(uint32_t addr)
-{
-    uint32_t r;
-    asm volatile("{\n.reg .u16 t;\nld.shared.u8 t, [%1];\ncvt.u32.u16 %0, t;\n}\n" : "=r"(r) : "r"(addr));
-    return r;
-}
-__device__ __forceinline__ uint32_t lds_u16(uint32_t addr)
-{
-    uint16_t r;
-    asm volatile("ld.shared.u16 %0, [%1];" : "=h"(r) : "r"(addr));
-    return r;
-}
-__device__ __forceinline__ uint32_t lds_u32(uint32_t addr)
-{
-    uint32_t r;
-    asm volatile("ld.shared.u32 %0, [%1];" : "=r"(r) : "r"(addr));
-    return r;
-}
-__device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1)
-{
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t a)
-{
-    uint32_t r;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(a));
-    return r;
-}
-__device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t bytes, uint64_t *bar)
-{
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)), "l"(src),
-                 "r"(bytes), "r"(smem_u32(bar))
-                 : "memory");
-}
-
-// queries and cached tokens of sequence b, checked against what the caller's tensors hold
-__device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n, int &L)
-{
-    if (g.cu_q) {
-        q0 = __ldg(g.cu_q + b);
-        n = __ldg(g.cu_q + b + 1) - q0;
-        if (q0 < 0 || n < 0 || n > g.max_q || (int64_t)q0 + n > g.rows) {
-            atomicMax(&g_qcc_error, QCC_DEVERR_QUERIES);
-            q0 = 0;
-            n = 0;
-        }
-    } else {
-        q0 = b;
-        n = 1;
-    }
-    L = max(__ldg(g.kv_lens + b), 0);
-    if (L > (int64_t)g.width * g.page) {
-        atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
-        L = g.width * g.page;
-    }
-}
 
 // -------------------------------------------------------------------------------------------------------------------
 // Few queries: work split over the cached tokens
@@ -302,9 +215,8 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
             uint32_t m = f2u(hmax_halves_f32(acc));
             m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 1));
             m = max(m, __shfl_xor_sync(0xFFFFFFFFu, m, 2));
-            uint32_t e = m >> 23;
-            e = e == 255u ? 134u : max(e, 8u);
-            const float mult = u2f((261u - e) << 23), back = u2f((e - 7u) << 23);
+            float mult, back;
+            q_power(m, mult, back);
 #pragma unroll
             for (int j = 0; j < KW; j++) {
                 qf[nt][4 * j] = pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult);
@@ -645,6 +557,8 @@ static int split_launch(const AttnArgs &g, int max_q, cudaStream_t st)
 
 // how the rows of a sequence and kv head are tiled: 8 * nt rows
 static int row_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
+// more rows than one row tile: the tcgen05 kernel
+static bool many_queries(int max_q, int group) { return (int64_t)max_q * group > 32; }
 
 }  // namespace qcc
 
@@ -652,9 +566,10 @@ using namespace qcc;
 
 extern "C" int qcc_kv_attention_device_error(unsigned int *out) { return read_clear_device_error(out); }
 
-extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int seqs, int max_q, int q_heads, int kv_heads, int head_dim)
+extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int64_t rows, int seqs, int max_q, int q_heads, int kv_heads, int head_dim)
 {
-    if (seqs < 0 || max_q < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+    if (rows < 0 || seqs < 0 || max_q < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
+    if (many_queries(max_q, q_heads / kv_heads)) return prompt_workspace_bytes(rows, q_heads / kv_heads, seqs, head_dim);
     const int nt = row_tiles_of((int64_t)max_q * (q_heads / kv_heads));
     const size_t prefix = (((size_t)seqs + 1) * 4 + 15) / 16 * 16;
     return prefix + (size_t)2 * sm_count() * (nt == 1 ? 4 : 2) * nt * 8 * (head_dim + 2) * 4;
@@ -673,9 +588,11 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     if (!p->q || !p->cache || !p->kv_lens || !p->k_outer || !p->v_outer || !p->out || (!p->table && p->table_width > 0)) return QCC_ERR_ARG;
     if (!aligned16(p->q) || !aligned16(p->cache) || !aligned16(p->out) || (p->q_stride[0] | p->q_stride[1]) % 8 != 0) return QCC_ERR_ALIGN;
     const int group = p->q_heads / p->kv_heads, max_q = p->cu_q ? p->max_q : 1, nt = row_tiles_of((int64_t)max_q * group);
-    const int64_t rts = ((int64_t)max_q * group + nt * 8 - 1) / (nt * 8), kvt = ((int64_t)p->table_width * p->page + SP_TOK - 1) / SP_TOK;
-    if (rts * p->kv_heads * p->seqs > 0x7FFFFF00 || rts * p->kv_heads * p->seqs * (kvt + 1) > 0x7FFFFFFF) return QCC_ERR_SHAPE;
-    if (!workspace || workspace_bytes < qcc_nvfp4_kv_attention_workspace_bytes(p->seqs, max_q, p->q_heads, p->kv_heads, p->head_dim)) return QCC_ERR_WORKSPACE;
+    const int64_t cached = (int64_t)p->table_width * p->page;
+    if (many_queries(max_q, group) ? !prompt_fits(p->rows, group, p->seqs, p->kv_heads, cached)
+                                   : (int64_t)p->seqs * p->kv_heads > 0x7FFFFF00 / ((cached + SP_TOK - 1) / SP_TOK + 1))
+        return QCC_ERR_SHAPE;
+    if (!workspace || workspace_bytes < qcc_nvfp4_kv_attention_workspace_bytes(p->rows, p->seqs, max_q, p->q_heads, p->kv_heads, p->head_dim)) return QCC_ERR_WORKSPACE;
     if (!aligned16(workspace)) return QCC_ERR_ALIGN;
     AttnArgs g;
     g.q = static_cast<const uint16_t *>(p->q);
@@ -691,6 +608,7 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     g.scale_log2 = p->scale * LOG2E;
     g.seqs = p->seqs; g.width = p->table_width; g.q_heads = p->q_heads; g.kv_heads = p->kv_heads; g.group = group; g.page = p->page; g.max_q = max_q;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (many_queries(max_q, group)) return prompt_launch(g, p->head_dim, workspace, st);
     if (p->head_dim == 128)
         return nt == 1 ? split_launch<128, 1>(g, max_q, st) : nt == 2 ? split_launch<128, 2>(g, max_q, st) : split_launch<128, 4>(g, max_q, st);
     return nt == 1 ? split_launch<64, 1>(g, max_q, st) : nt == 2 ? split_launch<64, 2>(g, max_q, st) : split_launch<64, 4>(g, max_q, st);

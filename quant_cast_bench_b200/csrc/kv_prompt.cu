@@ -1,0 +1,601 @@
+// Attention of many queries (chunks of prompts) over the paged nvfp4 key/value cache, on the tcgen05 tensor cores of sm_100a.
+#include "kv_attention.cuh"
+#include "tcgen05.cuh"
+
+#include "host_util.h"
+
+namespace qcc {
+
+// -------------------------------------------------------------------------------------------------------------------
+// Many queries: bound by the tensor cores and by the exponentials
+//
+// A unit is 256 rows (queries times the heads of a group, token-major) of a sequence and kv head: two row tiles of 128, whose
+// softmaxes take turns with the matrix instructions.  For each tile of 128 tokens
+//   S = Q K^T   128 x 128 x D, Q and K in shared memory, S in tensor memory;
+//   P = exp2(S * factor - m), one thread a row, written back over S as fp16;
+//   O += P V    P from tensor memory, V in shared memory (its elements contiguous: the N-major form), O in tensor memory.
+// The codes of a page come by bulk copies; four warps widen them to fp16 (codes times block scales: exact) straight into the
+// 128-byte swizzled rows that the instructions read, the same layout for K and V.  That happens once for 256 rows.
+// q is brought to fp16 by a power of two for its row, exact for all elements above 2^-22 of the row's largest; P is rounded to fp16, half a step
+// of 2^-11; sums and maxima stay in fp32.  O is only rescaled when a row's maximum has grown by more than 2^8.
+//
+// Roles: warp 0 copies, warp 1 issues the matrix instructions, warps 4-7 widen, warps 8-11 and 12-15 are the softmax of the two
+// row tiles.  All (unit, tile) pairs are numbered, by a first small kernel, and dealt out evenly to one CTA per SM, whatever the lengths and however
+// many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, joined by a third kernel in a fixed order.
+// -------------------------------------------------------------------------------------------------------------------
+constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3;
+constexpr unsigned int PT_ERR = 9u;    // a barrier wait of this kernel ran out
+
+template <int D> struct PromptCfg {
+    static constexpr int BLOCKS = D / 64;                       // 64-element blocks of a row: 128 bytes of fp16
+    static constexpr int TILE = BLOCKS * 128 * 128;             // 128 rows of Q, K or V as fp16
+    static constexpr int RAW = PT_TOK * kv_row_bytes<D>();      // codes and scales of 128 tokens, keys or values
+    static constexpr int SMEM = 1024 + 6 * TILE + PT_RAW * RAW + 256;
+};
+
+// ---- numbering: prefix[p] = tiles of all (sequence, row tile) pairs before p, times the kv heads; pairs[p] = (sequence, row tile)
+struct PromptPlan {
+    int32_t *count;      // [0]: pairs
+    int2 *pairs;
+    int32_t *prefix;     // pairs + 1
+};
+__host__ __device__ __forceinline__ int64_t prompt_max_pairs(int64_t rows, int group, int seqs) { return rows * group / PT_ROWS + seqs; }
+static size_t prompt_plan_bytes(int64_t max_pairs) { return 16 + (size_t)(max_pairs + 1) * 16; }
+static PromptPlan prompt_plan(void *ws, int64_t max_pairs)
+{
+    PromptPlan p;
+    p.count = static_cast<int32_t *>(ws);
+    p.pairs = reinterpret_cast<int2 *>(p.count + 4);
+    p.prefix = reinterpret_cast<int32_t *>(p.pairs + max_pairs + 1);
+    return p;
+}
+// tiles of row tile qt of a sequence: up to the last key that its last row sees
+__device__ __forceinline__ int prompt_tiles(int n, int L, int qt, int group)
+{
+    const int i = (int)min((int64_t)n - 1, ((int64_t)(qt + 1) * PT_ROWS - 1) / group);
+    return (max(L - n + i + 1, 0) + PT_TOK - 1) / PT_TOK;
+}
+
+__device__ __forceinline__ int block_scan(int v, int32_t *wsum, int &all)     // inclusive; 1024 threads
+{
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
+        if (lane >= o) v += u;
+    }
+    if (lane == 31) wsum[warp] = v;
+    __syncthreads();
+    if (warp == 0) {
+        int u = wsum[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int x = __shfl_up_sync(0xFFFFFFFFu, u, o);
+            if (lane >= o) u += x;
+        }
+        wsum[lane] = u;
+    }
+    __syncthreads();
+    all = wsum[31];
+    const int r = v + (warp ? wsum[warp - 1] : 0);
+    __syncthreads();
+    return r;
+}
+
+__global__ void __launch_bounds__(1024) kv_prompt_plan_kernel(const AttnArgs g, const PromptPlan plan)
+{
+    __shared__ int32_t start[KV_MAX_SEQS + 1], wsum[32];
+    int carry = 0;
+    for (int b0 = 0; b0 < g.seqs; b0 += 1024) {
+        const int b = b0 + threadIdx.x;
+        int q0, n = 0, L, all;
+        if (b < g.seqs) seq_of(g, b, q0, n, L);
+        const int v = block_scan((int)(((int64_t)n * g.group + PT_ROWS - 1) / PT_ROWS), wsum, all);
+        if (b < g.seqs) start[b + 1] = carry + v;
+        carry += all;
+    }
+    if (threadIdx.x == 0) start[0] = 0;
+    __syncthreads();
+    const int pairs = min((int64_t)carry, prompt_max_pairs(g.rows, g.group, g.seqs));     // (more only if offsets overlap)
+    int tiles = 0;
+    for (int p0 = 0; p0 < pairs; p0 += 1024) {
+        const int p = p0 + threadIdx.x;
+        int v = 0, all;
+        if (p < pairs) {
+            int lo = 0, up = g.seqs - 1;
+            while (lo < up) {
+                const int mid = (lo + up + 1) >> 1;
+                if (start[mid] <= p) lo = mid; else up = mid - 1;
+            }
+            int q0, n, L;
+            seq_of(g, lo, q0, n, L);
+            plan.pairs[p] = make_int2(lo, p - start[lo]);
+            v = prompt_tiles(n, L, p - start[lo], g.group) * g.kv_heads;
+        }
+        const int s = block_scan(v, wsum, all);
+        if (p < pairs) plan.prefix[p + 1] = tiles + s;
+        tiles += all;
+    }
+    if (threadIdx.x == 0) {
+        plan.prefix[0] = 0;
+        plan.count[0] = pairs;
+    }
+}
+
+// ---- the work of a CTA: parts of units
+struct Part {
+    int b, q0, n, L, qt, head, tiles, first, last, unit_first;     // tiles: of the unit; first, last: of this part; unit_first: flat
+};
+__device__ __forceinline__ void find_part(const AttnArgs &g, const PromptPlan &plan, int pairs, int t, int hi, Part &s)
+{
+    int lo = 0, up = pairs - 1;       // the last pair with prefix <= t, which has tiles
+    while (lo < up) {
+        const int mid = (lo + up + 1) >> 1;
+        if (plan.prefix[mid] <= t) lo = mid; else up = mid - 1;
+    }
+    const int2 pr = plan.pairs[lo];
+    const int start = plan.prefix[lo];
+    s.b = pr.x;
+    s.qt = pr.y;
+    seq_of(g, s.b, s.q0, s.n, s.L);
+    s.tiles = (plan.prefix[lo + 1] - start) / g.kv_heads;
+    s.head = (t - start) / s.tiles;
+    s.unit_first = start + s.head * s.tiles;
+    s.first = t - s.unit_first;
+    s.last = min(s.tiles, s.first + hi - t);
+}
+template <int D> __host__ __device__ constexpr int prompt_part_floats() { return PT_ROWS * (D + 2); }
+
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
+{
+    asm volatile("tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+                 "r"(r[15])
+                 : "memory");
+}
+__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// byte of 16-byte chunk `ch` (0 .. D / 8 - 1) of row r in a swizzled tile of 128 rows
+__device__ __forceinline__ uint32_t tile_at(int r, int ch) { return (uint32_t)((ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)); }
+
+template <int D>
+__global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs g, const PromptPlan plan)
+{
+    using C = PromptCfg<D>;
+    constexpr int RB = kv_row_bytes<D>();
+    extern __shared__ uint8_t raw_smem[];
+    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
+    uint8_t *s_q = sm, *s_k = sm + 2 * C::TILE, *s_v = sm + 4 * C::TILE, *s_raw = sm + 6 * C::TILE;
+    uint64_t *bars = reinterpret_cast<uint64_t *>(s_raw + PT_RAW * C::RAW);
+    uint64_t *raw_full = bars, *raw_empty = bars + 3, *k_full = bars + 6, *k_empty = bars + 8, *v_full = bars + 10, *v_empty = bars + 12, *q_full = bars + 14,
+             *s_full = bars + 16, *p_full = bars + 18, *o_done = bars + 20;
+    uint32_t *slot = reinterpret_cast<uint32_t *>(bars + 22);
+    volatile uint32_t *abort = slot + 1;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    pdl_wait();      // the numbering
+    const int pairs = plan.count[0], total = plan.prefix[pairs], ctas = min((int)gridDim.x, total);
+
+    // rows that see no key, and rows behind the last sequence
+    for (int p = blockIdx.x; p < pairs; p += gridDim.x) {
+        if (plan.prefix[p + 1] != plan.prefix[p]) continue;
+        const int2 pr = plan.pairs[p];
+        int q0, n, L;
+        seq_of(g, pr.x, q0, n, L);
+        const int64_t rows = (int64_t)n * g.group, r0 = (int64_t)pr.y * PT_ROWS, r1 = min(rows, r0 + PT_ROWS);
+        for (int64_t e = threadIdx.x; e < (r1 - r0) * g.kv_heads * D; e += PT_THREADS) {
+            const int64_t x = e / D, r = r0 + x / g.kv_heads;
+            const int64_t at = (q0 + r / g.group) * g.q_heads + x % g.kv_heads * g.group + r % g.group;
+            g.out[at * D + e % D] = 0;
+            if (e % D == 0 && g.lse) g.lse[at] = -INFINITY;
+        }
+    }
+    if (g.cu_q) {
+        const int64_t first = (int64_t)max(__ldg(g.cu_q + g.seqs), 0) * g.q_heads, n = g.rows * g.q_heads;
+        for (int64_t r = first + blockIdx.x; r < n; r += gridDim.x) {
+            for (int d = threadIdx.x; d < D; d += PT_THREADS) g.out[r * D + d] = 0;
+            if (threadIdx.x == 0 && g.lse) g.lse[r] = -INFINITY;
+        }
+    }
+    if ((int)blockIdx.x >= ctas) return;
+    const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < PT_RAW; i++) { mbar_init(raw_full + i, 1); mbar_init(raw_empty + i, 4); }
+        for (int i = 0; i < 2; i++) {
+            mbar_init(k_full + i, 4); mbar_init(k_empty + i, 1);
+            mbar_init(v_full + i, 4); mbar_init(v_empty + i, 1);
+            mbar_init(q_full + i, 128); mbar_init(s_full + i, 1); mbar_init(p_full + i, 128); mbar_init(o_done + i, 1);
+        }
+        *abort = 0;
+        fence_barrier_init();
+    }
+    if (warp == 2) tmem_alloc(slot, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = *slot;      // S0, S1 at columns 0 and 128 (P over their first halves), O0, O1 at 256 and 384
+
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        if (warp == 0) {
+            // ---- copies: a tile's keys, then its values
+            uint32_t st = 0, ph = 1;
+            const int pages = PT_TOK / g.page;
+            const uint32_t half = (uint32_t)(g.page * RB);
+            for (int t = lo; t < hi;) {
+                Part s;
+                find_part(g, plan, pairs, t, hi, s);
+                const int have = (s.L + g.page - 1) / g.page;
+                const int32_t *row = g.table + s.b * g.table_stride;
+                for (int tile = s.first; tile < s.last; tile++) {
+                    const int p = tile * pages + lane;
+                    int64_t pg = -1;
+                    if (lane < pages && p < have) {
+                        pg = __ldg(row + p);
+                        if (pg < 0 || pg >= g.num_pages) {
+                            atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
+                            pg = -1;
+                        }
+                    }
+                    const int n = __popc(__ballot_sync(0xFFFFFFFFu, pg >= 0));
+                    const uint8_t *src = g.cache + (pg * g.kv_heads + s.head) * (int64_t)(2 * half);
+#pragma unroll
+                    for (int w = 0; w < 2; w++) {
+                        mbar_wait_abort(raw_empty + st, ph, PT_ERR, abort);
+                        if (lane == 0) mbar_expect_tx(raw_full + st, n * half);
+                        __syncwarp();
+                        if (pg >= 0) bulk_load(s_raw + st * C::RAW + lane * half, src + w * half, half, raw_full + st);
+                        if (++st == PT_RAW) { st = 0; ph ^= 1; }
+                    }
+                }
+                t += s.last - s.first;
+            }
+        } else if (warp == 1 && elect_one()) {
+            // ---- matrix instructions
+            constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(PT_TOK >> 3) << 17) | (8u << 24);
+            constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
+            const uint64_t dq = desc_kmajor_sw128(smem_u32(s_q)), dk = desc_kmajor_sw128(smem_u32(s_k));
+            // V: rows are tokens, the contracted side; 64-element blocks of a row 16384 bytes apart
+            const uint64_t dv = (uint64_t)((smem_u32(s_v) >> 4) & 0x3FFFu) | (1024ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+            uint32_t kt = 0, vt = 0, qn[2] = {0, 0}, pn[2] = {0, 0};      // tiles of K and V; of each row tile: units, probabilities so far
+            const auto scores = [&](int x, uint32_t kb) {
+                const uint64_t a = dq + (uint64_t)(x * (C::TILE >> 4)), b = dk + (uint64_t)(kb * (C::TILE >> 4));
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    const uint32_t step = (uint32_t)((k >> 2) * 1024 + (k & 3) * 2);
+                    asm volatile(
+                        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem + x * 128),
+                        "l"(a + step), "l"(b + step), "r"(id_s), "r"(k > 0 ? 1u : 0u)
+                        : "memory");
+                }
+                tc_commit(s_full + x);
+            };
+            for (int t = lo; t < hi;) {
+                Part s;
+                find_part(g, plan, pairs, t, hi, s);
+                const int nx = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? 2 : 1;
+                const int count = s.last - s.first;
+                mbar_wait_abort(k_full + (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
+                for (int x = 0; x < nx; x++) {
+                    mbar_wait_abort(q_full + x, qn[x]++ & 1, PT_ERR, abort);
+                    tc_fence_after();
+                    scores(x, kt & 1);
+                }
+                tc_commit(k_empty + (kt & 1));
+                kt++;
+                for (int j = 0; j < count; j++, vt++) {
+                    mbar_wait_abort(v_full + (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
+                    for (int x = 0; x < nx; x++) {
+                        mbar_wait_abort(p_full + x, pn[x]++ & 1, PT_ERR, abort);
+                        tc_fence_after();
+                        const uint64_t b = dv + (uint64_t)((vt & 1) * (C::TILE >> 4));
+#pragma unroll
+                        for (int k = 0; k < PT_TOK / 16; k++)
+                            asm volatile(
+                                "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+                                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem + 256 + x * 128),
+                                "r"(tmem + x * 128 + k * 8), "l"(b + (uint64_t)(k * 128)), "r"(id_o), "r"((j > 0 || k > 0) ? 1u : 0u)
+                                : "memory");
+                        tc_commit(o_done + x);
+                        if (j + 1 < count) {
+                            if (x == 0) {
+                                mbar_wait_abort(k_full + (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
+                                tc_fence_after();
+                            }
+                            scores(x, kt & 1);      // over P: instructions run in order, the product above has read it
+                        }
+                    }
+                    tc_commit(v_empty + (vt & 1));
+                    if (j + 1 < count) {
+                        tc_commit(k_empty + (kt & 1));
+                        kt++;
+                    }
+                }
+                t += count;
+            }
+        }
+    } else if (warp < 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+        // ---- widening.  A warp takes 8 tokens at a time: 4 threads a token (2 for D = 64), 32 elements each.  The order of the lanes
+        // keeps the stores free of bank conflicts and the loads at two to a bank.
+        constexpr int PIECES = D / 32;
+        const int w = warp - 4;
+        const int r_in = D == 128 ? (lane & 3) + ((lane >> 4) << 2) : (lane & 3) + ((lane >> 3) << 2), ch = D == 128 ? ((lane >> 2) & 1) | (((lane >> 3) & 1) << 1) : (lane >> 2) & 1;
+        constexpr int PER = 32 / PIECES;         // tokens of a warp at a time
+        const int shift = 31 - __clz(g.page);
+        uint32_t st = 0, ph = 0, tiles = 0;
+        for (int t = lo; t < hi;) {
+            Part s;
+            find_part(g, plan, pairs, t, hi, s);
+            for (int tile = s.first; tile < s.last; tile++, tiles++) {
+                const int left = s.L - tile * PT_TOK;      // tokens of the tile that exist
+#pragma unroll
+                for (int v = 0; v < 2; v++) {
+                    const uint32_t buf = tiles & 1;
+                    mbar_wait_abort((v ? v_empty : k_empty) + buf, ((tiles >> 1) & 1) ^ 1, PT_ERR, abort);
+                    mbar_wait_abort(raw_full + st, ph, PT_ERR, abort);
+                    const uint32_t src = smem_u32(s_raw + st * C::RAW), dst = smem_u32((v ? s_v : s_k) + buf * C::TILE);
+#pragma unroll
+                    for (int i = 0; i < 128 / (4 * PER); i++) {
+                        const int r = (i * 4 + w) * PER + r_in, off = r & (g.page - 1);
+                        const uint32_t base = src + (uint32_t)((r >> shift) << shift) * RB;
+                        const uint4 c = lds_v4(base + off * (D / 2) + ch * 16);
+                        uint32_t two = lds_u16(base + (D / 2 << shift) + off * (D / 16) + ch * 2);
+                        if (r >= left) two = 0;            // whatever the slots behind the last token hold, it counts as zero
+                        const uint32_t sc = e4m3x2_to_half2(two), s0 = __byte_perm(sc, sc, 0x1010), s1 = __byte_perm(sc, sc, 0x3232);
+                        const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            uint32_t h[4];
+                            e2m1x8_to_half(word[j], h);
+#pragma unroll
+                            for (int u = 0; u < 4; u++) h[u] = hmul2_bits(h[u], j < 2 ? s0 : s1);
+                            sts_v4(dst + tile_at(r, ch * 4 + j), make_uint4(h[0], h[1], h[2], h[3]));
+                        }
+                    }
+                    proxy_fence();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(raw_empty + st);
+                        mbar_arrive((v ? v_full : k_full) + buf);
+                    }
+                    if (++st == PT_RAW) { st = 0; ph ^= 1; }
+                }
+            }
+            t += s.last - s.first;
+        }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
+        // ---- softmax of row tile x, one thread a row
+        const int x = (warp - 8) >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
+        const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
+        uint32_t sn = 0, on = 0;        // scores, products so far
+        for (int t = lo; t < hi;) {
+            Part s;
+            find_part(g, plan, pairs, t, hi, s);
+            const int64_t rows = (int64_t)s.n * g.group, r = (int64_t)s.qt * PT_ROWS + x * 128 + row;
+            const bool live = r < rows, idle = rows - (int64_t)s.qt * PT_ROWS <= x * 128;      // idle: no row of this tile exists
+            const int i = live ? (int)(r / g.group) : 0, h = s.head * g.group + (live ? (int)(r - (int64_t)i * g.group) : 0);
+            const int limit = live ? s.L - s.n + i + 1 : 0;
+            float factor = 0.0f;
+            if (!idle) {
+                uint4 w[D / 8];
+                uint32_t acc = 0;
+                const uint16_t *src = g.q + (int64_t)(s.q0 + i) * g.q_token + h * g.q_head;
+#pragma unroll
+                for (int j = 0; j < D / 8; j++) {
+                    w[j] = live ? ld_v4(src + 8 * j) : make_uint4(0, 0, 0, 0);
+                    acc = absmax2_acc(absmax2_acc(absmax2_acc(absmax2_acc(acc, w[j].x), w[j].y), w[j].z), w[j].w);
+                }
+                float mult, back;
+                q_power(f2u(hmax_halves_f32(acc)), mult, back);
+                factor = back * (g.scale_log2 * k_outer);
+                factor = factor < 1e-37f ? 1e-37f : factor;       // not zero: -inf of a hidden key has to stay
+                const uint32_t dst = smem_u32(s_q + x * C::TILE);
+#pragma unroll
+                for (int j = 0; j < D / 8; j++)
+                    sts_v4(dst + tile_at(row, j),
+                           make_uint4(pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult), pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult),
+                                      pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult), pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult)));
+                proxy_fence();
+                mbar_arrive(q_full + x);
+                float m = -INFINITY, l = 0.0f;
+                for (int tile = s.first; tile < s.last; tile++) {
+                    mbar_wait_abort(s_full + x, sn++ & 1, PT_ERR, abort);
+                    tc_fence_after();
+                    uint32_t v[4][32];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) tmem_ld32(t_s + 32 * c, v[c]);
+                    tmem_wait_ld();
+                    const int see = limit - tile * PT_TOK;       // columns that the row sees
+                    if (__any_sync(0xFFFFFFFFu, see < PT_TOK)) {
+#pragma unroll
+                        for (int c = 0; c < 4; c++)
+#pragma unroll
+                            for (int j = 0; j < 32; j++)
+                                if (32 * c + j >= see) v[c][j] = 0xFF800000u;
+                    }
+                    float top[4];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        top[c] = u2f(v[c][0]);
+#pragma unroll
+                        for (int j = 1; j < 32; j++) top[c] = fmaxf(top[c], u2f(v[c][j]));
+                    }
+                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
+                    const bool grow = most - m > 8.0f;           // (from -inf: always, once the row sees a key)
+                    if (__any_sync(0xFFFFFFFFu, grow)) {
+                        const float up = grow ? most : m, a = grow ? ex2(m - up) : 1.0f;
+                        m = up;
+                        l *= a;
+                        if (tile > s.first) {
+                            mbar_wait_abort(o_done + x, (on - 1) & 1, PT_ERR, abort);
+                            tc_fence_after();
+#pragma unroll
+                            for (int c = 0; c < D; c += 16) {
+                                uint32_t o[16];
+                                tmem_ld16(t_o + c, o);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 16; j++) o[j] = f2u(u2f(o[j]) * a);
+                                tmem_st16(t_o + c, o);
+                            }
+                        }
+                    }
+                    const float base = m == -INFINITY ? 0.0f : m;
+                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int c = 0; c < 4; c++) {
+                        uint32_t p[16];
+#pragma unroll
+                        for (int j = 0; j < 16; j++) {
+                            // (factor is finite and positive: -inf stays -inf and exp2 gives 0)
+                            const float e0 = ex2(fmaf(u2f(v[c][2 * j]), factor, -base)), e1 = ex2(fmaf(u2f(v[c][2 * j + 1]), factor, -base));
+                            sum[j & 3] += e0 + e1;
+                            p[j] = pack_half2(e0, e1);
+                        }
+                        tmem_st16(t_s + 16 * c, p);
+                    }
+                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(p_full + x);
+                    on++;
+                }
+                mbar_wait_abort(o_done + x, (on - 1) & 1, PT_ERR, abort);
+                tc_fence_after();
+                const bool whole = s.first == 0 && s.last == s.tiles;
+                const float scale = l == 0.0f ? 0.0f : __fdividef(v_outer, l);
+                const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + h;
+                float *part = g.part + (size_t)(2 * blockIdx.x + (t == lo ? 0 : 1)) * prompt_part_floats<D>();
+#pragma unroll
+                for (int c = 0; c < D; c += 16) {
+                    uint32_t o[16];
+                    tmem_ld16(t_o + c, o);
+                    tmem_wait_ld();
+                    if (whole) {
+                        uint32_t y[8];
+#pragma unroll
+                        for (int j = 0; j < 8; j++) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(l == 0.0f ? 0.0f : u2f(o[2 * j]) * scale, l == 0.0f ? 0.0f : u2f(o[2 * j + 1]) * scale);
+                            y[j] = *reinterpret_cast<const uint32_t *>(&b);
+                        }
+                        if (live) {
+                            uint4 *dst = reinterpret_cast<uint4 *>(g.out + at * D + c);
+                            dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
+                            dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+                        }
+                    } else {
+                        uint4 *dst = reinterpret_cast<uint4 *>(part + (x * 128 + row) * D + c);
+#pragma unroll
+                        for (int j = 0; j < 4; j++) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                    }
+                }
+                if (!whole) reinterpret_cast<float2 *>(part + PT_ROWS * D)[x * 128 + row] = make_float2(m, l);
+                else if (live && g.lse) g.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                tc_fence_before();       // the next unit's products write O
+            }
+            t += s.last - s.first;
+        }
+    }
+    __syncwarp();
+    tc_fence_before();
+    __syncthreads();
+    if (warp == 2) {
+        tc_fence_after();
+        tmem_free(tmem, 512);
+    }
+}
+
+// Joins the units that span CTAs.  CTA (i, y) takes 32 rows of the unit in which CTA i begins, if that begins in CTA i - 1.
+template <int D>
+__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs g, const PromptPlan plan, int grid)
+{
+    pdl_wait();
+    const int pairs = plan.count[0], total = plan.prefix[pairs], ctas = min(grid, total), c = blockIdx.x;
+    if (c < 1 || c >= ctas) return;
+    const int lo = (int)((int64_t)total * c / ctas);
+    Part s;
+    find_part(g, plan, pairs, lo, total, s);
+    if (s.unit_first == lo) return;
+    const int i0 = (int)((((int64_t)s.unit_first + 1) * ctas - 1) / total), i1 = (int)((((int64_t)s.unit_first + s.tiles) * ctas - 1) / total);
+    if (i0 != c - 1) return;
+    const int second = (int)((int64_t)total * i0 / ctas) < s.unit_first ? 1 : 0;
+    const int64_t rows = (int64_t)s.n * g.group;
+    constexpr int TPR = D / 4, STEP = 256 / TPR;
+    const int d = threadIdx.x % TPR * 4;
+    for (int k = threadIdx.x / TPR; k < 32; k += STEP) {
+        const int row = blockIdx.y * 32 + k;
+        const int64_t r = (int64_t)s.qt * PT_ROWS + row;
+        if (r >= rows) break;
+        float top = -INFINITY, den = 0.0f;
+        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j = i0; j <= i1; j++) {
+            const float *part = g.part + (size_t)(2 * j + (j == i0 ? second : 0)) * prompt_part_floats<D>();
+            const float2 w = reinterpret_cast<const float2 *>(part + PT_ROWS * D)[row];
+            const float4 v = *reinterpret_cast<const float4 *>(part + row * D + d);
+            const float up = fmaxf(top, w.x), a = top == -INFINITY ? 0.0f : ex2(top - up), b = w.x == -INFINITY ? (w.y == 0.0f ? 0.0f : 1.0f) : ex2(w.x - up);
+            const bool first = top == -INFINITY && den == 0.0f;
+            den = (first ? 0.0f : den * a) + w.y * b;
+            sum.x = (first ? 0.0f : sum.x * a) + v.x * b; sum.y = (first ? 0.0f : sum.y * a) + v.y * b;
+            sum.z = (first ? 0.0f : sum.z * a) + v.z * b; sum.w = (first ? 0.0f : sum.w * a) + v.w * b;
+            top = up;
+        }
+        const int i = (int)(r / g.group);
+        const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + s.head * g.group + (r - (int64_t)i * g.group);
+        const float inv = den == 0.0f ? 0.0f : __fdividef(__ldg(g.v_outer), den);
+        const __nv_bfloat162 y0 = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.x * inv, den == 0.0f ? 0.0f : sum.y * inv);
+        const __nv_bfloat162 y1 = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.z * inv, den == 0.0f ? 0.0f : sum.w * inv);
+        *reinterpret_cast<uint2 *>(g.out + at * D + d) = make_uint2(*reinterpret_cast<const uint32_t *>(&y0), *reinterpret_cast<const uint32_t *>(&y1));
+        if (d == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
+    }
+}
+
+bool prompt_fits(int64_t rows, int group, int seqs, int kv_heads, int64_t cached)
+{
+    return prompt_max_pairs(rows, group, seqs) * kv_heads <= 0x7FFFFFFF / ((cached + PT_TOK - 1) / PT_TOK + 1);
+}
+size_t prompt_workspace_bytes(int64_t rows, int group, int seqs, int head_dim)
+{
+    return (prompt_plan_bytes(prompt_max_pairs(rows, group, seqs)) + 15) / 16 * 16 + (size_t)2 * sm_count() * PT_ROWS * (head_dim + 2) * 4;
+}
+
+template <int D>
+static int launch(AttnArgs g, void *ws, cudaStream_t st)
+{
+    using C = PromptCfg<D>;
+    static PerDeviceFlag done;
+    const int dev = current_device_slot();
+    if (dev < 0) return QCC_ERR_ARG;
+    if (!done.get(dev)) {
+        cudaError_t e = cudaFuncSetAttribute(kv_prompt_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return (int)e;
+        // the warps re-divide the registers of the launch, 256 threads with 72 and 256 with 184: it has to bring as many
+        cudaFuncAttributes at;
+        if ((e = cudaFuncGetAttributes(&at, kv_prompt_kernel<D>)) != cudaSuccess) return (int)e;
+        if (at.numRegs * PT_THREADS < 256 * (72 + 184)) return (int)cudaErrorInvalidConfiguration;
+        done.set(dev);
+    }
+    const int64_t max_pairs = prompt_max_pairs(g.rows, g.group, g.seqs);
+    const PromptPlan plan = prompt_plan(ws, max_pairs);
+    g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + (prompt_plan_bytes(max_pairs) + 15) / 16 * 16);
+    kv_prompt_plan_kernel<<<1, 1024, 0, st>>>(g, plan);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return (int)e;
+    const int grid = sm_count();
+    e = launch_maybe_pdl(kv_prompt_kernel<D>, dim3(grid), dim3(PT_THREADS), C::SMEM, st, true, g, plan);
+    if (e != cudaSuccess) return (int)e;
+    return (int)launch_maybe_pdl(kv_prompt_join_kernel<D>, dim3(grid, PT_ROWS / 32), dim3(256), 0, st, true, g, plan, grid);
+}
+
+int prompt_launch(const AttnArgs &g, int head_dim, void *ws, cudaStream_t st)
+{
+    return head_dim == 128 ? launch<128>(g, ws, st) : launch<64>(g, ws, st);
+}
+
+}  // namespace qcc
+
+extern "C" int qcc_kv_prompt_device_error(unsigned int *out) { return qcc::read_clear_device_error(out); }

@@ -540,7 +540,7 @@ std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_cuda(const at::Tensor &q, 
         lse.fill_(-std::numeric_limits<float>::infinity());
         return {out, lse};
     }
-    const size_t ws_bytes = qcc_nvfp4_kv_attention_workspace_bytes((int)std::min<int64_t>(seqs, 1 << 20), (int)max_q, (int)hq, c.heads, (int)D);
+    const size_t ws_bytes = qcc_nvfp4_kv_attention_workspace_bytes(rows, (int)std::min<int64_t>(seqs, 1 << 20), (int)max_q, (int)hq, c.heads, (int)D);
     at::Tensor ws = at::empty({(int64_t)ws_bytes}, cache.options());
     a.q = q.data_ptr();
     a.q_stride[0] = q.stride(0); a.q_stride[1] = q.stride(1);

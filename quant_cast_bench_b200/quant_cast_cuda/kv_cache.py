@@ -152,7 +152,7 @@ def nvfp4_kv_attention_cuda(q, cache, block_table, kv_lens, k_outer, v_outer, cu
     lse = torch.empty((rows, hq), dtype=torch.float32, device=q.device)
     if rows == 0 or seqs == 0:
         return out.zero_(), lse.fill_(-math.inf)
-    nws = lib.qcc_nvfp4_kv_attention_workspace_bytes(seqs, max_q, hq, heads, D)
+    nws = lib.qcc_nvfp4_kv_attention_workspace_bytes(rows, seqs, max_q, hq, heads, D)
     ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
     a = L.KvAttentionArgs(_p(q), (ctypes.c_int64 * 2)(*q.stride()[:2]), rows, _p(cache), cache.shape[0], _p(block_table), block_table.stride(0),
                           block_table.shape[1], _p(kv_lens), _p(cu_q), seqs, max_q, _p(k_outer), _p(v_outer),
