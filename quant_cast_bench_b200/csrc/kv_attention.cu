@@ -49,11 +49,10 @@ template <int D, int NT> struct SplitCfg {
 template <int D, int NT> __host__ __device__ constexpr int part_floats() { return NT * 8 * (D + 2); }   // sums (NT * 8, D), then (maximum, denominator) of each row
 
 struct Segment {
-    int b, q0, n, L, head, rt, first, last, unit_last;   // first, last: tiles of the unit; unit_last: flat number of the tile behind it
+    int b, q0, n, L, head, first, last, unit_last;   // first, last: tiles of the unit; unit_last: flat number of the tile behind it
 };
 
 // the segment that starts at flat tile t: its unit's tiles [first, last) within hi
-template <int NT>
 __device__ __forceinline__ void find_segment(const AttnArgs &g, const int32_t *prefix, int t, int hi, Segment &s)
 {
     int lo = 0, up = g.seqs - 1;      // last b with prefix[b] <= t (t < total, so it has tiles)
@@ -63,21 +62,11 @@ __device__ __forceinline__ void find_segment(const AttnArgs &g, const int32_t *p
     }
     s.b = lo;
     seq_of(g, lo, s.q0, s.n, s.L);
-    const int kvt = (s.L + SP_TOK - 1) / SP_TOK, rts = (s.n * g.group + NT * 8 - 1) / (NT * 8);
-    const int local = t - prefix[lo], unit = local / kvt;
-    s.head = unit / rts;
-    s.rt = unit - s.head * rts;
-    s.first = local - unit * kvt;
+    const int kvt = (s.L + SP_TOK - 1) / SP_TOK, local = t - prefix[lo];
+    s.head = local / kvt;
+    s.first = local - s.head * kvt;
     s.last = min(kvt, s.first + hi - t);
-    s.unit_last = prefix[lo] + (unit + 1) * kvt;
-}
-// tiles that some row of the row tile sees
-template <int NT>
-__device__ __forceinline__ int seen_tiles(const AttnArgs &g, const Segment &s)
-{
-    const int i = min(s.n - 1, ((s.rt + 1) * NT * 8 - 1) / g.group);
-    const int end = s.L - s.n + i + 1;
-    return min(s.last, (max(end, 0) + SP_TOK - 1) / SP_TOK);
+    s.unit_last = prefix[lo] + (s.head + 1) * kvt;
 }
 
 template <int D, int NT>
@@ -98,15 +87,19 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         for (int i = 0; i < C::STAGES; i++) mbar_init(full + i, 1);
     if (threadIdx.x == 0) prefix[0] = 0;
     fence_barrier_init();
+    pdl_trigger();
+    pdl_wait();
     // tiles of each sequence, summed up
     int carry = 0;
+    bool gap = false;
     for (int b0 = 0; b0 < g.seqs; b0 += SP_THREADS) {
         const int b = b0 + threadIdx.x;
         int v = 0;
         if (b < g.seqs) {
             int q0, n, L;
             seq_of(g, b, q0, n, L);
-            v = g.kv_heads * ((n * g.group + NT * 8 - 1) / (NT * 8)) * ((L + SP_TOK - 1) / SP_TOK);
+            gap |= n && !L;
+            v = n ? g.kv_heads * ((L + SP_TOK - 1) / SP_TOK) : 0;
         }
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -124,10 +117,24 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         carry = all;
         __syncthreads();
     }
+    const bool empty = __syncthreads_or(gap);      // some sequence has queries and no tokens
     const int total = carry, ctas = min((int)gridDim.x, total);
-    if (blockIdx.x == 0)
-        for (int i = threadIdx.x; i <= g.seqs; i += SP_THREADS) g.prefix[i] = prefix[i];
-    if ((int)blockIdx.x >= ctas) return;
+    if (empty) {
+        for (int b = blockIdx.x; b < g.seqs; b += gridDim.x) {
+            if (prefix[b + 1] != prefix[b]) continue;
+            int q0, n, L;
+            seq_of(g, b, q0, n, L);
+            fill_rows<D>(g, q0, n, 0, 1);
+        }
+    }
+    if (g.cu_q) {
+        const int64_t first = max(__ldg(g.cu_q + g.seqs), 0);
+        fill_rows<D>(g, first, g.rows - first, blockIdx.x, gridDim.x);
+    }
+    if ((int)blockIdx.x >= ctas) {
+        if (threadIdx.x == 0) g.seams[2 * blockIdx.x].x = -1;
+        return;
+    }
     const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
 
     // ---- fetching: the warp's tokens of tile after tile, C::STAGES ahead of their use.  The pages of the next fetch are looked up
@@ -146,9 +153,9 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                 f.t += f.s.last - f.s.first;
             }
             if (f.t >= hi) return;
-            find_segment<NT>(g, prefix, f.t, hi, f.s);
+            find_segment(g, prefix, f.t, hi, f.s);
             f.tile = f.s.first - 1;
-            f.end = seen_tiles<NT>(g, f.s);
+            f.end = f.s.last;
             fresh = false;
         }
         const int tok = f.tile * SP_TOK + warp * SP_WTOK + (lane & 1) * 16;
@@ -194,16 +201,17 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     uint32_t stage = 0, phase = 0;
     for (int t = lo; t < hi;) {
         Segment s;
-        find_segment<NT>(g, prefix, t, hi, s);
-        const int end = seen_tiles<NT>(g, s);
+        find_segment(g, prefix, t, hi, s);
+        const int end = s.last;
         const int rows = s.n * g.group;
+        if (t == lo && threadIdx.x == 0) note_seam(g, s.first ? t - s.first : -1, s.unit_last, total, rows, s.q0, s.head, 0);
 
         uint32_t qf[NT][2 * KW * 2];    // row gr of each n tile, elements of this thread
         float factor[NT][2];            // score -> log2 units, columns 2c and 2c + 1
         int limit[NT][2];               // keys that the column sees
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int r = s.rt * NT * 8 + nt * 8 + gr;
+            const int r = nt * 8 + gr;
             const int i = r / g.group, h = s.head * g.group + r - i * g.group;
             uint4 w[KW];
             uint32_t acc = 0;
@@ -227,7 +235,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
 #pragma unroll
             for (int x = 0; x < 2; x++) {
                 factor[nt][x] = __shfl_sync(0xFFFFFFFFu, back, (2 * c + x) * 4) * (g.scale_log2 * k_outer);
-                const int rc = s.rt * NT * 8 + nt * 8 + 2 * c + x;
+                const int rc = nt * 8 + 2 * c + x;
                 limit[nt][x] = rc < rows ? s.L - s.n + rc / g.group + 1 : 0;
             }
         }
@@ -378,7 +386,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                 }
             }
         };
-        const int clear = s.L - s.n + s.rt * NT * 8 / g.group + 1;      // keys that the row tile's first row, and so every row, sees
+        const int clear = s.L - s.n + 1;      // keys that every row sees
 
         for (int tile = s.first; tile < end; tile++) {
             mbar_wait(full + stage, phase, KV_ATTN_ERR);
@@ -442,7 +450,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                     den += v.y * (v.x == -INFINITY ? 1.0f : ex2(v.x - top));
                 }
                 if (whole) {
-                    const int r = s.rt * NT * 8 + qi;
+                    const int r = qi;
                     if (r < rows) {
                         const int i = r / g.group;
                         const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + s.head * g.group + r - i * g.group;
@@ -461,80 +469,8 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     }
 }
 
-// One CTA per unit (sequence, head, row tile): joins the partial sums of a unit that several CTAs worked on, in the order of
-// its tokens, and fills the rows of a unit without tokens.  A thread has four neighbouring elements of a row, and the weights of
-// the parts are worked out once, so the loads of the sums do not wait for one another (a thread an element that found the maximum
-// first took 74 us to join 16 units of 19 parts, this takes 5).
-constexpr int JOIN_MAX = 1024;     // parts of a unit: at most one for each CTA of the first kernel
 template <int D, int NT>
-__global__ void __launch_bounds__(NT * 2 * D) kv_attn_join_kernel(const AttnArgs g, int grid, int max_rts, int units)
-{
-    constexpr int ROWS = NT * 8, THREADS = ROWS * D / 4;
-    __shared__ float2 ml[JOIN_MAX];
-    pdl_wait();
-    if ((int)blockIdx.x >= units) {
-        // rows behind the last sequence
-        const int64_t first = (int64_t)max(__ldg(g.cu_q + g.seqs), 0) * g.q_heads, n = g.rows * g.q_heads;
-        for (int64_t r = first + blockIdx.x - units; r < n; r += gridDim.x - units) {
-            for (int d = threadIdx.x; d < D; d += THREADS) g.out[r * D + d] = 0;
-            if (threadIdx.x == 0 && g.lse) g.lse[r] = -INFINITY;
-        }
-        return;
-    }
-    const int rt = blockIdx.x % max_rts, head = blockIdx.x / max_rts % g.kv_heads, b = blockIdx.x / max_rts / g.kv_heads;
-    int q0, n, L;
-    seq_of(g, b, q0, n, L);
-    const int rows = n * g.group, rts = (rows + ROWS - 1) / ROWS, kvt = (L + SP_TOK - 1) / SP_TOK;
-    if (rt >= rts) return;
-    const int total = g.prefix[g.seqs], ctas = min(grid, total);
-    int i0 = 0, parts = 0, first = 0;
-    if (kvt > 0) {
-        first = g.prefix[b] + (head * rts + rt) * kvt;
-        // CTA i works on tiles [total * i / ctas, total * (i + 1) / ctas): tile t belongs to ((t + 1) * ctas - 1) / total
-        i0 = (int)((((int64_t)first + 1) * ctas - 1) / total);
-        parts = (int)((((int64_t)first + kvt) * ctas - 1) / total) - i0 + 1;
-        if (parts == 1) return;
-    }
-    // the slot of part j: the second one of the CTA whose first tile is not this unit's
-    const int second = kvt > 0 && (int)((int64_t)total * i0 / ctas) < first ? 1 : 0;
-    const float *base = g.part + (size_t)2 * i0 * part_floats<D, NT>();
-    const int row = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4, r = rt * ROWS + row;
-    float top = -INFINITY, den = 0.0f;
-    float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    for (int j0 = 0; j0 < parts; j0 += JOIN_MAX / ROWS) {
-        const int some = min(parts - j0, JOIN_MAX / ROWS);
-        __syncthreads();
-        for (int e = threadIdx.x; e < some * ROWS; e += THREADS) {
-            const int j = j0 + e / ROWS;
-            ml[e] = reinterpret_cast<const float2 *>(base + (size_t)(2 * j + (j == 0 ? second : 0)) * part_floats<D, NT>() + ROWS * D)[e % ROWS];
-        }
-        __syncthreads();
-        float up = top;
-        for (int j = 0; j < some; j++) up = fmaxf(up, ml[j * ROWS + row].x);
-        const float old = top == -INFINITY ? 1.0f : ex2(top - up);
-        top = up;
-        den *= old; sum.x *= old; sum.y *= old; sum.z *= old; sum.w *= old;
-#pragma unroll 8
-        for (int j = 0; j < some; j++) {
-            const float4 v = *reinterpret_cast<const float4 *>(base + (size_t)(2 * (j0 + j) + (j0 + j == 0 ? second : 0)) * part_floats<D, NT>() + row * D + d);
-            const float2 w = ml[j * ROWS + row];
-            const float a = w.x == -INFINITY ? 1.0f : ex2(w.x - top);     // a part that saw nothing holds zeros (or NaN, which stays)
-            den += w.y * a;
-            sum.x += v.x * a; sum.y += v.y * a; sum.z += v.z * a; sum.w += v.w * a;
-        }
-    }
-    if (r >= rows) return;
-    const int i = r / g.group;
-    const int64_t at = (int64_t)(q0 + i) * g.q_heads + head * g.group + r - i * g.group;
-    const float inv = den == 0.0f ? 0.0f : __fdividef(__ldg(g.v_outer), den);
-    const __nv_bfloat162 lo = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.x * inv, den == 0.0f ? 0.0f : sum.y * inv);
-    const __nv_bfloat162 hi = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.z * inv, den == 0.0f ? 0.0f : sum.w * inv);
-    *reinterpret_cast<uint2 *>(g.out + at * D + d) = make_uint2(*reinterpret_cast<const uint32_t *>(&lo), *reinterpret_cast<const uint32_t *>(&hi));
-    if (d == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
-}
-
-template <int D, int NT>
-static int split_launch(const AttnArgs &g, int max_q, cudaStream_t st)
+static int split_launch(const AttnArgs &g, cudaStream_t st)
 {
     using C = SplitCfg<D, NT>;
     static PerDeviceFlag done;
@@ -546,13 +482,9 @@ static int split_launch(const AttnArgs &g, int max_q, cudaStream_t st)
         done.set(dev);
     }
     const int grid = sm_count() * C::CTAS;
-    kv_attn_split_kernel<D, NT><<<grid, SP_THREADS, C::FIXED + (g.seqs + 1) * 4, st>>>(g);
-    cudaError_t e = cudaGetLastError();
+    cudaError_t e = launch_maybe_pdl(kv_attn_split_kernel<D, NT>, dim3(grid), dim3(SP_THREADS), C::FIXED + (g.seqs + 1) * 4, st, true, g);
     if (e != cudaSuccess) return (int)e;
-    const int max_rts = (int)(((int64_t)max_q * g.group + NT * 8 - 1) / (NT * 8));
-    const int units = g.seqs * g.kv_heads * max_rts;
-    const int behind = g.cu_q ? 32 : 0;      // CTAs for the rows behind the last sequence
-    return (int)launch_maybe_pdl(kv_attn_join_kernel<D, NT>, dim3((unsigned)(units + behind)), dim3(NT * 2 * D), 0, st, true, g, grid, max_rts, units);
+    return (int)launch_maybe_pdl(kv_join_kernel<D, 4, 8, 8 * D>, dim3(grid, NT), dim3(8 * D), 0, st, true, g, grid, NT * 8);
 }
 
 // how the rows of a sequence and kv head are tiled: 8 * nt rows
@@ -571,8 +503,7 @@ extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int64_t rows, int seqs,
     if (rows < 0 || seqs < 0 || max_q < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
     if (many_queries(max_q, q_heads / kv_heads)) return prompt_workspace_bytes(rows, q_heads / kv_heads, seqs, head_dim);
     const int nt = row_tiles_of((int64_t)max_q * (q_heads / kv_heads));
-    const size_t prefix = (((size_t)seqs + 1) * 4 + 15) / 16 * 16;
-    return prefix + (size_t)2 * sm_count() * (nt == 1 ? 4 : 2) * nt * 8 * (head_dim + 2) * 4;
+    return (size_t)2 * sm_count() * (nt == 1 ? 4 : 2) * (16 + nt * 8 * (head_dim + 2) * 4);
 }
 
 extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *workspace, size_t workspace_bytes, void *stream)
@@ -601,8 +532,8 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     g.k_outer = p->k_outer; g.v_outer = p->v_outer;
     g.out = static_cast<uint16_t *>(p->out);
     g.lse = p->lse;
-    g.prefix = static_cast<int32_t *>(workspace);
-    g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(workspace) + (((size_t)p->seqs + 1) * 4 + 15) / 16 * 16);
+    g.seams = static_cast<int4 *>(workspace);
+    g.part = reinterpret_cast<float *>(g.seams + 2 * sm_count() * (nt == 1 ? 4 : 2));
     g.q_token = p->q_stride[0]; g.q_head = p->q_stride[1];
     g.table_stride = p->table_stride; g.num_pages = p->num_pages; g.rows = p->rows;
     g.scale_log2 = p->scale * LOG2E;
@@ -610,6 +541,6 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (many_queries(max_q, group)) return prompt_launch(g, p->head_dim, workspace, st);
     if (p->head_dim == 128)
-        return nt == 1 ? split_launch<128, 1>(g, max_q, st) : nt == 2 ? split_launch<128, 2>(g, max_q, st) : split_launch<128, 4>(g, max_q, st);
-    return nt == 1 ? split_launch<64, 1>(g, max_q, st) : nt == 2 ? split_launch<64, 2>(g, max_q, st) : split_launch<64, 4>(g, max_q, st);
+        return nt == 1 ? split_launch<128, 1>(g, st) : nt == 2 ? split_launch<128, 2>(g, st) : split_launch<128, 4>(g, st);
+    return nt == 1 ? split_launch<64, 1>(g, st) : nt == 2 ? split_launch<64, 2>(g, st) : split_launch<64, 4>(g, st);
 }

@@ -21,7 +21,7 @@ namespace qcc {
 //
 // Roles: warp 0 copies, warp 1 issues the matrix instructions, warps 4-7 widen, warps 8-11 and 12-15 are the softmax of the two
 // row tiles.  All (unit, tile) pairs are numbered, by a first small kernel, and dealt out evenly to one CTA per SM, whatever the lengths and however
-// many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, joined by a third kernel in a fixed order.
+// many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3;
 constexpr unsigned int PT_ERR = 9u;    // a barrier wait of this kernel ran out
@@ -35,18 +35,20 @@ template <int D> struct PromptCfg {
 
 // ---- numbering: prefix[p] = tiles of all (sequence, row tile) pairs before p, times the kv heads; pairs[p] = (sequence, row tile)
 struct PromptPlan {
-    int32_t *count;      // [0]: pairs
+    int32_t *count;      // [0]: pairs, [1]: those without tiles
     int2 *pairs;
     int32_t *prefix;     // pairs + 1
+    int32_t *empty;      // the pairs without tiles
 };
 __host__ __device__ __forceinline__ int64_t prompt_max_pairs(int64_t rows, int group, int seqs) { return rows * group / PT_ROWS + seqs; }
-static size_t prompt_plan_bytes(int64_t max_pairs) { return 16 + (size_t)(max_pairs + 1) * 16; }
+static size_t prompt_plan_bytes(int64_t max_pairs) { return 16 + (size_t)(max_pairs + 1) * (8 + 4 + 4); }
 static PromptPlan prompt_plan(void *ws, int64_t max_pairs)
 {
     PromptPlan p;
     p.count = static_cast<int32_t *>(ws);
     p.pairs = reinterpret_cast<int2 *>(p.count + 4);
     p.prefix = reinterpret_cast<int32_t *>(p.pairs + max_pairs + 1);
+    p.empty = p.prefix + max_pairs + 1;
     return p;
 }
 // tiles of row tile qt of a sequence: up to the last key that its last row sees
@@ -85,6 +87,8 @@ __device__ __forceinline__ int block_scan(int v, int32_t *wsum, int &all)     //
 __global__ void __launch_bounds__(1024) kv_prompt_plan_kernel(const AttnArgs g, const PromptPlan plan)
 {
     __shared__ int32_t start[KV_MAX_SEQS + 1], wsum[32];
+    pdl_trigger();
+    pdl_wait();
     int carry = 0;
     for (int b0 = 0; b0 < g.seqs; b0 += 1024) {
         const int b = b0 + threadIdx.x;
@@ -97,7 +101,7 @@ __global__ void __launch_bounds__(1024) kv_prompt_plan_kernel(const AttnArgs g, 
     if (threadIdx.x == 0) start[0] = 0;
     __syncthreads();
     const int pairs = min((int64_t)carry, prompt_max_pairs(g.rows, g.group, g.seqs));     // (more only if offsets overlap)
-    int tiles = 0;
+    int tiles = 0, without = 0;
     for (int p0 = 0; p0 < pairs; p0 += 1024) {
         const int p = p0 + threadIdx.x;
         int v = 0, all;
@@ -115,17 +119,34 @@ __global__ void __launch_bounds__(1024) kv_prompt_plan_kernel(const AttnArgs g, 
         const int s = block_scan(v, wsum, all);
         if (p < pairs) plan.prefix[p + 1] = tiles + s;
         tiles += all;
+        const bool none = p < pairs && v == 0;
+        if (__syncthreads_or(none)) {
+            const int e = block_scan(none ? 1 : 0, wsum, all);
+            if (none) plan.empty[without + e - 1] = p;
+            without += all;
+        }
     }
     if (threadIdx.x == 0) {
         plan.prefix[0] = 0;
         plan.count[0] = pairs;
+        plan.count[1] = without;
     }
 }
 
 // ---- the work of a CTA: parts of units
 struct Part {
     int b, q0, n, L, qt, head, tiles, first, last, unit_first;     // tiles: of the unit; first, last: of this part; unit_first: flat
+    int pair;
 };
+__device__ __forceinline__ void read_pair(const AttnArgs &g, const PromptPlan &plan, Part &s)
+{
+    const int2 pr = plan.pairs[s.pair];
+    s.b = pr.x;
+    s.qt = pr.y;
+    s.tiles = (plan.prefix[s.pair + 1] - plan.prefix[s.pair]) / g.kv_heads;
+    seq_of(g, s.b, s.q0, s.n, s.L);
+}
+// the part that starts at flat tile t, by search
 __device__ __forceinline__ void find_part(const AttnArgs &g, const PromptPlan &plan, int pairs, int t, int hi, Part &s)
 {
     int lo = 0, up = pairs - 1;       // the last pair with prefix <= t, which has tiles
@@ -133,17 +154,34 @@ __device__ __forceinline__ void find_part(const AttnArgs &g, const PromptPlan &p
         const int mid = (lo + up + 1) >> 1;
         if (plan.prefix[mid] <= t) lo = mid; else up = mid - 1;
     }
-    const int2 pr = plan.pairs[lo];
+    s.pair = lo;
+    read_pair(g, plan, s);
     const int start = plan.prefix[lo];
-    s.b = pr.x;
-    s.qt = pr.y;
-    seq_of(g, s.b, s.q0, s.n, s.L);
-    s.tiles = (plan.prefix[lo + 1] - start) / g.kv_heads;
     s.head = (t - start) / s.tiles;
     s.unit_first = start + s.head * s.tiles;
     s.first = t - s.unit_first;
     s.last = min(s.tiles, s.first + hi - t);
 }
+// the part behind it, at t < hi: the first of the next unit
+__device__ __forceinline__ void next_part(const AttnArgs &g, const PromptPlan &plan, int t, int hi, Part &s)
+{
+    if (++s.head == g.kv_heads) {
+        s.head = 0;
+        do {
+            s.pair++;
+            read_pair(g, plan, s);
+        } while (s.tiles == 0);
+    }
+    s.unit_first = t;
+    s.first = 0;
+    s.last = min(s.tiles, hi - t);
+}
+// for (Part s ...) over the parts of [lo, hi)
+#define QCC_FOR_PARTS(s, t)                                             \
+    Part s;                                                             \
+    int t = lo;                                                         \
+    for (find_part(g, plan, pairs, t, hi, s); t < hi; t += s.last - s.first, t < hi ? next_part(g, plan, t, hi, s) : (void)0)
+
 template <int D> __host__ __device__ constexpr int prompt_part_floats() { return PT_ROWS * (D + 2); }
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
@@ -173,31 +211,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
     volatile uint32_t *abort = slot + 1;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+    pdl_trigger();
     pdl_wait();      // the numbering
     const int pairs = plan.count[0], total = plan.prefix[pairs], ctas = min((int)gridDim.x, total);
 
     // rows that see no key, and rows behind the last sequence
-    for (int p = blockIdx.x; p < pairs; p += gridDim.x) {
-        if (plan.prefix[p + 1] != plan.prefix[p]) continue;
-        const int2 pr = plan.pairs[p];
+    for (int e = blockIdx.x; e < plan.count[1] * 8; e += gridDim.x) {
+        const int2 pr = plan.pairs[plan.empty[e >> 3]];
         int q0, n, L;
         seq_of(g, pr.x, q0, n, L);
-        const int64_t rows = (int64_t)n * g.group, r0 = (int64_t)pr.y * PT_ROWS, r1 = min(rows, r0 + PT_ROWS);
-        for (int64_t e = threadIdx.x; e < (r1 - r0) * g.kv_heads * D; e += PT_THREADS) {
-            const int64_t x = e / D, r = r0 + x / g.kv_heads;
-            const int64_t at = (q0 + r / g.group) * g.q_heads + x % g.kv_heads * g.group + r % g.group;
-            g.out[at * D + e % D] = 0;
-            if (e % D == 0 && g.lse) g.lse[at] = -INFINITY;
+        const int r0 = pr.y * PT_ROWS + (e & 7) * (PT_ROWS / 8), count = (int)min((int64_t)(PT_ROWS / 8), (int64_t)n * g.group - r0) * g.kv_heads;
+        for (int k = warp; k < count; k += PT_THREADS / 32) {
+            const int r = r0 + k / g.kv_heads, i = r / g.group;
+            const int64_t at = (int64_t)(q0 + i) * g.q_heads + k % g.kv_heads * g.group + r - i * g.group;
+            if (lane < D / 8) reinterpret_cast<uint4 *>(g.out + at * D)[lane] = make_uint4(0, 0, 0, 0);
+            if (lane == 0 && g.lse) g.lse[at] = -INFINITY;
         }
     }
     if (g.cu_q) {
-        const int64_t first = (int64_t)max(__ldg(g.cu_q + g.seqs), 0) * g.q_heads, n = g.rows * g.q_heads;
-        for (int64_t r = first + blockIdx.x; r < n; r += gridDim.x) {
-            for (int d = threadIdx.x; d < D; d += PT_THREADS) g.out[r * D + d] = 0;
-            if (threadIdx.x == 0 && g.lse) g.lse[r] = -INFINITY;
-        }
+        const int64_t first = max(__ldg(g.cu_q + g.seqs), 0);
+        fill_rows<D>(g, first, g.rows - first, blockIdx.x, gridDim.x);
     }
-    if ((int)blockIdx.x >= ctas) return;
+    if ((int)blockIdx.x >= ctas) {
+        if (threadIdx.x == 0) g.seams[2 * blockIdx.x].x = -1;
+        return;
+    }
     const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
 
     if (threadIdx.x == 0) {
@@ -223,9 +261,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
             uint32_t st = 0, ph = 1;
             const int pages = PT_TOK / g.page;
             const uint32_t half = (uint32_t)(g.page * RB);
-            for (int t = lo; t < hi;) {
-                Part s;
-                find_part(g, plan, pairs, t, hi, s);
+            QCC_FOR_PARTS(s, t) {
+                if (t == lo && lane == 0) note_seam(g, s.first ? s.unit_first : -1, s.unit_first + s.tiles, total, (int)((int64_t)s.n * g.group), s.q0, s.head, s.qt * PT_ROWS);
                 const int have = (s.L + g.page - 1) / g.page;
                 const int32_t *row = g.table + s.b * g.table_stride;
                 for (int tile = s.first; tile < s.last; tile++) {
@@ -249,7 +286,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                         if (++st == PT_RAW) { st = 0; ph ^= 1; }
                     }
                 }
-                t += s.last - s.first;
             }
         } else if (warp == 1 && elect_one()) {
             // ---- matrix instructions
@@ -272,9 +308,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 }
                 tc_commit(s_full + x);
             };
-            for (int t = lo; t < hi;) {
-                Part s;
-                find_part(g, plan, pairs, t, hi, s);
+            QCC_FOR_PARTS(s, t) {
                 const int nx = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? 2 : 1;
                 const int count = s.last - s.first;
                 mbar_wait_abort(k_full + (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
@@ -313,7 +347,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                         kt++;
                     }
                 }
-                t += count;
             }
         }
     } else if (warp < 8) {
@@ -326,9 +359,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
         constexpr int PER = 32 / PIECES;         // tokens of a warp at a time
         const int shift = 31 - __clz(g.page);
         uint32_t st = 0, ph = 0, tiles = 0;
-        for (int t = lo; t < hi;) {
-            Part s;
-            find_part(g, plan, pairs, t, hi, s);
+        QCC_FOR_PARTS(s, t) {
             for (int tile = s.first; tile < s.last; tile++, tiles++) {
                 const int left = s.L - tile * PT_TOK;      // tokens of the tile that exist
 #pragma unroll
@@ -364,7 +395,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     if (++st == PT_RAW) { st = 0; ph ^= 1; }
                 }
             }
-            t += s.last - s.first;
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 184;");
@@ -373,9 +403,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
         const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
         uint32_t sn = 0, on = 0;        // scores, products so far
-        for (int t = lo; t < hi;) {
-            Part s;
-            find_part(g, plan, pairs, t, hi, s);
+        QCC_FOR_PARTS(s, t) {
             const int64_t rows = (int64_t)s.n * g.group, r = (int64_t)s.qt * PT_ROWS + x * 128 + row;
             const bool live = r < rows, idle = rows - (int64_t)s.qt * PT_ROWS <= x * 128;      // idle: no row of this tile exists
             const int i = live ? (int)(r / g.group) : 0, h = s.head * g.group + (live ? (int)(r - (int64_t)i * g.group) : 0);
@@ -498,7 +526,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 else if (live && g.lse) g.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
                 tc_fence_before();       // the next unit's products write O
             }
-            t += s.last - s.first;
         }
     }
     __syncwarp();
@@ -510,57 +537,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
     }
 }
 
-// Joins the units that span CTAs.  CTA (i, y) takes 32 rows of the unit in which CTA i begins, if that begins in CTA i - 1.
-template <int D>
-__global__ void __launch_bounds__(256) kv_prompt_join_kernel(const AttnArgs g, const PromptPlan plan, int grid)
-{
-    pdl_wait();
-    const int pairs = plan.count[0], total = plan.prefix[pairs], ctas = min(grid, total), c = blockIdx.x;
-    if (c < 1 || c >= ctas) return;
-    const int lo = (int)((int64_t)total * c / ctas);
-    Part s;
-    find_part(g, plan, pairs, lo, total, s);
-    if (s.unit_first == lo) return;
-    const int i0 = (int)((((int64_t)s.unit_first + 1) * ctas - 1) / total), i1 = (int)((((int64_t)s.unit_first + s.tiles) * ctas - 1) / total);
-    if (i0 != c - 1) return;
-    const int second = (int)((int64_t)total * i0 / ctas) < s.unit_first ? 1 : 0;
-    const int64_t rows = (int64_t)s.n * g.group;
-    constexpr int TPR = D / 4, STEP = 256 / TPR;
-    const int d = threadIdx.x % TPR * 4;
-    for (int k = threadIdx.x / TPR; k < 32; k += STEP) {
-        const int row = blockIdx.y * 32 + k;
-        const int64_t r = (int64_t)s.qt * PT_ROWS + row;
-        if (r >= rows) break;
-        float top = -INFINITY, den = 0.0f;
-        float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int j = i0; j <= i1; j++) {
-            const float *part = g.part + (size_t)(2 * j + (j == i0 ? second : 0)) * prompt_part_floats<D>();
-            const float2 w = reinterpret_cast<const float2 *>(part + PT_ROWS * D)[row];
-            const float4 v = *reinterpret_cast<const float4 *>(part + row * D + d);
-            const float up = fmaxf(top, w.x), a = top == -INFINITY ? 0.0f : ex2(top - up), b = w.x == -INFINITY ? (w.y == 0.0f ? 0.0f : 1.0f) : ex2(w.x - up);
-            const bool first = top == -INFINITY && den == 0.0f;
-            den = (first ? 0.0f : den * a) + w.y * b;
-            sum.x = (first ? 0.0f : sum.x * a) + v.x * b; sum.y = (first ? 0.0f : sum.y * a) + v.y * b;
-            sum.z = (first ? 0.0f : sum.z * a) + v.z * b; sum.w = (first ? 0.0f : sum.w * a) + v.w * b;
-            top = up;
-        }
-        const int i = (int)(r / g.group);
-        const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + s.head * g.group + (r - (int64_t)i * g.group);
-        const float inv = den == 0.0f ? 0.0f : __fdividef(__ldg(g.v_outer), den);
-        const __nv_bfloat162 y0 = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.x * inv, den == 0.0f ? 0.0f : sum.y * inv);
-        const __nv_bfloat162 y1 = __floats2bfloat162_rn(den == 0.0f ? 0.0f : sum.z * inv, den == 0.0f ? 0.0f : sum.w * inv);
-        *reinterpret_cast<uint2 *>(g.out + at * D + d) = make_uint2(*reinterpret_cast<const uint32_t *>(&y0), *reinterpret_cast<const uint32_t *>(&y1));
-        if (d == 0 && g.lse) g.lse[at] = den == 0.0f ? -INFINITY : (top + log2f(den)) * LN2;
-    }
-}
-
 bool prompt_fits(int64_t rows, int group, int seqs, int kv_heads, int64_t cached)
 {
     return prompt_max_pairs(rows, group, seqs) * kv_heads <= 0x7FFFFFFF / ((cached + PT_TOK - 1) / PT_TOK + 1);
 }
 size_t prompt_workspace_bytes(int64_t rows, int group, int seqs, int head_dim)
 {
-    return (prompt_plan_bytes(prompt_max_pairs(rows, group, seqs)) + 15) / 16 * 16 + (size_t)2 * sm_count() * PT_ROWS * (head_dim + 2) * 4;
+    return (prompt_plan_bytes(prompt_max_pairs(rows, group, seqs)) + 15) / 16 * 16 + (size_t)2 * sm_count() * (16 + PT_ROWS * (head_dim + 2) * 4);
 }
 
 template <int D>
@@ -581,14 +564,14 @@ static int launch(AttnArgs g, void *ws, cudaStream_t st)
     }
     const int64_t max_pairs = prompt_max_pairs(g.rows, g.group, g.seqs);
     const PromptPlan plan = prompt_plan(ws, max_pairs);
-    g.part = reinterpret_cast<float *>(static_cast<uint8_t *>(ws) + (prompt_plan_bytes(max_pairs) + 15) / 16 * 16);
-    kv_prompt_plan_kernel<<<1, 1024, 0, st>>>(g, plan);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return (int)e;
     const int grid = sm_count();
+    g.seams = reinterpret_cast<int4 *>(static_cast<uint8_t *>(ws) + (prompt_plan_bytes(max_pairs) + 15) / 16 * 16);
+    g.part = reinterpret_cast<float *>(g.seams + 2 * grid);
+    cudaError_t e = launch_maybe_pdl(kv_prompt_plan_kernel, dim3(1), dim3(1024), 0, st, true, g, plan);
+    if (e != cudaSuccess) return (int)e;
     e = launch_maybe_pdl(kv_prompt_kernel<D>, dim3(grid), dim3(PT_THREADS), C::SMEM, st, true, g, plan);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_maybe_pdl(kv_prompt_join_kernel<D>, dim3(grid, PT_ROWS / 32), dim3(256), 0, st, true, g, plan, grid);
+    return (int)launch_maybe_pdl(kv_join_kernel<D, 1, 32, 256>, dim3(grid, PT_ROWS / 32), dim3(256), 0, st, true, g, grid, PT_ROWS);
 }
 
 int prompt_launch(const AttnArgs &g, int head_dim, void *ws, cudaStream_t st)
