@@ -70,6 +70,11 @@ __device__ __forceinline__ void bulk_load(void *dst, const void *src, uint32_t b
                  : "memory");
 }
 
+__device__ __forceinline__ void bulk_load_at(uint32_t dst, const void *src, uint32_t bytes, uint32_t bar)
+{
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst), "l"(src), "r"(bytes), "r"(bar) : "memory");
+}
+
 // queries and cached tokens of sequence b, checked against what the caller's tensors hold
 __device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n, int &L)
 {

@@ -24,6 +24,7 @@ namespace qcc {
 // many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3;
+constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u;      // notes on a tile: the last of its part; both row tiles have rows
 constexpr unsigned int PT_ERR = 9u;    // a barrier wait of this kernel ran out
 
 template <int D> struct PromptCfg {
@@ -191,6 +192,20 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
                  "r"(r[15])
                  : "memory");
 }
+__device__ __forceinline__ float max3(float a, float b, float c)
+{
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c)
+{
+    uint64_t r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+
 __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // byte of 16-byte chunk `ch` (0 .. D / 8 - 1) of row r in a swizzled tile of 128 rows
@@ -202,13 +217,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
     using C = PromptCfg<D>;
     constexpr int RB = kv_row_bytes<D>();
     extern __shared__ uint8_t raw_smem[];
-    uint8_t *sm = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw_smem) + 1023) & ~(uintptr_t)1023);
-    uint8_t *s_q = sm, *s_k = sm + 2 * C::TILE, *s_v = sm + 4 * C::TILE, *s_raw = sm + 6 * C::TILE;
-    uint64_t *bars = reinterpret_cast<uint64_t *>(s_raw + PT_RAW * C::RAW);
-    uint64_t *raw_full = bars, *raw_empty = bars + 3, *k_full = bars + 6, *k_empty = bars + 8, *v_full = bars + 10, *v_empty = bars + 12, *q_full = bars + 14,
-             *s_full = bars + 16, *p_full = bars + 18, *o_done = bars + 20;
-    uint32_t *slot = reinterpret_cast<uint32_t *>(bars + 22);
-    volatile uint32_t *abort = slot + 1;
+    // shared memory: Q of both row tiles, K and V twice, copied codes, barriers (in pairs but for the codes' three), tile notes
+    const uint32_t sm = (smem_u32(raw_smem) + 1023u) & ~1023u;
+    const uint32_t s_q = sm, s_k = sm + 2 * C::TILE, s_v = sm + 4 * C::TILE, s_raw = sm + 6 * C::TILE, bars = s_raw + PT_RAW * C::RAW;
+    const uint32_t raw_full = bars, raw_empty = bars + 24, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96, q_full = bars + 112,
+                   s_full = bars + 128, p_full = bars + 144, o_done = bars + 160;
+    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212;      // notes of the last 8 tiles: tokens that exist, PT_LAST, PT_TWO
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
@@ -239,33 +253,34 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
     const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < PT_RAW; i++) { mbar_init(raw_full + i, 1); mbar_init(raw_empty + i, 4); }
+        for (int i = 0; i < PT_RAW; i++) { mbar_init_at(raw_full + 8 * i, 1); mbar_init_at(raw_empty + 8 * i, 4); }
         for (int i = 0; i < 2; i++) {
-            mbar_init(k_full + i, 4); mbar_init(k_empty + i, 1);
-            mbar_init(v_full + i, 4); mbar_init(v_empty + i, 1);
-            mbar_init(q_full + i, 128); mbar_init(s_full + i, 1); mbar_init(p_full + i, 128); mbar_init(o_done + i, 1);
+            mbar_init_at(k_full + 8 * i, 4); mbar_init_at(k_empty + 8 * i, 1);
+            mbar_init_at(v_full + 8 * i, 4); mbar_init_at(v_empty + 8 * i, 1);
+            mbar_init_at(q_full + 8 * i, 4); mbar_init_at(s_full + 8 * i, 1); mbar_init_at(p_full + 8 * i, 4); mbar_init_at(o_done + 8 * i, 1);
         }
-        *abort = 0;
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort), "r"(0u) : "memory");
         fence_barrier_init();
     }
-    if (warp == 2) tmem_alloc(slot, 512);
+    if (warp == 2) tmem_alloc_at(slot, 512);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;      // S0, S1 at columns 0 and 128 (P over their first halves), O0, O1 at 256 and 384
+    const uint32_t tmem = lds_u32(slot);      // S0, S1 at columns 0 and 128 (P over their first halves), O0, O1 at 256 and 384
 
     if (warp < 4) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0) {
             // ---- copies: a tile's keys, then its values
-            uint32_t st = 0, ph = 1;
+            uint32_t st = 0, ph = 1, tiles = 0;
             const int pages = PT_TOK / g.page;
             const uint32_t half = (uint32_t)(g.page * RB);
             QCC_FOR_PARTS(s, t) {
                 if (t == lo && lane == 0) note_seam(g, s.first ? s.unit_first : -1, s.unit_first + s.tiles, total, (int)((int64_t)s.n * g.group), s.q0, s.head, s.qt * PT_ROWS);
                 const int have = (s.L + g.page - 1) / g.page;
                 const int32_t *row = g.table + s.b * g.table_stride;
-                for (int tile = s.first; tile < s.last; tile++) {
+                const uint32_t two = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? PT_TWO : 0;
+                for (int tile = s.first; tile < s.last; tile++, tiles++) {
                     const int p = tile * pages + lane;
                     int64_t pg = -1;
                     if (lane < pages && p < have) {
@@ -279,10 +294,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     const uint8_t *src = g.cache + (pg * g.kv_heads + s.head) * (int64_t)(2 * half);
 #pragma unroll
                     for (int w = 0; w < 2; w++) {
-                        mbar_wait_abort(raw_empty + st, ph, PT_ERR, abort);
-                        if (lane == 0) mbar_expect_tx(raw_full + st, n * half);
+                        mbar_wait_at(raw_empty + 8 * (st), ph, PT_ERR, abort);
+                        if (lane == 0) {
+                            if (w == 0)
+                                sts_u32(s_info + 4 * (tiles & 7), (uint32_t)min(max(s.L - tile * PT_TOK, 0), PT_TOK) | (tile + 1 == s.last ? PT_LAST : 0) | two);
+                            mbar_expect_at(raw_full + 8 * st, n * half);
+                        }
                         __syncwarp();
-                        if (pg >= 0) bulk_load(s_raw + st * C::RAW + lane * half, src + w * half, half, raw_full + st);
+                        if (pg >= 0) bulk_load_at(s_raw + st * C::RAW + lane * half, src + w * half, half, raw_full + 8 * st);
                         if (++st == PT_RAW) { st = 0; ph ^= 1; }
                     }
                 }
@@ -291,92 +310,101 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
             // ---- matrix instructions
             constexpr uint32_t id_s = (1u << 4) | ((uint32_t)(PT_TOK >> 3) << 17) | (8u << 24);
             constexpr uint32_t id_o = (1u << 4) | (1u << 16) | ((uint32_t)(D >> 3) << 17) | (8u << 24);
-            const uint64_t dq = desc_kmajor_sw128(smem_u32(s_q)), dk = desc_kmajor_sw128(smem_u32(s_k));
-            // V: rows are tokens, the contracted side; 64-element blocks of a row 16384 bytes apart
-            const uint64_t dv = (uint64_t)((smem_u32(s_v) >> 4) & 0x3FFFu) | (1024ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
+            // descriptors: the high words are the same (8 rows are 1024 bytes, 128-byte swizzle); the low words hold the address and, for V, whose
+            // rows are tokens, the contracted side, the 16384 bytes between 64-element blocks of a row
+            constexpr uint32_t high = 64u | (1u << 14) | (2u << 29);
+            const uint32_t dq = (s_q >> 4) | (1u << 16), dk = (s_k >> 4) | (1u << 16), dv = (s_v >> 4) | (1024u << 16);
             uint32_t kt = 0, vt = 0, qn[2] = {0, 0}, pn[2] = {0, 0};      // tiles of K and V; of each row tile: units, probabilities so far
             const auto scores = [&](int x, uint32_t kb) {
-                const uint64_t a = dq + (uint64_t)(x * (C::TILE >> 4)), b = dk + (uint64_t)(kb * (C::TILE >> 4));
+                const uint32_t a = dq + x * (C::TILE >> 4), b = dk + kb * (C::TILE >> 4);
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const uint32_t step = (uint32_t)((k >> 2) * 1024 + (k & 3) * 2);
                     asm volatile(
-                        "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                        "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem + x * 128),
-                        "l"(a + step), "l"(b + step), "r"(id_s), "r"(k > 0 ? 1u : 0u)
+                        "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+                        "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n}\n" ::"r"(tmem + x * 128),
+                        "r"(a + step), "r"(b + step), "r"(id_s), "r"(k > 0 ? 1u : 0u), "r"(high)
                         : "memory");
                 }
-                tc_commit(s_full + x);
+                tc_commit_at(s_full + 8 * (x));
             };
-            QCC_FOR_PARTS(s, t) {
-                const int nx = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? 2 : 1;
-                const int count = s.last - s.first;
-                mbar_wait_abort(k_full + (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
+            const uint32_t count = hi - lo;
+            while (kt < count) {
+                // a part's first scores
+                mbar_wait_at(k_full + 8 * (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
+                uint32_t info = lds_volatile(s_info + 4 * (kt & 7));
+                const int nx = info & PT_TWO ? 2 : 1;
                 for (int x = 0; x < nx; x++) {
-                    mbar_wait_abort(q_full + x, qn[x]++ & 1, PT_ERR, abort);
+                    mbar_wait_at(q_full + 8 * (x), qn[x]++ & 1, PT_ERR, abort);
                     tc_fence_after();
                     scores(x, kt & 1);
                 }
-                tc_commit(k_empty + (kt & 1));
+                tc_commit_at(k_empty + 8 * (kt & 1));
                 kt++;
-                for (int j = 0; j < count; j++, vt++) {
-                    mbar_wait_abort(v_full + (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
+                for (uint32_t o = 0;; o = 1) {      // o: whether O holds anything
+                    const bool more = !(info & PT_LAST);
+                    mbar_wait_at(v_full + 8 * (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
+                    if (more) mbar_wait_at(k_full + 8 * (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
                     for (int x = 0; x < nx; x++) {
-                        mbar_wait_abort(p_full + x, pn[x]++ & 1, PT_ERR, abort);
+                        mbar_wait_at(p_full + 8 * (x), pn[x]++ & 1, PT_ERR, abort);
                         tc_fence_after();
-                        const uint64_t b = dv + (uint64_t)((vt & 1) * (C::TILE >> 4));
+                        const uint32_t b = dv + (vt & 1) * (C::TILE >> 4);
 #pragma unroll
                         for (int k = 0; k < PT_TOK / 16; k++)
                             asm volatile(
-                                "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(tmem + 256 + x * 128),
-                                "r"(tmem + x * 128 + k * 8), "l"(b + (uint64_t)(k * 128)), "r"(id_o), "r"((j > 0 || k > 0) ? 1u : 0u)
+                                "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\n"
+                                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(tmem + 256 + x * 128),
+                                "r"(tmem + x * 128 + k * 8), "r"(b + k * 128), "r"(id_o), "r"(k > 0 ? 1u : o), "r"(high)
                                 : "memory");
-                        tc_commit(o_done + x);
-                        if (j + 1 < count) {
-                            if (x == 0) {
-                                mbar_wait_abort(k_full + (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
-                                tc_fence_after();
-                            }
-                            scores(x, kt & 1);      // over P: instructions run in order, the product above has read it
-                        }
+                        tc_commit_at(o_done + 8 * (x));
+                        if (more) scores(x, kt & 1);      // over P: instructions run in order, the product above has read it
                     }
-                    tc_commit(v_empty + (vt & 1));
-                    if (j + 1 < count) {
-                        tc_commit(k_empty + (kt & 1));
-                        kt++;
-                    }
+                    tc_commit_at(v_empty + 8 * (vt & 1));
+                    vt++;
+                    if (!more || lds_volatile(abort)) break;
+                    info = lds_volatile(s_info + 4 * (kt & 7));
+                    tc_commit_at(k_empty + 8 * (kt & 1));
+                    kt++;
                 }
+                if (lds_volatile(abort)) break;
             }
         }
     } else if (warp < 8) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
-        // ---- widening.  A warp takes 8 tokens at a time: 4 threads a token (2 for D = 64), 32 elements each.  The order of the lanes
-        // keeps the stores free of bank conflicts and the loads at two to a bank.
+        // ---- widening, a tile's keys, then its values.  A warp takes 8 tokens at a time: 4 threads a token (2 for D = 64), 32 elements
+        // each.  The order of the lanes keeps the stores free of bank conflicts and the loads at two to a bank.
         constexpr int PIECES = D / 32;
-        const int w = warp - 4;
+        const int w = warp & 3;
         const int r_in = D == 128 ? (lane & 3) + ((lane >> 4) << 2) : (lane & 3) + ((lane >> 3) << 2), ch = D == 128 ? ((lane >> 2) & 1) | (((lane >> 3) & 1) << 1) : (lane >> 2) & 1;
         constexpr int PER = 32 / PIECES;         // tokens of a warp at a time
         const int shift = 31 - __clz(g.page);
         uint32_t st = 0, ph = 0, tiles = 0;
-        QCC_FOR_PARTS(s, t) {
-            for (int tile = s.first; tile < s.last; tile++, tiles++) {
-                const int left = s.L - tile * PT_TOK;      // tokens of the tile that exist
+        for (const uint32_t count = hi - lo; tiles < count; tiles++) {
+            const uint32_t buf = tiles & 1;
 #pragma unroll
-                for (int v = 0; v < 2; v++) {
-                    const uint32_t buf = tiles & 1;
-                    mbar_wait_abort((v ? v_empty : k_empty) + buf, ((tiles >> 1) & 1) ^ 1, PT_ERR, abort);
-                    mbar_wait_abort(raw_full + st, ph, PT_ERR, abort);
-                    const uint32_t src = smem_u32(s_raw + st * C::RAW), dst = smem_u32((v ? s_v : s_k) + buf * C::TILE);
+            for (int v = 0; v < 2; v++) {
+                {
+                    const uint32_t out_full = v ? v_full : k_full, out_empty = v ? v_empty : k_empty, out = v ? s_v : s_k;
+                    mbar_wait_at(out_empty + 8 * (buf), ((tiles >> 1) & 1) ^ 1, PT_ERR, abort);
+                    mbar_wait_at(raw_full + 8 * (st), ph, PT_ERR, abort);
+                    const int left = lds_volatile(s_info + 4 * (tiles & 7)) & 255;      // tokens of the tile that exist
+                    const uint32_t src = s_raw + st * C::RAW, dst = out + buf * C::TILE;
+                    constexpr int STEPS = 128 / (4 * PER);
+                    uint4 c[STEPS];
+                    uint32_t two[STEPS];
 #pragma unroll
-                    for (int i = 0; i < 128 / (4 * PER); i++) {
+                    for (int i = 0; i < STEPS; i++) {       // all loads first: a step's stores would hold the next one's loads back
                         const int r = (i * 4 + w) * PER + r_in, off = r & (g.page - 1);
                         const uint32_t base = src + (uint32_t)((r >> shift) << shift) * RB;
-                        const uint4 c = lds_v4(base + off * (D / 2) + ch * 16);
-                        uint32_t two = lds_u16(base + (D / 2 << shift) + off * (D / 16) + ch * 2);
-                        if (r >= left) two = 0;            // whatever the slots behind the last token hold, it counts as zero
-                        const uint32_t sc = e4m3x2_to_half2(two), s0 = __byte_perm(sc, sc, 0x1010), s1 = __byte_perm(sc, sc, 0x3232);
-                        const uint32_t word[4] = {c.x, c.y, c.z, c.w};
+                        c[i] = lds_v4(base + off * (D / 2) + ch * 16);
+                        two[i] = lds_u16(base + (D / 2 << shift) + off * (D / 16) + ch * 2);
+                        if (r >= left) two[i] = 0;          // whatever the slots behind the last token hold, it counts as zero
+                    }
+#pragma unroll
+                    for (int i = 0; i < STEPS; i++) {
+                        const int r = (i * 4 + w) * PER + r_in;
+                        const uint32_t sc = e4m3x2_to_half2(two[i]), s0 = __byte_perm(sc, sc, 0x1010), s1 = __byte_perm(sc, sc, 0x3232);
+                        const uint32_t word[4] = {c[i].x, c[i].y, c[i].z, c[i].w};
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             uint32_t h[4];
@@ -389,8 +417,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     proxy_fence();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(raw_empty + st);
-                        mbar_arrive((v ? v_full : k_full) + buf);
+                        mbar_arrive_at(raw_empty + 8 * st);
+                        mbar_arrive_at(out_full + 8 * buf);
                     }
                     if (++st == PT_RAW) { st = 0; ph ^= 1; }
                 }
@@ -422,17 +450,18 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 q_power(f2u(hmax_halves_f32(acc)), mult, back);
                 factor = back * (g.scale_log2 * k_outer);
                 factor = factor < 1e-37f ? 1e-37f : factor;       // not zero: -inf of a hidden key has to stay
-                const uint32_t dst = smem_u32(s_q + x * C::TILE);
+                const uint32_t dst = s_q + x * C::TILE;
 #pragma unroll
                 for (int j = 0; j < D / 8; j++)
                     sts_v4(dst + tile_at(row, j),
                            make_uint4(pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult), pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult),
                                       pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult), pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult)));
                 proxy_fence();
-                mbar_arrive(q_full + x);
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(q_full + 8 * x);
                 float m = -INFINITY, l = 0.0f;
                 for (int tile = s.first; tile < s.last; tile++) {
-                    mbar_wait_abort(s_full + x, sn++ & 1, PT_ERR, abort);
+                    mbar_wait_at(s_full + 8 * (x), sn++ & 1, PT_ERR, abort);
                     tc_fence_after();
                     uint32_t v[4][32];
 #pragma unroll
@@ -448,19 +477,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     }
                     float top[4];
 #pragma unroll
-                    for (int c = 0; c < 4; c++) {
-                        top[c] = u2f(v[c][0]);
+                    for (int c = 0; c < 4; c++) top[c] = fmaxf(u2f(v[c][0]), u2f(v[c][1]));
 #pragma unroll
-                        for (int j = 1; j < 32; j++) top[c] = fmaxf(top[c], u2f(v[c][j]));
-                    }
-                    const float most = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * factor;
+                    for (int j = 2; j < 32; j += 2)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) top[c] = max3(top[c], u2f(v[c][j]), u2f(v[c][j + 1]));
+                    const float most = fmaxf(max3(top[0], top[1], top[2]), top[3]) * factor;
                     const bool grow = most - m > 8.0f;           // (from -inf: always, once the row sees a key)
                     if (__any_sync(0xFFFFFFFFu, grow)) {
                         const float up = grow ? most : m, a = grow ? ex2(m - up) : 1.0f;
                         m = up;
                         l *= a;
                         if (tile > s.first) {
-                            mbar_wait_abort(o_done + x, (on - 1) & 1, PT_ERR, abort);
+                            mbar_wait_at(o_done + 8 * x, (on - 1) & 1, PT_ERR, abort);
                             tc_fence_after();
 #pragma unroll
                             for (int c = 0; c < D; c += 16) {
@@ -474,26 +503,35 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    const uint64_t factor2 = pack2(factor, factor), base2 = pack2(-base, -base);
+                    uint64_t sum[2] = {0, 0};
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         uint32_t p[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
                             // (factor is finite and positive: -inf stays -inf and exp2 gives 0)
-                            const float e0 = ex2(fmaf(u2f(v[c][2 * j]), factor, -base)), e1 = ex2(fmaf(u2f(v[c][2 * j + 1]), factor, -base));
-                            sum[j & 3] += e0 + e1;
+                            float e0, e1;
+                            unpack2(fma2(pack2(u2f(v[c][2 * j]), u2f(v[c][2 * j + 1])), factor2, base2), e0, e1);
+                            e0 = ex2(e0);
+                            e1 = ex2(e1);
+                            sum[j & 1] = add2(sum[j & 1], pack2(e0, e1));
                             p[j] = pack_half2(e0, e1);
                         }
                         tmem_st16(t_s + 16 * c, p);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    {
+                        float a, b;
+                        unpack2(add2(sum[0], sum[1]), a, b);
+                        l += a + b;
+                    }
                     tmem_wait_st();
                     tc_fence_before();
-                    mbar_arrive(p_full + x);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_at(p_full + 8 * x);
                     on++;
                 }
-                mbar_wait_abort(o_done + x, (on - 1) & 1, PT_ERR, abort);
+                mbar_wait_at(o_done + 8 * (x), (on - 1) & 1, PT_ERR, abort);
                 tc_fence_after();
                 const bool whole = s.first == 0 && s.last == s.tiles;
                 const float scale = l == 0.0f ? 0.0f : __fdividef(v_outer, l);

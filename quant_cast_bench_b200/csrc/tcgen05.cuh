@@ -39,13 +39,46 @@ __device__ __forceinline__ void mbar_wait_abort(uint64_t *bar, uint32_t parity, 
     atomicMax(&g_qcc_error, code);
 }
 
-// --------------------------------------------------------------------------------------------- tensor memory
-// The address of `cols` columns (a power of two >= 32) lands in *slot (shared memory).  One whole warp calls it.
-__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols)
+// The same by shared-memory address (32 bits: a kernel with many barriers then keeps one base register, the rest are immediates)
+__device__ __forceinline__ void mbar_init_at(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
+__device__ __forceinline__ void mbar_expect_at(uint32_t bar, uint32_t bytes)
 {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(slot)), "r"(cols) : "memory");
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void mbar_arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
+__device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
+__device__ __forceinline__ uint32_t lds_volatile(uint32_t addr)
+{
+    uint32_t v;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsigned int code, uint32_t abort)
+{
+    for (uint32_t it = 0; it < (1u << 22); it++) {
+        uint32_t done;
+        asm volatile(
+            "{\n.reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return;
+        if ((it & 63u) == 63u && lds_volatile(abort)) return;
+    }
+    asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort), "r"(1u) : "memory");
+    atomicMax(&g_qcc_error, code);
+}
+
+// --------------------------------------------------------------------------------------------- tensor memory
+// The address of `cols` columns (a power of two >= 32) lands in `slot` (shared memory).  One whole warp calls it.
+__device__ __forceinline__ void tmem_alloc_at(uint32_t slot, uint32_t cols)
+{
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
 }
+__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) { tmem_alloc_at(smem_u32(slot), cols); }
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols)
 {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
@@ -58,6 +91,10 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 __device__ __forceinline__ void tc_commit(uint64_t *bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ void tc_commit_at(uint32_t bar)
+{
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 // 32 lanes (of this warp's quadrant) x 32 columns of 32 bits: thread = lane, r[i] = column i
 __device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&r)[32])
