@@ -48,6 +48,8 @@ template <int CH>
 __global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t *__restrict__ x, int64_t N, uint8_t *__restrict__ q,
                                                                   float *__restrict__ scale, int recip_div)
 {
+    pdl_trigger();
+    pdl_wait();
     const int64_t row = blockIdx.x;
     const uint16_t *xr = x + row * N;
     uint8_t *qr = q + row * N;
@@ -91,32 +93,40 @@ __global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t
 // ---------------------------------------------------------------------------------------------
 // product
 // ---------------------------------------------------------------------------------------------
-// tcgen05.mma kind::i8 on tiles of 128 output channels (the M side of the instruction: one accumulator row per thread of the
-// epilogue, so a warp stores 32 neighbouring channels of a token) by BN tokens, K in blocks of 128 bytes staged by TMA.  The
-// tokens are on the N side because it goes down to 16: a decode batch wastes little of the instruction.
-constexpr int MM_BM = 128, MM_BK = 128, MM_THREADS = 256;
+// tcgen05.mma kind::i8 on tiles of 128 output channels (the M side of the instruction) by BN tokens, K in blocks of 128 bytes
+// staged by TMA.  The tokens are on the N side because it goes down to 16: a decode batch wastes little of the instruction.
+// Where there are fewer tiles than SMs, the CTAs of a cluster share out K and add their sums up through each other's shared
+// memory; whole numbers, so in any order the same.
+constexpr int MM_BM = 128, MM_BK = 128, MM_THREADS = 384;
 constexpr unsigned int MM_ERR = 7;   // a barrier wait of the product ran out
 
 template <int BN> struct MmCfg {
     static constexpr int STAGE = (MM_BM + BN) * MM_BK;
     static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
-    static constexpr int RED = BN <= 128 ? MM_BM * BN * 4 : 0;             // partial sums of one CTA (split form), in the stages' memory
-    static constexpr int SMEM = (STAGE * STAGES > RED ? STAGE * STAGES : RED) + 1024 + BN * 4 * 2 + 256;
+    static constexpr int RED = MM_BM * BN * 4;                              // sums of one CTA (split form), in the stages' memory
+    static constexpr int BODY = STAGE * STAGES > RED ? STAGE * STAGES : RED;
+    static constexpr int PARTS = BN >= 64 ? 2 : 1;                          // epilogue warps per 32 channels, each with a share of the tokens
+    static constexpr int TURN = 4 * PARTS * 16 * 32 * 4;                    // 16 tokens x 32 channels of each epilogue warp
+    static constexpr int SMEM = 1024 + BODY + TURN + BN * 4 * 2 + 256;
 };
 
 struct MmArgs {
     const float *sa, *sb;
     const uint16_t *bias;
     void *out;
-    int M, N, kblocks, tiles_n, tiles_m, splits, out_kind;
+    int M, N, kblocks, tiles_n, tiles_m, splits, piece;      // piece: log2 of the bytes that every row of the output is aligned to, up to 16
 };
 
-__device__ __forceinline__ void mm_store(const MmArgs &g, int64_t m, int n, float y)
+template <int OUT> struct OutType;
+template <> struct OutType<QCC_OUT_BF16> { using T = uint16_t; static __device__ __forceinline__ T of(float y) { return __bfloat16_as_ushort(__float2bfloat16_rn(y)); } };
+template <> struct OutType<QCC_OUT_F16> { using T = uint16_t; static __device__ __forceinline__ T of(float y) { return __half_as_ushort(__float2half_rn(y)); } };
+template <> struct OutType<QCC_OUT_F32> { using T = float; static __device__ __forceinline__ T of(float y) { return y; } };
+
+// the scales in fp32, a multiplication each, then the bias
+__device__ __forceinline__ float mm_scaled(int32_t sum, float sa, float sb, bool has_bias, float bias)
 {
-    const size_t at = (size_t)m * g.N + n;
-    if (g.out_kind == 0) reinterpret_cast<__nv_bfloat16 *>(g.out)[at] = __float2bfloat16_rn(y);
-    else if (g.out_kind == 1) reinterpret_cast<__half *>(g.out)[at] = __float2half_rn(y);
-    else reinterpret_cast<float *>(g.out)[at] = y;
+    const float y = __fmul_rn(__fmul_rn((float)sum, sa), sb);
+    return has_bias ? __fadd_rn(y, bias) : y;
 }
 
 // groups of 8 token tiles share the weights that pass through L2
@@ -127,33 +137,59 @@ __device__ __forceinline__ void mm_tile(const MmArgs &g, int t, int &tn, int &tm
     tn = r / rows;
 }
 
-template <int BN, bool SPLIT>
+// 16 tokens x 32 channels from shared memory to the output, in pieces of 2^LOG bytes: neighbouring lanes have neighbouring pieces of a row
+template <int LOG, typename T>
+__device__ __forceinline__ void mm_write(const MmArgs &g, uint32_t turn, int64_t m0, int n0, int lane)
+{
+    constexpr int ROW = 32 * sizeof(T), PIECES = ROW >> LOG, EACH = 16 * PIECES / 32;
+#pragma unroll
+    for (int i = 0; i < EACH; i++) {
+        const int e = i * 32 + lane, tok = e / PIECES, at = (e % PIECES) << LOG, n = n0 + at / (int)sizeof(T);
+        if (m0 + tok >= g.M || n >= g.N) continue;
+        uint8_t *dst = static_cast<uint8_t *>(g.out) + ((m0 + tok) * g.N + n) * (int64_t)sizeof(T);
+        const uint32_t src = turn + tok * ROW + at;
+        if (LOG == 4) *reinterpret_cast<uint4 *>(dst) = lds_v4(src);
+        else if (LOG == 3) *reinterpret_cast<uint2 *>(dst) = lds_v2(src);
+        else if (LOG == 2) {
+            uint32_t v;
+            asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(src));
+            *reinterpret_cast<uint32_t *>(dst) = v;
+        } else {
+            uint16_t v;
+            asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(src));
+            *reinterpret_cast<uint16_t *>(dst) = v;
+        }
+    }
+}
+
+template <int BN, bool SPLIT, int OUT>
 __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x,
                                                                 const MmArgs g)
 {
     using C = MmCfg<BN>;
+    using T = typename OutType<OUT>::T;
     extern __shared__ uint8_t raw[];
-    uint8_t *stages = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    constexpr int BODY = C::STAGE * C::STAGES > C::RED ? C::STAGE * C::STAGES : C::RED;
-    float *s_sa = reinterpret_cast<float *>(stages + BODY);                 // 2 x BN token scales
-    uint64_t *full = reinterpret_cast<uint64_t *>(s_sa + 2 * BN), *empty = full + C::STAGES, *acc_full = empty + C::STAGES,
-             *acc_empty = acc_full + 2;
-    uint32_t *slot = reinterpret_cast<uint32_t *>(acc_empty + 2);
-    volatile uint32_t *abort = slot + 1;
+    const uint32_t stages = (smem_u32(raw) + 1023u) & ~1023u, turns = stages + C::BODY, s_sa = turns + C::TURN;       // s_sa: 2 x BN token scales
+    const uint32_t full = s_sa + 2 * BN * 4, empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16,
+                   abort = slot + 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     constexpr uint32_t ACC_COLS = BN < 32 ? 32 : BN, TMEM_COLS = SPLIT ? ACC_COLS : 2 * ACC_COLS;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < C::STAGES; i++) { mbar_init(full + i, 1); mbar_init(empty + i, 1); }
-        for (int i = 0; i < 2; i++) { mbar_init(acc_full + i, 1); mbar_init(acc_empty + i, 4); }
-        *abort = 0;
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&map_x) : "memory");
+        for (int i = 0; i < C::STAGES; i++) { mbar_init_at(full + 8 * i, 1); mbar_init_at(empty + 8 * i, 1); }
+        for (int i = 0; i < 2; i++) { mbar_init_at(acc_full + 8 * i, 1); mbar_init_at(acc_empty + 8 * i, 4 * C::PARTS); }
+        sts_u32(abort, 0);
         fence_barrier_init();
     }
-    if (warp == 2) tmem_alloc(slot, TMEM_COLS);
+    if (warp == 2) tmem_alloc_at(slot, TMEM_COLS);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *slot;
+    pdl_trigger();
+    pdl_wait();
+    const uint32_t tmem = lds_volatile(slot);
     const int total = g.tiles_n * g.tiles_m;
     // SPLIT: the CTAs of a cluster take one tile together, each a share of the K blocks
     const int rank = SPLIT ? blockIdx.x % g.splits : 0;
@@ -162,121 +198,139 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
 
     if (warp == 0) {
         if (elect_one()) {
-            uint32_t it = 0;
+            uint32_t s = 0, ph = 1;
             for (int t = t0; t < total; t += step) {
                 int tn, tm;
                 mm_tile(g, t, tn, tm);
-                for (int kb = kb0; kb < kb1; kb++, it++) {
-                    const uint32_t s = it % C::STAGES, ph = (it / C::STAGES) & 1;
-                    mbar_wait_abort(empty + s, ph ^ 1, MM_ERR, abort);
-                    uint8_t *p = stages + s * C::STAGE;
-                    mbar_expect_tx(full + s, C::STAGE);
-                    tma_load_2d(p, &map_w, full + s, kb * MM_BK, tn * MM_BM);
-                    tma_load_2d(p + MM_BM * MM_BK, &map_x, full + s, kb * MM_BK, tm * BN);
+                for (int kb = kb0; kb < kb1; kb++) {
+                    mbar_wait_at(empty + 8 * s, ph, MM_ERR, abort);
+                    const uint32_t p = stages + s * C::STAGE, bar = full + 8 * s;
+                    mbar_expect_at(bar, C::STAGE);
+                    tma_load_2d_at(p, &map_w, bar, kb * MM_BK, tn * MM_BM);
+                    tma_load_2d_at(p + MM_BM * MM_BK, &map_x, bar, kb * MM_BK, tm * BN);
+                    if (++s == C::STAGES) { s = 0; ph ^= 1; }
                 }
             }
         }
     } else if (warp == 1) {
         if (elect_one()) {
             constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(MM_BM >> 4) << 24);
-            uint32_t it = 0, n = 0;
+            constexpr uint32_t high = 64u | (1u << 14) | (2u << 29);      // high words of the descriptors: 8 rows are 1024 bytes, 128-byte swizzle
+            uint32_t s = 0, ph = 0, n = 0;
             for (int t = t0; t < total; t += step, n++) {
                 const uint32_t acc = SPLIT ? 0 : n & 1, aph = SPLIT ? 0 : (n >> 1) & 1;
-                mbar_wait_abort(acc_empty + acc, aph ^ 1, MM_ERR, abort);
+                mbar_wait_at(acc_empty + 8 * acc, aph ^ 1, MM_ERR, abort);
                 tc_fence_after();
-                for (int kb = kb0; kb < kb1; kb++, it++) {
-                    const uint32_t s = it % C::STAGES, ph = (it / C::STAGES) & 1;
-                    mbar_wait_abort(full + s, ph, MM_ERR, abort);
+                for (int kb = kb0; kb < kb1; kb++) {
+                    mbar_wait_at(full + 8 * s, ph, MM_ERR, abort);
                     tc_fence_after();
-                    const uint32_t a = smem_u32(stages + s * C::STAGE);
-                    const uint64_t da = desc_kmajor_sw128(a), db = desc_kmajor_sw128(a + MM_BM * MM_BK);
+                    const uint32_t da = ((stages + s * C::STAGE) >> 4) | (1u << 16), db = da + (MM_BM * MM_BK >> 4);
 #pragma unroll
                     for (int k = 0; k < MM_BK / 32; k++)
                         asm volatile(
-                            "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-                            "tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, p;\n}\n" ::"r"(tmem + acc * ACC_COLS),
-                            "l"(da + 2 * k), "l"(db + 2 * k), "r"(idesc), "r"((kb > kb0 || k > 0) ? 1u : 0u)
+                            "{\n.reg .pred p;\n.reg .b64 a, b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 a, {%1, %5};\nmov.b64 b, {%2, %5};\n"
+                            "tcgen05.mma.cta_group::1.kind::i8 [%0], a, b, %3, p;\n}\n" ::"r"(tmem + acc * ACC_COLS),
+                            "r"(da + 2 * k), "r"(db + 2 * k), "r"(idesc), "r"((kb > kb0 || k > 0) ? 1u : 0u), "r"(high)
                             : "memory");
-                    tc_commit(empty + s);
+                    tc_commit_at(empty + 8 * s);
+                    if (++s == C::STAGES) { s = 0; ph ^= 1; }
                 }
-                tc_commit(acc_full + acc);
+                tc_commit_at(acc_full + 8 * acc);
             }
         }
-    } else if (warp >= 4) {
-        const int w = warp - 4, et = threadIdx.x - 128;
+    } else if (warp >= 4 && warp < 4 + 4 * C::PARTS) {
+        constexpr int EPI = 128 * C::PARTS, SHARE = BN / C::PARTS;
+        const int w = warp & 3, part = (warp - 4) >> 2, et = threadIdx.x - 128;
+        const uint32_t turn = turns + (warp - 4) * (16 * 32 * 4);
         uint32_t n = 0;
         for (int t = t0; t < total; t += step, n++) {
             int tn, tm;
             mm_tile(g, t, tn, tm);
             const uint32_t acc = SPLIT ? 0 : n & 1, aph = SPLIT ? 0 : (n >> 1) & 1;
-            const int ch = tn * MM_BM + w * 32 + lane;
-            float *sa = s_sa + acc * BN;
-            for (int i = et; i < BN; i += 128) sa[i] = tm * BN + i < g.M ? g.sa[(int64_t)tm * BN + i] : 0.0f;
-            named_barrier(1, 128);
-            const float sb = ch < g.N ? g.sb[ch] : 0.0f;
-            const float bias = g.bias != nullptr && ch < g.N ? u2f((uint32_t)g.bias[ch] << 16) : 0.0f;
-            mbar_wait_abort(acc_full + acc, aph, MM_ERR, abort);
+            const int n0 = tn * MM_BM + w * 32, ch = n0 + lane;
+            const uint32_t sa = s_sa + acc * BN * 4;
+            for (int i = et; i < BN; i += EPI) sts_u32(sa + 4 * i, tm * BN + i < g.M ? f2u(g.sa[(int64_t)tm * BN + i]) : 0);
+            named_barrier(1, EPI);
+            const bool has_bias = g.bias != nullptr;
+            const float sb = ch < g.N ? g.sb[ch] : 0.0f, bias = has_bias && ch < g.N ? u2f((uint32_t)g.bias[ch] << 16) : 0.0f;
+            mbar_wait_at(acc_full + 8 * acc, aph, MM_ERR, abort);
             tc_fence_after();
-            if (SPLIT) {
-                int32_t *red = reinterpret_cast<int32_t *>(stages);
 #pragma unroll 1
-                for (int c = 0; c < BN; c += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(tmem + ((uint32_t)w << 21) + c, r);
-                    tmem_wait_ld();
+            for (int c = part * SHARE; c < (part + 1) * SHARE; c += 16) {
+                uint32_t r[16];
+                tmem_ld16(tmem + ((uint32_t)w << 21) + acc * ACC_COLS + c, r);
+                tmem_wait_ld();
+                if (SPLIT) {
 #pragma unroll
-                    for (int j = 0; j < 16; j++) red[(c + j) * MM_BM + w * 32 + lane] = (int32_t)r[j];
+                    for (int j = 0; j < 16; j++) sts_u32(stages + (uint32_t)((c + j) * MM_BM + w * 32 + lane) * 4, r[j]);
+                    continue;
                 }
-            } else {
-#pragma unroll 1
-                for (int c = 0; c < BN; c += 16) {
-                    uint32_t r[16];
-                    tmem_ld16(tmem + ((uint32_t)w << 21) + acc * ACC_COLS + c, r);
-                    tmem_wait_ld();
-                    if (c + 16 >= BN) {                 // the accumulator is in registers: the next tile may have it
-                        tc_fence_before();
-                        if (lane == 0) mbar_arrive(acc_empty + acc);
-                    }
-                    if (ch < g.N) {
+                if (c + 16 == (part + 1) * SHARE) {                 // the accumulator is in registers: the next tile may have it
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive_at(acc_empty + 8 * acc);
+                }
+                const int64_t m0 = (int64_t)tm * BN + c;
+                if (m0 >= g.M) continue;
 #pragma unroll
-                        for (int j = 0; j < 16; j++) {
-                            const int64_t m = (int64_t)tm * BN + c + j;
-                            if (m < g.M) {
-                                float y = __fmul_rn(__fmul_rn((float)(int32_t)r[j], sa[c + j]), sb);
-                                if (g.bias != nullptr) y = __fadd_rn(y, bias);
-                                mm_store(g, m, ch, y);
-                            }
-                        }
+                for (int j = 0; j < 16; j += 4) {
+                    const uint4 q = lds_v4(sa + 4 * (c + j));
+                    const float s4[4] = {u2f(q.x), u2f(q.y), u2f(q.z), u2f(q.w)};
+#pragma unroll
+                    for (int u = 0; u < 4; u++) {
+                        const T y = OutType<OUT>::of(mm_scaled((int32_t)r[j + u], s4[u], sb, has_bias, bias));
+                        const uint32_t at = turn + ((j + u) * 32 + lane) * (uint32_t)sizeof(T);
+                        if (sizeof(T) == 4) sts_u32(at, *reinterpret_cast<const uint32_t *>(&y));
+                        else asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(*reinterpret_cast<const uint16_t *>(&y)) : "memory");
                     }
                 }
+                __syncwarp();
+                if (g.piece == 4) mm_write<4, T>(g, turn, m0, n0, lane);
+                else if (g.piece == 3) mm_write<3, T>(g, turn, m0, n0, lane);
+                else if (g.piece == 2 || sizeof(T) == 4) mm_write<2, T>(g, turn, m0, n0, lane);
+                else mm_write<sizeof(T) == 4 ? 2 : 1, T>(g, turn, m0, n0, lane);
+                __syncwarp();
             }
         }
     }
     __syncwarp();
     if (SPLIT) {
-        // every CTA of the cluster adds up its share of the tokens from all shares of K; whole numbers, so in any order the same
+        // every CTA of the cluster adds up its share of the tokens from all shares of K, four channels a thread
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
         int tn, tm;
         mm_tile(g, t0, tn, tm);
-        const uint32_t red = smem_u32(stages);
-        const int rows = min(BN, g.M - tm * BN);
-        const int lo = rows * rank / g.splits, hi = rows * (rank + 1) / g.splits;
-        const int ch = threadIdx.x & 127, n = tn * MM_BM + ch;
-        const float sb = n < g.N ? g.sb[n] : 0.0f;
-        const float bias = g.bias != nullptr && n < g.N ? u2f((uint32_t)g.bias[n] << 16) : 0.0f;
-        for (int i = lo + (threadIdx.x >> 7); i < hi; i += MM_THREADS / 128) {
-            int32_t sum = 0;
+        const int rows = min(BN, g.M - tm * BN), lo = rows * rank / g.splits, hi = rows * (rank + 1) / g.splits;
+        const int n = tn * MM_BM + lane * 4;
+        const bool has_bias = g.bias != nullptr;
+        float sb[4], bias[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            sb[u] = n + u < g.N ? g.sb[n + u] : 0.0f;
+            bias[u] = has_bias && n + u < g.N ? u2f((uint32_t)g.bias[n + u] << 16) : 0.0f;
+        }
+        for (int i = lo + warp; i < hi; i += MM_THREADS / 32) {
+            int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 8
             for (int p = 0; p < g.splits; p++) {
                 uint32_t addr;
-                int32_t v;
-                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(red + (uint32_t)(i * MM_BM + ch) * 4u), "r"(p));
-                asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(addr));
-                sum += v;
+                int4 v;
+                asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(addr) : "r"(stages + (uint32_t)(i * MM_BM + lane * 4) * 4u), "r"(p));
+                asm volatile("ld.shared::cluster.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr));
+                sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
             }
-            if (n < g.N) {
-                float y = __fmul_rn(__fmul_rn((float)sum, s_sa[i]), sb);
-                if (g.bias != nullptr) y = __fadd_rn(y, bias);
-                mm_store(g, (int64_t)tm * BN + i, n, y);
+            const int s4[4] = {sum.x, sum.y, sum.z, sum.w};
+            const float sa = u2f(lds_volatile(s_sa + 4 * i));
+            T *dst = static_cast<T *>(g.out) + ((int64_t)tm * BN + i) * g.N + n;
+            T y[4];
+#pragma unroll
+            for (int u = 0; u < 4; u++) y[u] = OutType<OUT>::of(mm_scaled(s4[u], sa, sb[u], has_bias, bias[u]));
+            if (n < g.N && (1 << g.piece) >= 4 * (int)sizeof(T)) {      // (then N is a multiple of 4)
+                if (sizeof(T) == 4) *reinterpret_cast<uint4 *>(dst) = *reinterpret_cast<const uint4 *>(y);
+                else *reinterpret_cast<uint2 *>(dst) = make_uint2(reinterpret_cast<const uint32_t *>(y)[0], reinterpret_cast<const uint32_t *>(y)[1]);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+                    if (n + u < g.N) dst[u] = y[u];
             }
         }
         // no CTA leaves while another may still read its sums
@@ -290,7 +344,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
     }
 }
 
-template <int BN, bool SPLIT>
+template <int BN, bool SPLIT, int OUT>
 static int mm_launch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArgs &g, cudaStream_t st)
 {
     using C = MmCfg<BN>;
@@ -298,7 +352,7 @@ static int mm_launch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArgs 
     const int dev = current_device_slot();
     if (dev < 0) return QCC_ERR_ARG;
     if (!done.get(dev)) {
-        cudaError_t e = cudaFuncSetAttribute(int8_mm_kernel<BN, SPLIT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(int8_mm_kernel<BN, SPLIT, OUT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
         if (e != cudaSuccess) return (int)e;
         done.set(dev);
     }
@@ -308,13 +362,50 @@ static int mm_launch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArgs 
     cfg.blockDim = MM_THREADS;
     cfg.dynamicSmemBytes = C::SMEM;
     cfg.stream = st;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = SPLIT ? g.splits : 1;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = SPLIT ? g.splits : 1;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
-    cfg.numAttrs = SPLIT ? 1 : 0;
-    return (int)cudaLaunchKernelEx(&cfg, int8_mm_kernel<BN, SPLIT>, mw, mx, g);
+    cfg.numAttrs = SPLIT ? 2 : 1;
+    return (int)cudaLaunchKernelEx(&cfg, int8_mm_kernel<BN, SPLIT, OUT>, mw, mx, g);
+}
+template <int BN>
+static int mm_dispatch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArgs &g, int out, cudaStream_t st)
+{
+    if (g.splits > 1)
+        return out == QCC_OUT_BF16 ? mm_launch<BN, true, QCC_OUT_BF16>(mw, mx, g, st)
+               : out == QCC_OUT_F16 ? mm_launch<BN, true, QCC_OUT_F16>(mw, mx, g, st) : mm_launch<BN, true, QCC_OUT_F32>(mw, mx, g, st);
+    return out == QCC_OUT_BF16 ? mm_launch<BN, false, QCC_OUT_BF16>(mw, mx, g, st)
+           : out == QCC_OUT_F16 ? mm_launch<BN, false, QCC_OUT_F16>(mw, mx, g, st) : mm_launch<BN, false, QCC_OUT_F32>(mw, mx, g, st);
+}
+
+// Tokens a tile and shares of K for a product: the pair with the least estimated time.  A block of K takes the longer of its matrix
+// instructions (2 clocks a token, 128 at least: the weights' tile is read at 128 bytes a clock) and of its way from L2 (64 bytes a
+// clock and SM); a tile has a start and an end of about 2500 clocks, of which all but the first overlap with other tiles; adding up
+// over a cluster costs about 1500.
+static void mm_choose(int64_t M, int64_t N, int kblocks, int &bn, int &splits)
+{
+    const int sms = sm_count();
+    double best = 0;
+    bn = 0;
+    for (int b = 16; b <= 256; b *= 2) {
+        if (b > 16 && b / 2 >= M) break;
+        const int64_t tiles = (N + MM_BM - 1) / MM_BM * ((M + b - 1) / b);
+        const double block = b * 2 > 128 ? (b * 2 > (128 + b) * 2 ? b * 2 : (128 + b) * 2) : (128 + b) * 2;
+        for (int s = 1; s <= 8; s *= 2) {
+            if (s > 1 && (kblocks < 2 * s || tiles * s > sms)) break;
+            const int64_t waves = (tiles * s + sms - 1) / sms;
+            const double t = waves * ((kblocks + s - 1) / s) * block + 2500 + (waves - 1) * (b * 6.0) + (s > 1 ? 1500 : 0);
+            if (bn == 0 || t < best) {
+                best = t;
+                bn = b;
+                splits = s;
+            }
+        }
+    }
 }
 
 static int byte_map(CUtensorMap *map, const void *base, int64_t rows, int64_t cols, int box_rows)
@@ -342,14 +433,13 @@ extern "C" int qcc_int8_rowwise(const void *x, int64_t M, int64_t N, int flags, 
     const uint16_t *xp = static_cast<const uint16_t *>(x);
     uint8_t *qp = static_cast<uint8_t *>(q);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define QCC_I8(CH) int8_rowwise_kernel<CH><<<(unsigned)M, I8_THREADS, 0, st>>>(xp, N, qp, scale, recip)
+#define QCC_I8(CH) return (int)launch_maybe_pdl(int8_rowwise_kernel<CH>, dim3((unsigned)M), dim3(I8_THREADS), 0, st, true, xp, N, qp, scale, recip)
     if (N % 8 != 0 || N > 8 * 8 * I8_THREADS) QCC_I8(0);
-    else if (N <= 8 * I8_THREADS) QCC_I8(1);
-    else if (N <= 2 * 8 * I8_THREADS) QCC_I8(2);
-    else if (N <= 4 * 8 * I8_THREADS) QCC_I8(4);
-    else QCC_I8(8);
+    if (N <= 8 * I8_THREADS) QCC_I8(1);
+    if (N <= 2 * 8 * I8_THREADS) QCC_I8(2);
+    if (N <= 4 * 8 * I8_THREADS) QCC_I8(4);
+    QCC_I8(8);
 #undef QCC_I8
-    return (int)cudaGetLastError();
 }
 
 extern "C" int qcc_int8_scaled_mm(const void *a, const void *b, int64_t M, int64_t N, int64_t K, const float *scale_a, const float *scale_b,
@@ -360,25 +450,24 @@ extern "C" int qcc_int8_scaled_mm(const void *a, const void *b, int64_t M, int64
     if (M == 0 || N == 0) return 0;
     if (!a || !b || !scale_a || !scale_b || !out) return QCC_ERR_ARG;
     if (!aligned16(a) || !aligned16(b) || !aligned16(out)) return QCC_ERR_ALIGN;
-    int bn = M <= 16 ? 16 : M <= 32 ? 32 : M <= 64 ? 64 : M <= 128 ? 128 : 256;
-    const int64_t tiles_n = (N + MM_BM - 1) / MM_BM;
-    int64_t tiles_m = (M + bn - 1) / bn;
-    if (tiles_n * tiles_m > 0x7FFFFFFF) return QCC_ERR_SHAPE;
-    const int kblocks = (int)((K + MM_BK - 1) / MM_BK), sms = sm_count();
-    int splits = 1;
-    if (bn <= 128)   // fewer tiles than SMs: share K out over clusters of up to 8, at least 4 blocks of K each
-        while (splits < 8 && tiles_n * tiles_m * splits * 2 <= sms && kblocks >= 4 * splits * 2) splits *= 2;
-    MmArgs g = {scale_a, scale_b, static_cast<const uint16_t *>(bias), out, (int)M, (int)N, kblocks, (int)tiles_n, (int)tiles_m, splits, out_dtype};
+    const int kblocks = (int)((K + MM_BK - 1) / MM_BK);
+    int bn, splits;
+    mm_choose(M, N, kblocks, bn, splits);
+    const int64_t tiles_n = (N + MM_BM - 1) / MM_BM, tiles_m = (M + bn - 1) / bn;
+    if (tiles_n * tiles_m > 0x7FFFFFFF / 8) return QCC_ERR_SHAPE;
+    const int64_t row = N * (out_dtype == QCC_OUT_F32 ? 4 : 2);
+    const int piece = row % 16 == 0 ? 4 : row % 8 == 0 ? 3 : row % 4 == 0 ? 2 : 1;
+    const MmArgs g = {scale_a, scale_b, static_cast<const uint16_t *>(bias), out, (int)M, (int)N, kblocks, (int)tiles_n, (int)tiles_m, splits, piece};
     CUtensorMap mw, mx;
     int rc = byte_map(&mw, b, N, K, MM_BM);
     if (rc == 0) rc = byte_map(&mx, a, M, K, bn);
     if (rc) return rc;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     switch (bn) {
-    case 16: return splits > 1 ? mm_launch<16, true>(mw, mx, g, st) : mm_launch<16, false>(mw, mx, g, st);
-    case 32: return splits > 1 ? mm_launch<32, true>(mw, mx, g, st) : mm_launch<32, false>(mw, mx, g, st);
-    case 64: return splits > 1 ? mm_launch<64, true>(mw, mx, g, st) : mm_launch<64, false>(mw, mx, g, st);
-    case 128: return splits > 1 ? mm_launch<128, true>(mw, mx, g, st) : mm_launch<128, false>(mw, mx, g, st);
-    default: return mm_launch<256, false>(mw, mx, g, st);
+    case 16: return mm_dispatch<16>(mw, mx, g, out_dtype, st);
+    case 32: return mm_dispatch<32>(mw, mx, g, out_dtype, st);
+    case 64: return mm_dispatch<64>(mw, mx, g, out_dtype, st);
+    case 128: return mm_dispatch<128>(mw, mx, g, out_dtype, st);
+    default: return mm_dispatch<256>(mw, mx, g, out_dtype, st);
     }
 }

@@ -71,6 +71,14 @@ __device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsi
     atomicMax(&g_qcc_error, code);
 }
 
+__device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y)
+        : "memory");
+}
+
 // --------------------------------------------------------------------------------------------- tensor memory
 // The address of `cols` columns (a power of two >= 32) lands in `slot` (shared memory).  One whole warp calls it.
 __device__ __forceinline__ void tmem_alloc_at(uint32_t slot, uint32_t cols)
