@@ -38,6 +38,8 @@ template <int D>
 __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const AppendArgs g)
 {
     constexpr int TPR = D / 16, GROUPS = KV_THREADS / TPR;
+    pdl_trigger();
+    pdl_wait();
     const int t = threadIdx.x % TPR;
     const int rows = g.q_heads + 2 * g.kv_heads, per_token = (rows + KV_ROWS - 1) / KV_ROWS;
     const int64_t item = (int64_t)blockIdx.x * GROUPS + threadIdx.x / TPR;
@@ -56,7 +58,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const AppendArgs 
     uint4 xa[KV_ROWS], xb[KV_ROWS];
 #pragma unroll
     for (int i = 0; i < KV_ROWS; i++) {
-        const int r = part + i * per_token;      // queries first, then keys, then values
+        const int r = part * KV_ROWS + i;        // queries first, then keys, then values
         const uint16_t *p = nullptr;
         if (live && r < rows) {
             if (r < g.q_heads) p = g.q + token * g.q_token + r * g.q_head;
@@ -105,11 +107,15 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const AppendArgs 
             }
         }
     }
+    const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer), k_inv = __fdiv_rn(1.0f, k_outer), v_inv = __fdiv_rn(1.0f, v_outer);
+    // the page, and the place in it, of this token
+    const int shift = 31 - __clz(g.page), off = (int)(slot & (g.page - 1));
+    uint8_t *const page = g.cache + (slot >> shift) * ((int64_t)g.kv_heads * 2 * g.page * kv_row_bytes<D>());
     const bool turn_halves = !g.interleaved && t < g.rot / 16;
 
 #pragma unroll
     for (int i = 0; i < KV_ROWS; i++) {
-        const int r = part + i * per_token;
+        const int r = part * KV_ROWS + i;
         const bool is_q = r < g.q_heads, is_v = r >= g.q_heads + g.kv_heads;
         float a[8], b[8];
         const uint32_t wa[4] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w}, wb[4] = {xb[i].x, xb[i].y, xb[i].z, xb[i].w};
@@ -141,15 +147,27 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const AppendArgs 
                 }
             }
         }
-        // block maxima: the other half of a block is in the neighbouring thread (all lanes take part)
-        float ma = 0.0f, mb = 0.0f;
+        // Block maxima and scales, where the warp has a key or a value at all.  A block is half in this thread and half in its neighbour,
+        // so are two blocks: the even thread works out the scale of `ca`'s, the odd one that of `cb`'s (three divisions each).
+        float ra = 0.0f, rb = 0.0f;
+        uint32_t scale = 0;
+        const float outer = is_v ? v_outer : k_outer;
+        if (__any_sync(0xFFFFFFFFu, keep && r < rows && !is_q)) {
+            float ma = 0.0f, mb = 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            ma = max_nan(ma, fabsf(a[j]));
-            mb = max_nan(mb, fabsf(b[j]));
+            for (int j = 0; j < 8; j++) {
+                ma = max_nan(ma, fabsf(a[j]));
+                mb = max_nan(mb, fabsf(b[j]));
+            }
+            const bool odd = t & 1;
+            const float mine = max_nan(odd ? mb : ma, __shfl_xor_sync(0xFFFFFFFFu, odd ? ma : mb, 1));
+            float rec;
+            scale = nvfp4_inner(mine, outer, is_v ? v_inv : k_inv, rec, g.recip_div != 0);
+            if (mine != mine) scale = 0x7Fu;     // e4m3 NaN
+            const float other = __shfl_xor_sync(0xFFFFFFFFu, rec, 1);
+            ra = odd ? other : rec;
+            rb = odd ? rec : other;
         }
-        ma = max_nan(ma, __shfl_xor_sync(0xFFFFFFFFu, ma, 1));
-        mb = max_nan(mb, __shfl_xor_sync(0xFFFFFFFFu, mb, 1));
         if (!live || r >= rows) continue;
         if (is_q) {
             uint4 oa = make_uint4(0, 0, 0, 0), ob = oa;
@@ -165,16 +183,9 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const AppendArgs 
             o[cb] = ob;
         } else if (keep) {
             const int head = is_v ? r - g.q_heads - g.kv_heads : r - g.q_heads;
-            const float outer = is_v ? __ldg(g.v_outer) : __ldg(g.k_outer), inv = __fdiv_rn(1.0f, outer);
-            const int64_t pg = slot / g.page;
-            const int off = (int)(slot - pg * g.page);
-            uint8_t *base = g.cache + ((pg * g.kv_heads + head) * 2 + (is_v ? 1 : 0)) * (int64_t)(g.page * kv_row_bytes<D>());
+            uint8_t *base = page + (head * 2 + (is_v ? 1 : 0)) * (g.page * kv_row_bytes<D>());
             uint32_t *codes = reinterpret_cast<uint32_t *>(base + off * kv_row_codes<D>());
             uint8_t *scales = base + g.page * kv_row_codes<D>() + off * kv_row_scales<D>();
-            float ra, rb;
-            uint32_t sa = nvfp4_inner(ma, outer, inv, ra, g.recip_div != 0), sb = nvfp4_inner(mb, outer, inv, rb, g.recip_div != 0);
-            if (ma != ma) sa = 0x7Fu;     // e4m3 NaN
-            if (mb != mb) sb = 0x7Fu;
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 a[j] = __fmul_rn(a[j], ra);
@@ -182,10 +193,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_append_kernel(const AppendArgs 
             }
             codes[ca] = cvt_e2m1x8(a);
             codes[cb] = cvt_e2m1x8(b);
-            if (!(t & 1)) {
-                scales[ca >> 1] = (uint8_t)sa;
-                scales[cb >> 1] = (uint8_t)sb;
-            }
+            scales[(t & 1 ? cb : ca) >> 1] = (uint8_t)scale;
         }
     }
 }
@@ -205,6 +213,8 @@ template <int D>
 __global__ void __launch_bounds__(KV_THREADS) kv_gather_kernel(const GatherArgs g)
 {
     constexpr int TPR = D / 16, TOKENS = KV_THREADS / TPR;
+    pdl_trigger();
+    pdl_wait();
     const int t = threadIdx.x % TPR;
     const int64_t row = (int64_t)blockIdx.x * TOKENS + threadIdx.x / TPR;
     const int head = blockIdx.y;
@@ -298,9 +308,8 @@ extern "C" int qcc_nvfp4_kv_append(const qcc_kv_append_args *p, void *stream)
     const int64_t blocks = (p->tokens * per_token + groups - 1) / groups;
     if (blocks > 0x7FFFFFFF) return QCC_ERR_SHAPE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p->head_dim == 128) kv_append_kernel<128><<<(unsigned)blocks, KV_THREADS, 0, st>>>(g);
-    else kv_append_kernel<64><<<(unsigned)blocks, KV_THREADS, 0, st>>>(g);
-    return (int)cudaGetLastError();
+    return (int)(p->head_dim == 128 ? launch_maybe_pdl(kv_append_kernel<128>, dim3((unsigned)blocks), dim3(KV_THREADS), 0, st, true, g)
+                                    : launch_maybe_pdl(kv_append_kernel<64>, dim3((unsigned)blocks), dim3(KV_THREADS), 0, st, true, g));
 }
 
 extern "C" int qcc_nvfp4_kv_gather(const void *cache, int64_t num_pages, int kv_heads, int page, int head_dim, const int32_t *table,
@@ -320,7 +329,6 @@ extern "C" int qcc_nvfp4_kv_gather(const void *cache, int64_t num_pages, int kv_
     if (blocks > 0x7FFFFFFF) return QCC_ERR_SHAPE;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const dim3 grid((unsigned)blocks, (unsigned)kv_heads);
-    if (head_dim == 128) kv_gather_kernel<128><<<grid, KV_THREADS, 0, st>>>(g);
-    else kv_gather_kernel<64><<<grid, KV_THREADS, 0, st>>>(g);
-    return (int)cudaGetLastError();
+    return (int)(head_dim == 128 ? launch_maybe_pdl(kv_gather_kernel<128>, grid, dim3(KV_THREADS), 0, st, true, g)
+                                 : launch_maybe_pdl(kv_gather_kernel<64>, grid, dim3(KV_THREADS), 0, st, true, g));
 }
