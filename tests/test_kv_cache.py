@@ -161,6 +161,7 @@ APPEND = [  # D, page, kv heads, q heads, rot, interleaved, tokens
     (128, 16, 8, 32, 128, False, 5), (128, 32, 2, 0, 128, False, 67), (128, 64, 1, 4, 64, False, 33), (128, 128, 3, 3, 32, False, 130),
     (128, 16, 2, 10, 96, False, 9), (64, 16, 2, 4, 64, False, 40), (64, 32, 1, 12, 32, True, 21), (64, 64, 4, 4, 64, True, 1),
     (128, 16, 2, 2, 128, True, 50), (128, 32, 2, 2, 64, True, 7), (64, 128, 5, 0, 0, False, 300), (128, 16, 1, 1, 0, False, 1), (64, 16, 1, 0, 32, False, 2),
+    (128, 32, 8, 32, 128, False, 1500), (128, 64, 4, 17, 128, True, 1100),       # millions of roundings
 ]
 
 
