@@ -39,11 +39,24 @@ constexpr int SP_WARPS = 4, SP_THREADS = SP_WARPS * 32, SP_WTOK = 32, SP_TOK = S
 
 template <int D, int NT> struct SplitCfg {
     static constexpr int TILE = SP_WTOK * 2 * (D / 2 + D / 16);     // bytes of one warp's tokens, keys and values
-    static constexpr int CTAS = NT == 1 ? 4 : 2;
-    static constexpr int STAGES = (NT == 1 ? 2 : 4) * (D == 64 ? 2 : 1);
+#ifndef MANY
+#define MANY 32
+#endif
+#ifndef XU
+#define XU (NT == 4 ? 1 : 2)
+#endif
+#ifndef XC
+#define XC (NT == 1 ? 4 : NT == 2 ? (D == 64 ? 4 : 3) : 2)
+#define XS (NT == 1 ? 2 : NT == 2 ? 2 : 4)
+#define XH (NT >= 2 ? 1 : 2)
+#endif
+    static constexpr int CTAS = XC;
+    static constexpr int STAGES = XS * (D == 64 ? 2 : 1);
+    static constexpr bool QS = NT * D > 256;                        // Q in shared memory: it would not fit the registers beside O
+    static constexpr int QBYTES = QS ? NT * (D / 32) * 32 * 16 : 0;
     static constexpr int RED = SP_WARPS * NT * 8 * (D / 4) * 4;
     static constexpr int ML = SP_WARPS * NT * 8 * 2 * 4;
-    static constexpr int FIXED = SP_WARPS * (TILE * STAGES + STAGES * 8) + RED + ML;
+    static constexpr int FIXED = SP_WARPS * (TILE * STAGES + STAGES * 8) + RED + ML + QBYTES;
 };
 
 template <int D, int NT> __host__ __device__ constexpr int part_floats() { return NT * 8 * (D + 2); }   // sums (NT * 8, D), then (maximum, denominator) of each row
@@ -78,7 +91,8 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t *ring = smem + warp * (C::TILE * C::STAGES);
     float *red = reinterpret_cast<float *>(smem + SP_WARPS * C::TILE * C::STAGES);
-    float2 *ml = reinterpret_cast<float2 *>(red + C::RED / 4);
+    uint4 *s_q = reinterpret_cast<uint4 *>(red + C::RED / 4);
+    float2 *ml = reinterpret_cast<float2 *>(s_q + C::QBYTES / 16);
     uint64_t *full = reinterpret_cast<uint64_t *>(ml + C::ML / 8) + warp * C::STAGES;
     int32_t *prefix = reinterpret_cast<int32_t *>(reinterpret_cast<uint64_t *>(ml + C::ML / 8) + SP_WARPS * C::STAGES);
     __shared__ int32_t wsum[SP_WARPS];
@@ -206,7 +220,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         const int rows = s.n * g.group;
         if (t == lo && threadIdx.x == 0) note_seam(g, s.first ? t - s.first : -1, s.unit_last, total, rows, s.q0, s.head, 0);
 
-        uint32_t qf[NT][2 * KW * 2];    // row gr of each n tile, elements of this thread
+        uint32_t qf[C::QS ? 1 : NT][2 * KW * 2];    // row gr of each n tile, elements of this thread
         float factor[NT][2];            // score -> log2 units, columns 2c and 2c + 1
         int limit[NT][2];               // keys that the column sees
 #pragma unroll
@@ -227,10 +241,12 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
             q_power(m, mult, back);
 #pragma unroll
             for (int j = 0; j < KW; j++) {
-                qf[nt][4 * j] = pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult);
-                qf[nt][4 * j + 1] = pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult);
-                qf[nt][4 * j + 2] = pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult);
-                qf[nt][4 * j + 3] = pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult);
+                uint32_t *f4 = qf[C::QS ? 0 : nt] + 4 * j;
+                f4[0] = pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult);
+                f4[1] = pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult);
+                f4[2] = pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult);
+                f4[3] = pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult);
+                if (C::QS && warp == nt % SP_WARPS) s_q[(nt * KW + j) * 32 + lane] = make_uint4(f4[0], f4[1], f4[2], f4[3]);
             }
 #pragma unroll
             for (int x = 0; x < 2; x++) {
@@ -240,6 +256,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
             }
         }
 
+        if (C::QS) named_barrier(1, SP_WARPS * 32);
         float o[NT][MT][4], m[NT][2], l[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -252,8 +269,8 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         const auto step = [&](auto masked, int tok) {
             constexpr bool MASKED = decltype(masked)::value;
             const uint32_t base = smem_u32(ring + stage * C::TILE);
-            constexpr int HB = NT == 4 ? 1 : 2;      // 16-token blocks taken together, as registers allow
-#pragma unroll
+            constexpr int HB = XH, UH = XU;      // 16-token blocks taken together, as registers allow
+#pragma unroll UH
             for (int h0 = 0; h0 < 2; h0 += HB) {
                 float sc[HB][NT][4];
 #pragma unroll
@@ -288,8 +305,10 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++) {
-                            mma16816(sc[h][nt], ha[0], hb[0], ha[1], hb[1], qf[nt][4 * j], qf[nt][4 * j + 1]);
-                            mma16816(sc[h][nt], ha[2], hb[2], ha[3], hb[3], qf[nt][4 * j + 2], qf[nt][4 * j + 3]);
+                            const uint32_t *r4 = qf[C::QS ? 0 : nt] + 4 * j;
+                            const uint4 q4 = C::QS ? lds_v4(smem_u32(s_q + (nt * KW + j) * 32 + lane)) : make_uint4(r4[0], r4[1], r4[2], r4[3]);
+                            mma16816(sc[h][nt], ha[0], hb[0], ha[1], hb[1], q4.x, q4.y);
+                            mma16816(sc[h][nt], ha[2], hb[2], ha[3], hb[3], q4.z, q4.w);
                         }
                     }
                 }
@@ -490,7 +509,7 @@ static int split_launch(const AttnArgs &g, cudaStream_t st)
 // how the rows of a sequence and kv head are tiled: 8 * nt rows
 static int row_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 // more rows than one row tile: the tcgen05 kernel
-static bool many_queries(int max_q, int group) { return (int64_t)max_q * group > 32; }
+static bool many_queries(int max_q, int group) { return (int64_t)max_q * group > MANY; }
 
 }  // namespace qcc
 

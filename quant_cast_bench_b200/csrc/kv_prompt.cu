@@ -10,7 +10,8 @@ namespace qcc {
 // Many queries: bound by the tensor cores and by the exponentials
 //
 // A unit is 256 rows (queries times the heads of a group, token-major) of a sequence and kv head: two row tiles of 128, whose
-// softmaxes take turns with the matrix instructions.  For each tile of 128 tokens
+// softmaxes take turns with the matrix instructions.  (Of up to 128 rows both softmaxes take the one row tile, and the tiles of
+// tokens in turn.)  For each tile of 128 tokens
 //   S = Q K^T   128 x 128 x D, Q and K in shared memory, S in tensor memory;
 //   P = exp2(S * factor - m), one thread a row, written back over S as fp16;
 //   O += P V    P from tensor memory, V in shared memory (its elements contiguous: the N-major form), O in tensor memory.
@@ -24,14 +25,14 @@ namespace qcc {
 // many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3;
-constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u;      // notes on a tile: the last of its part; both row tiles have rows
+constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u;      // notes on a tile: the last of its part; both row tiles of its unit have rows
 constexpr unsigned int PT_ERR = 9u;    // a barrier wait of this kernel ran out
 
 template <int D> struct PromptCfg {
     static constexpr int BLOCKS = D / 64;                       // 64-element blocks of a row: 128 bytes of fp16
     static constexpr int TILE = BLOCKS * 128 * 128;             // 128 rows of Q, K or V as fp16
     static constexpr int RAW = PT_TOK * kv_row_bytes<D>();      // codes and scales of 128 tokens, keys or values
-    static constexpr int SMEM = 1024 + 6 * TILE + PT_RAW * RAW + 256;
+    static constexpr int SMEM = 1024 + 6 * TILE + PT_RAW * RAW + 256 + 128 * 8;
 };
 
 // ---- numbering: prefix[p] = tiles of all (sequence, row tile) pairs before p, times the kv heads; pairs[p] = (sequence, row tile)
@@ -222,7 +223,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
     const uint32_t s_q = sm, s_k = sm + 2 * C::TILE, s_v = sm + 4 * C::TILE, s_raw = sm + 6 * C::TILE, bars = s_raw + PT_RAW * C::RAW;
     const uint32_t raw_full = bars, raw_empty = bars + 24, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96, q_full = bars + 112,
                    s_full = bars + 128, p_full = bars + 144, o_done = bars + 160;
-    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212;      // notes of the last 8 tiles: tokens that exist, PT_LAST, PT_TWO
+    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_ml = bars + 256;      // notes of the last 8 tiles: tokens that exist, PT_LAST, PT_TWO
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
@@ -328,35 +329,66 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 }
                 tc_commit_at(s_full + 8 * (x));
             };
+            const auto product = [&](int x, uint32_t vb, uint32_t add) {      // add: whether O holds anything
+                const uint32_t b = dv + vb * (C::TILE >> 4);
+#pragma unroll
+                for (int k = 0; k < PT_TOK / 16; k++)
+                    asm volatile(
+                        "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\n"
+                        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(tmem + 256 + x * 128),
+                        "r"(tmem + x * 128 + k * 8), "r"(b + k * 128), "r"(id_o), "r"(k > 0 ? 1u : add), "r"(high)
+                        : "memory");
+                tc_commit_at(o_done + 8 * (x));
+            };
             const uint32_t count = hi - lo;
             while (kt < count) {
                 // a part's first scores
                 mbar_wait_at(k_full + 8 * (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
                 uint32_t info = lds_volatile(s_info + 4 * (kt & 7));
-                const int nx = info & PT_TWO ? 2 : 1;
-                for (int x = 0; x < nx; x++) {
+                if (!(info & PT_TWO)) {
+                    // one row tile: both softmaxes have the same rows, and take the tiles of tokens in turn
+                    const auto next = [&](int x) {
+                        mbar_wait_at(k_full + 8 * (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
+                        info = lds_volatile(s_info + 4 * (kt & 7));
+                        tc_fence_after();
+                        scores(x, kt & 1);
+                        tc_commit_at(k_empty + 8 * (kt & 1));
+                        kt++;
+                    };
+                    mbar_wait_at(q_full, qn[0]++ & 1, PT_ERR, abort);
+                    next(0);
+                    if (!(info & PT_LAST)) {
+                        mbar_wait_at(q_full + 8, qn[1]++ & 1, PT_ERR, abort);
+                        next(1);
+                    }
+                    for (uint32_t j = 0; vt != kt && !lds_volatile(abort); j++) {
+                        const int x = j & 1;
+                        mbar_wait_at(v_full + 8 * (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
+                        mbar_wait_at(p_full + 8 * x, pn[x]++ & 1, PT_ERR, abort);
+                        tc_fence_after();
+                        product(x, vt & 1, j > 1);
+                        tc_commit_at(v_empty + 8 * (vt & 1));
+                        vt++;
+                        if (!(info & PT_LAST)) next(x);
+                    }
+                    if (lds_volatile(abort)) break;
+                    continue;
+                }
+                for (int x = 0; x < 2; x++) {
                     mbar_wait_at(q_full + 8 * (x), qn[x]++ & 1, PT_ERR, abort);
                     tc_fence_after();
                     scores(x, kt & 1);
                 }
                 tc_commit_at(k_empty + 8 * (kt & 1));
                 kt++;
-                for (uint32_t o = 0;; o = 1) {      // o: whether O holds anything
+                for (uint32_t o = 0;; o = 1) {
                     const bool more = !(info & PT_LAST);
                     mbar_wait_at(v_full + 8 * (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
                     if (more) mbar_wait_at(k_full + 8 * (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
-                    for (int x = 0; x < nx; x++) {
+                    for (int x = 0; x < 2; x++) {
                         mbar_wait_at(p_full + 8 * (x), pn[x]++ & 1, PT_ERR, abort);
                         tc_fence_after();
-                        const uint32_t b = dv + (vt & 1) * (C::TILE >> 4);
-#pragma unroll
-                        for (int k = 0; k < PT_TOK / 16; k++)
-                            asm volatile(
-                                "{\n.reg .pred p;\n.reg .b64 b;\nsetp.ne.b32 p, %4, 0;\nmov.b64 b, {%2, %5};\n"
-                                "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n}\n" ::"r"(tmem + 256 + x * 128),
-                                "r"(tmem + x * 128 + k * 8), "r"(b + k * 128), "r"(id_o), "r"(k > 0 ? 1u : o), "r"(high)
-                                : "memory");
-                        tc_commit_at(o_done + 8 * (x));
+                        product(x, vt & 1, o);
                         if (more) scores(x, kt & 1);      // over P: instructions run in order, the product above has read it
                     }
                     tc_commit_at(v_empty + 8 * (vt & 1));
@@ -432,8 +464,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
         const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
         uint32_t sn = 0, on = 0;        // scores, products so far
         QCC_FOR_PARTS(s, t) {
-            const int64_t rows = (int64_t)s.n * g.group, r = (int64_t)s.qt * PT_ROWS + x * 128 + row;
-            const bool live = r < rows, idle = rows - (int64_t)s.qt * PT_ROWS <= x * 128;      // idle: no row of this tile exists
+            // both row tiles have rows: one for each softmax; one has: both softmaxes take it, and the tiles of tokens in turn
+            const bool two = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128;
+            const int64_t rows = (int64_t)s.n * g.group, r = (int64_t)s.qt * PT_ROWS + (two ? x * 128 : 0) + row;
+            const int first = two ? s.first : s.first + x, step = two ? 1 : 2;
+            const bool live = r < rows, idle = first >= s.last;
             const int i = live ? (int)(r / g.group) : 0, h = s.head * g.group + (live ? (int)(r - (int64_t)i * g.group) : 0);
             const int limit = live ? s.L - s.n + i + 1 : 0;
             float factor = 0.0f;
@@ -460,7 +495,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at(q_full + 8 * x);
                 float m = -INFINITY, l = 0.0f;
-                for (int tile = s.first; tile < s.last; tile++) {
+                for (int tile = first; tile < s.last; tile += step) {
                     mbar_wait_at(s_full + 8 * (x), sn++ & 1, PT_ERR, abort);
                     tc_fence_after();
                     uint32_t v[4][32];
@@ -488,7 +523,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                         const float up = grow ? most : m, a = grow ? ex2(m - up) : 1.0f;
                         m = up;
                         l *= a;
-                        if (tile > s.first) {
+                        if (tile > first) {
                             mbar_wait_at(o_done + 8 * x, (on - 1) & 1, PT_ERR, abort);
                             tc_fence_after();
 #pragma unroll
@@ -533,7 +568,35 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 }
                 mbar_wait_at(o_done + 8 * (x), (on - 1) & 1, PT_ERR, abort);
                 tc_fence_after();
-                const bool whole = s.first == 0 && s.last == s.tiles;
+                const bool whole = s.first == 0 && s.last == s.tiles, join = !two && s.last - s.first > 1;
+                float mine = 1.0f, others = 0.0f;         // weights of this softmax's sums and of the other's
+                if (join) {
+                    // the second softmax hands its sums over in Q's place, column by column
+                    named_barrier(1, 256);                // (both are done with Q)
+                    if (x) {
+#pragma unroll
+                        for (int c = 0; c < D; c += 16) {
+                            uint32_t o[16];
+                            tmem_ld16(t_o + c, o);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int j = 0; j < 16; j++) sts_u32(s_q + ((c + j) * 128 + row) * 4, o[j]);
+                        }
+                        sts_u32(s_ml + row * 8, f2u(m));
+                        sts_u32(s_ml + row * 8 + 4, f2u(l));
+                        tc_fence_before();
+                    }
+                    named_barrier(1, 256);
+                    if (x) {
+                        named_barrier(1, 256);            // (the sums are read)
+                        continue;
+                    }
+                    const float m1 = u2f(lds_volatile(s_ml + row * 8)), l1 = u2f(lds_volatile(s_ml + row * 8 + 4)), up = fmaxf(m, m1);
+                    mine = m == -INFINITY ? 1.0f : ex2(m - up);
+                    others = m1 == -INFINITY ? 1.0f : ex2(m1 - up);
+                    m = up;
+                    l = l * mine + l1 * others;
+                }
                 const float scale = l == 0.0f ? 0.0f : __fdividef(v_outer, l);
                 const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + h;
                 float *part = g.part + (size_t)(2 * blockIdx.x + (t == lo ? 0 : 1)) * prompt_part_floats<D>();
@@ -542,6 +605,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     uint32_t o[16];
                     tmem_ld16(t_o + c, o);
                     tmem_wait_ld();
+                    if (join) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) o[j] = f2u(u2f(o[j]) * mine + u2f(lds_volatile(s_q + ((c + j) * 128 + row) * 4)) * others);
+                    }
                     if (whole) {
                         uint32_t y[8];
 #pragma unroll
@@ -563,6 +630,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 if (!whole) reinterpret_cast<float2 *>(part + PT_ROWS * D)[x * 128 + row] = make_float2(m, l);
                 else if (live && g.lse) g.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
                 tc_fence_before();       // the next unit's products write O
+                if (join) named_barrier(1, 256);
             }
         }
     }
