@@ -454,11 +454,14 @@ __device__ __forceinline__ void mbar_expect_tx(uint64_t *bar, uint32_t bytes)
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
                  : "memory");
 }
+__device__ __forceinline__ void mbar_expect_at(uint32_t bar, uint32_t bytes)
+{
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+}
 // Wait for phase `parity` with an iteration cap; on timeout record the code and carry on (the caller
 // then works on whatever is in shared memory, but never hangs).
-__device__ __forceinline__ void mbar_wait(uint64_t *bar, uint32_t parity, unsigned int err_code)
+__device__ __forceinline__ void mbar_wait_addr(uint32_t a, uint32_t parity, unsigned int err_code)
 {
-    uint32_t a = smem_u32(bar);
     for (uint32_t it = 0; it < (1u << 24); it++) {
         uint32_t done;
         asm volatile(
@@ -472,6 +475,7 @@ __device__ __forceinline__ void mbar_wait(uint64_t *bar, uint32_t parity, unsign
     }
     atomicMax(&g_qcc_error, err_code);
 }
+__device__ __forceinline__ void mbar_wait(uint64_t *bar, uint32_t parity, unsigned int err_code) { mbar_wait_addr(smem_u32(bar), parity, err_code); }
 __device__ __forceinline__ void fence_barrier_init()
 {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

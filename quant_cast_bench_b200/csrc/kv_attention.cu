@@ -10,6 +10,11 @@
 
 #include "host_util.h"
 
+#ifndef XC
+#define XC 4
+#define XH 2
+#define XU 2
+#endif
 namespace qcc {
 
 constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ran out
@@ -37,21 +42,13 @@ constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ra
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int SP_WARPS = 4, SP_THREADS = SP_WARPS * 32, SP_WTOK = 32, SP_TOK = SP_WTOK * SP_WARPS;
 
+// CTAs on an SM, as the registers allow: the grid, and with it the workspace, is that many for each SM
+constexpr int split_ctas(int D, int NT) { return NT == 1 ? XC : NT == 2 ? (D == 64 ? 4 : 3) : 2; }
+
 template <int D, int NT> struct SplitCfg {
     static constexpr int TILE = SP_WTOK * 2 * (D / 2 + D / 16);     // bytes of one warp's tokens, keys and values
-#ifndef MANY
-#define MANY 32
-#endif
-#ifndef XU
-#define XU (NT == 4 ? 1 : 2)
-#endif
-#ifndef XC
-#define XC (NT == 1 ? 4 : NT == 2 ? (D == 64 ? 4 : 3) : 2)
-#define XS (NT == 1 ? 2 : NT == 2 ? 2 : 4)
-#define XH (NT >= 2 ? 1 : 2)
-#endif
-    static constexpr int CTAS = XC;
-    static constexpr int STAGES = XS * (D == 64 ? 2 : 1);
+    static constexpr int CTAS = split_ctas(D, NT);
+    static constexpr int STAGES = (NT == 4 ? 4 : 2) * (D == 64 ? 2 : 1);
     static constexpr bool QS = NT * D > 256;                        // Q in shared memory: it would not fit the registers beside O
     static constexpr int QBYTES = QS ? NT * (D / 32) * 32 * 16 : 0;
     static constexpr int RED = SP_WARPS * NT * 8 * (D / 4) * 4;
@@ -152,60 +149,50 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     const int lo = (int)((int64_t)total * blockIdx.x / ctas), hi = (int)((int64_t)total * (blockIdx.x + 1) / ctas);
 
     // ---- fetching: the warp's tokens of tile after tile, C::STAGES ahead of their use.  The pages of the next fetch are looked up
-    // one fetch early.  Pages of 32 tokens and more: four copies (codes and scales, keys and values); pages of 16: two of a whole
-    // (page, head) block.
-    const int shift = 31 - __clz(g.page);
-    const uint32_t block_bytes = (uint32_t)g.page * 2 * RB;
-    struct { Segment s; int t, tile, end; int32_t page; } f;     // page: lanes 0 and 1 hold the first and second 16 tokens' page
+    // one fetch early.  Pages of 32 tokens and more: four copies (codes and scales, keys and values), by a lane each; pages of 16:
+    // two of a whole (page, head) block.  What a lane copies, and to where, is the same for every tile.
+    const int shift = 31 - __clz(g.page), copies = shift == 4 ? 2 : 4;
+    const uint32_t block_bytes = (uint32_t)g.page * 2 * RB, page_bytes = block_bytes * g.kv_heads, num_pages = (uint32_t)min(g.num_pages, (int64_t)0x7FFFFFFF);
+    const uint32_t in_page = (warp * SP_WTOK) & (g.page - 1), scales_of = lane & 1;
+    const uint32_t lane_src = shift == 4 ? 0 : (lane >> 1 & 1) * (g.page * RB) + (scales_of ? g.page * (D / 2) + in_page * (D / 16) : in_page * (D / 2));
+    const uint32_t lane_dst = smem_u32(ring) + (shift == 4 ? lane * (C::TILE / 2) : (lane >> 1) * (C::TILE / 2) + scales_of * (SP_WTOK * D / 2));
+    const uint32_t lane_bytes = shift == 4 ? C::TILE / 2 : scales_of ? SP_WTOK * D / 16 : SP_WTOK * D / 2;
+    const uint32_t bar0 = smem_u32(full);
+    int f_t = lo, f_left = 0, f_tok = 0, f_L = 0, f_page = -1;      // next segment; tiles left of this one; this lane's first token, and its page
     uint32_t f_stage = 0;
-    f.t = lo;
-    // moves the cursor to the next tile that exists (f.t < hi), and asks for its pages
-    auto seek = [&](bool fresh) {
-        for (;;) {
-            if (!fresh) {
-                if (++f.tile < f.end) break;
-                f.t += f.s.last - f.s.first;
-            }
-            if (f.t >= hi) return;
-            find_segment(g, prefix, f.t, hi, f.s);
-            f.tile = f.s.first - 1;
-            f.end = f.s.last;
-            fresh = false;
+    const int32_t *f_row = nullptr;
+    const uint8_t *f_base = nullptr;
+    const auto seek = [&]() {
+        if (--f_left > 0) {
+            f_tok += SP_TOK;
+            f_row += SP_TOK >> shift;
+        } else if (f_t < hi) {
+            Segment s;
+            find_segment(g, prefix, f_t, hi, s);
+            f_left = s.last - s.first;
+            f_t += f_left;
+            f_L = s.L;
+            f_tok = s.first * SP_TOK + warp * SP_WTOK + (shift == 4 ? lane * 16 : 0);
+            f_row = g.table + s.b * g.table_stride + (f_tok >> shift);
+            f_base = g.cache + s.head * (int64_t)block_bytes + lane_src;
         }
-        const int tok = f.tile * SP_TOK + warp * SP_WTOK + (lane & 1) * 16;
-        f.page = tok < f.s.L ? __ldg(g.table + f.s.b * g.table_stride + (tok >> shift)) : -1;
+        f_page = f_left > 0 && lane < copies && f_tok < f_L ? __ldg(f_row) : -1;
     };
-    auto fetch = [&]() {
-        if (f.t >= hi) return;
-        uint64_t *bar = full + f_stage;
-        uint8_t *dst = ring + f_stage * C::TILE;
-        const int tok = f.tile * SP_TOK + warp * SP_WTOK;
-        const bool ok = f.page >= 0 && f.page < g.num_pages;
-        if (!ok && lane < 2 && tok + lane * 16 < f.s.L) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
-        if (shift == 4) {
-            const uint32_t both = __ballot_sync(0xFFFFFFFFu, ok) & 3u;
-            if (lane == 0) mbar_expect_tx(bar, __popc(both) * (C::TILE / 2));
-            __syncwarp();
-            if (lane < 2 && ok) bulk_load(dst + lane * (C::TILE / 2), g.cache + ((int64_t)f.page * g.kv_heads + f.s.head) * block_bytes, C::TILE / 2, bar);
-        } else {
-            const int32_t pg = __shfl_sync(0xFFFFFFFFu, f.page, 0);
-            const bool good = pg >= 0 && pg < g.num_pages;
-            if (lane == 0) mbar_expect_tx(bar, good ? C::TILE : 0);
-            __syncwarp();
-            if (good && lane < 4) {
-                const int off = tok & (g.page - 1), scales = lane & 1;
-                const uint8_t *src = g.cache + ((int64_t)pg * g.kv_heads + f.s.head) * block_bytes + (lane >> 1) * (g.page * RB);
-                bulk_load(dst + (lane >> 1) * (C::TILE / 2) + scales * (SP_WTOK * D / 2), src + (scales ? g.page * (D / 2) + off * (D / 16) : off * (D / 2)),
-                          scales ? SP_WTOK * D / 16 : SP_WTOK * D / 2, bar);
-            }
-        }
+    const auto fetch = [&]() {
+        if (f_left <= 0) return;
+        const bool ok = (uint32_t)f_page < num_pages;
+        if (!ok && lane < copies && f_tok < f_L) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
+        const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, ok)) * (shift == 4 ? C::TILE / 2 : C::TILE / 4), bar = bar0 + f_stage * 8;
+        if (lane == 0) mbar_expect_at(bar, bytes);
+        __syncwarp();
+        if (ok) bulk_load_at(lane_dst + f_stage * C::TILE, f_base + (uint64_t)(uint32_t)f_page * page_bytes, lane_bytes, bar);
         f_stage = f_stage + 1 == C::STAGES ? 0 : f_stage + 1;
-        seek(false);
+        seek();
     };
     // where a stage has codes and scales of keys and values, and the distance from the first 16 tokens to the second
     const uint32_t k_scales = shift == 4 ? 8 * D : SP_WTOK * D / 2, v_codes = shift == 4 ? 16 * RB : C::TILE / 2, v_scales = v_codes + k_scales;
     const uint32_t next_codes = shift == 4 ? C::TILE / 2 : 8 * D, next_scales = shift == 4 ? C::TILE / 2 : D;
-    seek(true);
+    seek();
 #pragma unroll 1
     for (int i = 0; i < C::STAGES; i++) fetch();
 
@@ -269,7 +256,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         const auto step = [&](auto masked, int tok) {
             constexpr bool MASKED = decltype(masked)::value;
             const uint32_t base = smem_u32(ring + stage * C::TILE);
-            constexpr int HB = XH, UH = XU;      // 16-token blocks taken together, as registers allow
+            constexpr int HB = NT == 1 ? XH : 1, UH = NT == 1 ? XU : NT == 2 ? 2 : 1;      // 16-token blocks taken together, as registers allow
 #pragma unroll UH
             for (int h0 = 0; h0 < 2; h0 += HB) {
                 float sc[HB][NT][4];
@@ -408,7 +395,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         const int clear = s.L - s.n + 1;      // keys that every row sees
 
         for (int tile = s.first; tile < end; tile++) {
-            mbar_wait(full + stage, phase, KV_ATTN_ERR);
+            mbar_wait_addr(bar0 + stage * 8, phase, KV_ATTN_ERR);
             const int tok = tile * SP_TOK + warp * SP_WTOK;
             if (tok + SP_WTOK <= clear) step(std::false_type(), tok);
             else if (tok < s.L) step(std::true_type(), tok);
@@ -509,7 +496,7 @@ static int split_launch(const AttnArgs &g, cudaStream_t st)
 // how the rows of a sequence and kv head are tiled: 8 * nt rows
 static int row_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 4; }
 // more rows than one row tile: the tcgen05 kernel
-static bool many_queries(int max_q, int group) { return (int64_t)max_q * group > MANY; }
+static bool many_queries(int max_q, int group) { return (int64_t)max_q * group > 32; }
 
 }  // namespace qcc
 
@@ -522,7 +509,7 @@ extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int64_t rows, int seqs,
     if (rows < 0 || seqs < 0 || max_q < 1 || kv_heads < 1 || q_heads < kv_heads || q_heads % kv_heads || (head_dim != 64 && head_dim != 128)) return 0;
     if (many_queries(max_q, q_heads / kv_heads)) return prompt_workspace_bytes(rows, q_heads / kv_heads, seqs, head_dim);
     const int nt = row_tiles_of((int64_t)max_q * (q_heads / kv_heads));
-    return (size_t)2 * sm_count() * (nt == 1 ? 4 : 2) * (16 + nt * 8 * (head_dim + 2) * 4);
+    return (size_t)sm_count() * split_ctas(head_dim, nt) * 2 * (16 + nt * 8 * (head_dim + 2) * 4);
 }
 
 extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *workspace, size_t workspace_bytes, void *stream)
@@ -552,7 +539,7 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     g.out = static_cast<uint16_t *>(p->out);
     g.lse = p->lse;
     g.seams = static_cast<int4 *>(workspace);
-    g.part = reinterpret_cast<float *>(g.seams + 2 * sm_count() * (nt == 1 ? 4 : 2));
+    g.part = reinterpret_cast<float *>(g.seams + 2 * sm_count() * split_ctas(p->head_dim, nt));
     g.q_token = p->q_stride[0]; g.q_head = p->q_stride[1];
     g.table_stride = p->table_stride; g.num_pages = p->num_pages; g.rows = p->rows;
     g.scale_log2 = p->scale * LOG2E;
