@@ -10,11 +10,6 @@
 
 #include "host_util.h"
 
-#ifndef XC
-#define XC 4
-#define XH 2
-#define XU 2
-#endif
 namespace qcc {
 
 constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ran out
@@ -43,7 +38,7 @@ constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ra
 constexpr int SP_WARPS = 4, SP_THREADS = SP_WARPS * 32, SP_WTOK = 32, SP_TOK = SP_WTOK * SP_WARPS;
 
 // CTAs on an SM, as the registers allow: the grid, and with it the workspace, is that many for each SM
-constexpr int split_ctas(int D, int NT) { return NT == 1 ? XC : NT == 2 ? (D == 64 ? 4 : 3) : 2; }
+constexpr int split_ctas(int D, int NT) { return NT == 1 ? 4 : NT == 2 ? (D == 64 ? 4 : 3) : 2; }
 
 template <int D, int NT> struct SplitCfg {
     static constexpr int TILE = SP_WTOK * 2 * (D / 2 + D / 16);     // bytes of one warp's tokens, keys and values
@@ -256,7 +251,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         const auto step = [&](auto masked, int tok) {
             constexpr bool MASKED = decltype(masked)::value;
             const uint32_t base = smem_u32(ring + stage * C::TILE);
-            constexpr int HB = NT == 1 ? XH : 1, UH = NT == 1 ? XU : NT == 2 ? 2 : 1;      // 16-token blocks taken together, as registers allow
+            constexpr int HB = NT == 1 ? 2 : 1, UH = NT == 4 ? 1 : 2;      // 16-token blocks taken together, as registers allow
 #pragma unroll UH
             for (int h0 = 0; h0 < 2; h0 += HB) {
                 float sc[HB][NT][4];
@@ -351,7 +346,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                     }
                     // values of tokens 2c, 2c + 1 and 2c + 8, 2c + 9
                     const uint32_t vc = base + v_codes + (h0 + h) * next_codes, vs = base + v_scales + (h0 + h) * next_scales;
-                    uint32_t vs2[2], vw[4][VW];
+                    uint32_t vs2[2], vw[4][VW], nan = 0;      // nan: tokens whose block of this thread's elements is NaN
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
                         const int t0 = 2 * c + 8 * x;
@@ -359,6 +354,10 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                         if (MASKED) {        // whatever the slots behind the last token hold, it counts as zero
                             if (tok + (h0 + h) * 16 + t0 >= s.L) s0 = 0;
                             if (tok + (h0 + h) * 16 + t0 + 1 >= s.L) s1 = 0;
+                        }
+                        if (MASKED) {        // a NaN reaches the columns that see its token: zero here, added to their sums below
+                            if ((s0 & 0x7Fu) == 0x7Fu) { nan |= 1u << t0; s0 = 0; }
+                            if ((s1 & 0x7Fu) == 0x7Fu) { nan |= 2u << t0; s1 = 0; }
                         }
                         vs2[x] = e4m3x2_to_half2(s0 | (s1 << 8));
                         if (D == 128) {
@@ -388,6 +387,20 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                         for (int u = 0; u < 4; u++)
 #pragma unroll
                             for (int nt = 0; nt < NT; nt++) mma16816(o[nt][4 * j + u], ev[0][u], od[0][u], ev[1][u], od[1][u], pb[nt][0], pb[nt][1]);
+                    }
+                    if (MASKED && __any_sync(0xFFFFFFFFu, nan)) {
+                        nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 1);
+                        nan |= __shfl_xor_sync(0xFFFFFFFFu, nan, 2);
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                            for (int x = 0; x < 2; x++) {
+                                const int sees = min(max(limit[nt][x] - tok - (h0 + h) * 16, 0), 16);
+                                if (nan & ((1u << sees) - 1u)) {
+#pragma unroll
+                                    for (int i = 0; i < MT; i++) o[nt][i][x] = o[nt][i][x + 2] = u2f(0x7FFFFFFFu);
+                                }
+                            }
                     }
                 }
             }

@@ -25,7 +25,8 @@ namespace qcc {
 // many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3;
-constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u;      // notes on a tile: the last of its part; both row tiles of its unit have rows
+constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u, PT_MASK = 1024u;      // notes on a tile: the last of its part; both row tiles of its
+                                                                                       // unit have rows; some row does not see all its tokens
 constexpr unsigned int PT_ERR = 9u;    // a barrier wait of this kernel ran out
 
 template <int D> struct PromptCfg {
@@ -59,6 +60,9 @@ __device__ __forceinline__ int prompt_tiles(int n, int L, int qt, int group)
     const int i = (int)min((int64_t)n - 1, ((int64_t)(qt + 1) * PT_ROWS - 1) / group);
     return (max(L - n + i + 1, 0) + PT_TOK - 1) / PT_TOK;
 }
+
+// the first of them that its first row does not see whole
+__device__ __forceinline__ int prompt_clear(int n, int L, int qt, int group) { return max(L - n + (int)((int64_t)qt * PT_ROWS / group) + 1, 0) / PT_TOK; }
 
 __device__ __forceinline__ int block_scan(int v, int32_t *wsum, int &all)     // inclusive; 1024 threads
 {
@@ -212,8 +216,23 @@ __device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.
 // byte of 16-byte chunk `ch` (0 .. D / 8 - 1) of row r in a swizzled tile of 128 rows
 __device__ __forceinline__ uint32_t tile_at(int r, int ch) { return (uint32_t)((ch >> 3) * 16384 + r * 128 + (((ch & 7) ^ (r & 7)) << 4)); }
 
+// blocks of 16 elements in which some value of tokens [from, to) is NaN
 template <int D>
-__global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs g, const PromptPlan plan)
+__device__ __noinline__ uint32_t nan_blocks(const AttnArgs &g, int b, int head, int from, int to)
+{
+    uint32_t bits = 0;
+    for (int t = from; t < to; t++) {
+        const int p = t / g.page, off = t - p * g.page;
+        const int64_t pg = __ldg(g.table + b * g.table_stride + p);
+        if (pg < 0 || pg >= g.num_pages) continue;
+        const uint8_t *sc = g.cache + ((pg * g.kv_heads + head) * 2 + 1) * ((int64_t)g.page * kv_row_bytes<D>()) + g.page * (D / 2) + off * (D / 16);
+        for (int i = 0; i < D / 16; i++) bits |= (uint32_t)((__ldg(sc + i) & 0x7Fu) == 0x7Fu) << i;
+    }
+    return bits;
+}
+
+template <int D>
+__global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_constant__ AttnArgs g, const PromptPlan plan)
 {
     using C = PromptCfg<D>;
     constexpr int RB = kv_row_bytes<D>();
@@ -223,7 +242,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
     const uint32_t s_q = sm, s_k = sm + 2 * C::TILE, s_v = sm + 4 * C::TILE, s_raw = sm + 6 * C::TILE, bars = s_raw + PT_RAW * C::RAW;
     const uint32_t raw_full = bars, raw_empty = bars + 24, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96, q_full = bars + 112,
                    s_full = bars + 128, p_full = bars + 144, o_done = bars + 160;
-    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_ml = bars + 256;      // notes of the last 8 tiles: tokens that exist, PT_LAST, PT_TWO
+    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_nan = bars + 216, s_ml = bars + 256;      // notes of the last 8 tiles: tokens that exist, PT_LAST, PT_TWO
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
@@ -261,6 +280,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
             mbar_init_at(q_full + 8 * i, 4); mbar_init_at(s_full + 8 * i, 1); mbar_init_at(p_full + 8 * i, 4); mbar_init_at(o_done + 8 * i, 1);
         }
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort), "r"(0u) : "memory");
+        sts_u32(s_nan, 0);
         fence_barrier_init();
     }
     if (warp == 2) tmem_alloc_at(slot, 512);
@@ -281,6 +301,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                 const int have = (s.L + g.page - 1) / g.page;
                 const int32_t *row = g.table + s.b * g.table_stride;
                 const uint32_t two = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? PT_TWO : 0;
+                const int clear = prompt_clear(s.n, s.L, s.qt, g.group);
                 for (int tile = s.first; tile < s.last; tile++, tiles++) {
                     const int p = tile * pages + lane;
                     int64_t pg = -1;
@@ -298,7 +319,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                         mbar_wait_at(raw_empty + 8 * (st), ph, PT_ERR, abort);
                         if (lane == 0) {
                             if (w == 0)
-                                sts_u32(s_info + 4 * (tiles & 7), (uint32_t)min(max(s.L - tile * PT_TOK, 0), PT_TOK) | (tile + 1 == s.last ? PT_LAST : 0) | two);
+                                sts_u32(s_info + 4 * (tiles & 7), (uint32_t)min(max(s.L - tile * PT_TOK, 0), PT_TOK) | (tile + 1 == s.last ? PT_LAST : 0) | (tile >= clear ? PT_MASK : 0) | two);
                             mbar_expect_at(raw_full + 8 * st, n * half);
                         }
                         __syncwarp();
@@ -419,7 +440,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     const uint32_t out_full = v ? v_full : k_full, out_empty = v ? v_empty : k_empty, out = v ? s_v : s_k;
                     mbar_wait_at(out_empty + 8 * (buf), ((tiles >> 1) & 1) ^ 1, PT_ERR, abort);
                     mbar_wait_at(raw_full + 8 * (st), ph, PT_ERR, abort);
-                    const int left = lds_volatile(s_info + 4 * (tiles & 7)) & 255;      // tokens of the tile that exist
+                    const uint32_t info = lds_volatile(s_info + 4 * (tiles & 7));
+                    const int left = info & 255;      // tokens of the tile that exist
                     const uint32_t src = s_raw + st * C::RAW, dst = out + buf * C::TILE;
                     constexpr int STEPS = 128 / (4 * PER);
                     uint4 c[STEPS];
@@ -431,6 +453,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                         c[i] = lds_v4(base + off * (D / 2) + ch * 16);
                         two[i] = lds_u16(base + (D / 2 << shift) + off * (D / 16) + ch * 2);
                         if (r >= left) two[i] = 0;          // whatever the slots behind the last token hold, it counts as zero
+                    }
+                    if (v && (info & PT_MASK)) {
+                        // a NaN reaches the rows that see its token: zero here, the end of the unit sets their sums
+#pragma unroll
+                        for (int i = 0; i < STEPS; i++) {
+                            const bool a = (two[i] & 0x7Fu) == 0x7Fu, b = (two[i] & 0x7F00u) == 0x7F00u;
+                            if (a || b) sts_u32(s_nan, 1);
+                            if (a) two[i] &= 0xFF00u;
+                            if (b) two[i] &= 0xFFu;
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < STEPS; i++) {
@@ -597,6 +629,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     m = up;
                     l = l * mine + l1 * others;
                 }
+                // 16-element blocks of the row that a NaN of a masked tile makes NaN (once this CTA has met one)
+                uint32_t nan = 0;
+                if (lds_volatile(s_nan)) nan = nan_blocks<D>(g, s.b, s.head, max(s.first, prompt_clear(s.n, s.L, s.qt, g.group)) * PT_TOK, min(limit, s.last * PT_TOK));
                 const float scale = l == 0.0f ? 0.0f : __fdividef(v_outer, l);
                 const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + h;
                 float *part = g.part + (size_t)(2 * blockIdx.x + (t == lo ? 0 : 1)) * prompt_part_floats<D>();
@@ -608,6 +643,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const AttnArgs
                     if (join) {
 #pragma unroll
                         for (int j = 0; j < 16; j++) o[j] = f2u(u2f(o[j]) * mine + u2f(lds_volatile(s_q + ((c + j) * 128 + row) * 4)) * others);
+                    }
+                    if (nan >> (c / 16) & 1u) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++) o[j] = 0x7FFFFFFFu;
                     }
                     if (whole) {
                         uint32_t y[8];

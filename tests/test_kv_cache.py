@@ -437,6 +437,57 @@ def test_nan_stays_with_its_query():
 
 
 @gpu
+@pytest.mark.parametrize("D,page,hq,heads", [(128, 16, 8, 2), (64, 64, 4, 4)])
+@pytest.mark.parametrize("lens,q_lens", [([200, 300], [2, 2]), ([200, 300], [4, 3]), ([90, 129], [8, 7]), ([200, 300], [33, 40]), ([257, 300], [257, 150])])
+def test_nan_in_the_cache_reaches_the_queries_that_see_it(D, page, hq, heads, lens, q_lens):
+    """One value block (its scale is NaN) and, in another call, one key of a late token: earlier queries do not see it."""
+    q, cache, _, table, ko, vo = attention_case(D, page, hq, heads, lens, q_lens, poison=False)
+    o, z, tol, ltol = attention_ref(q, cache, table, lens, q_lens, ko, vo, 1 / math.sqrt(D))
+    for b in range(2):
+        for back in {1, q_lens[b] // 2, q_lens[b]}:
+            t, head, block = lens[b] - max(back, 1), heads - 1, D // 16 - 2
+            first = sum(q_lens[:b]) + max(t - (lens[b] - q_lens[b]), 0)        # the first row that sees token t
+            rows, hs = slice(first, sum(q_lens[:b + 1])), slice(head * hq // heads, (head + 1) * hq // heads)
+            for w in (1, 0):
+                dirty = cache.clone()
+                planes(dirty, D)[1][table[b, t // page].long(), head, w, t % page, block] = 0xFF if b else 0x7F
+                out, lse = (x.cpu() for x in call(q, dirty, table, lens, q_lens, ko, vo))
+                hit = torch.zeros(out.shape, dtype=torch.bool)
+                hit[rows, hs, block * 16:block * 16 + 16 if w else D] = True
+                if w == 0:
+                    hit[rows, hs] = True
+                assert torch.equal(torch.isnan(out), hit), (b, back, w)
+                assert bool(((out.double() - o).abs() <= tol)[~hit].all())
+                assert torch.equal(torch.isnan(lse), hit[..., 0] if w == 0 else torch.zeros_like(lse, dtype=torch.bool))
+                assert bool(((lse.double() - z).abs() <= ltol)[~torch.isnan(lse)].all())
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("lens,q_lens", [([5000] * 40, [1] * 40), ([5000] * 40, [2] * 40), ([5000] * 40, [3] * 40), ([700, 3000, 90], [300, 70, 90])])
+def test_workspace_is_what_it_says(D, lens, q_lens):
+    """Partial sums of every CTA stay within the bytes that the size query returns: what lies behind them is untouched."""
+    import ctypes
+    lib = L.load()
+    hq, heads, page = 16, 2, 64
+    q, cache, _, table, ko, vo = attention_case(D, page, hq, heads, lens, q_lens, poison=False)
+    want = call(q, cache, table, lens, q_lens, ko, vo)
+    q, cache, table, ko, vo = (x.cuda() for x in (q, cache, table, ko, vo))
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    cu = torch.tensor([0] + q_lens).cumsum(0).to(torch.int32).cuda()
+    out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+    size = lib.qcc_nvfp4_kv_attention_workspace_bytes(q.shape[0], len(lens), max(q_lens), hq, heads, D)
+    ws = torch.full((size + (1 << 22),), 0xA5, dtype=torch.uint8, device="cuda")
+    p = lambda t: t.data_ptr()
+    a = L.KvAttentionArgs(p(q), (ctypes.c_int64 * 2)(*q.stride()[:2]), q.shape[0], p(cache), cache.shape[0], p(table), table.stride(0), table.shape[1], p(n), p(cu),
+                          len(lens), max(q_lens), p(ko), p(vo), 1 / math.sqrt(D), hq, heads, D, page, p(out), p(lse))
+    assert lib.qcc_nvfp4_kv_attention(ctypes.byref(a), p(ws), size - 1, torch.cuda.current_stream().cuda_stream) == -4
+    assert lib.qcc_nvfp4_kv_attention(ctypes.byref(a), p(ws), size, torch.cuda.current_stream().cuda_stream) == 0
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    assert bool((ws[size:] == 0xA5).all()) and bool((ws[:size] != 0xA5).any())
+
+
+@gpu
 def test_strided_queries_and_table():
     lens = [100, 333]
     q, cache, _, table, ko, vo = attention_case(128, 16, 8, 2, lens, [1, 1])
