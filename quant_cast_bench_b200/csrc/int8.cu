@@ -102,7 +102,7 @@ constexpr unsigned int MM_ERR = 7;   // a barrier wait of the product ran out
 
 template <int BN> struct MmCfg {
     static constexpr int STAGE = (MM_BM + BN) * MM_BK;
-    static constexpr int STAGES = BN == 256 ? 4 : BN == 128 ? 6 : 8;
+    static constexpr int STAGES = BN >= 224 ? 4 : BN >= 160 ? 5 : BN >= 96 ? 6 : 8;
     static constexpr int RED = MM_BM * BN * 4;                              // sums of one CTA (split form), in the stages' memory
     static constexpr int BODY = STAGE * STAGES > RED ? STAGE * STAGES : RED;
     static constexpr int PARTS = BN >= 64 ? 2 : 1;                          // epilogue warps per 32 channels, each with a share of the tokens
@@ -173,7 +173,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
     const uint32_t full = s_sa + 2 * BN * 4, empty = full + 8 * C::STAGES, acc_full = empty + 8 * C::STAGES, acc_empty = acc_full + 16, slot = acc_empty + 16,
                    abort = slot + 4;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    constexpr uint32_t ACC_COLS = BN < 32 ? 32 : BN, TMEM_COLS = SPLIT ? ACC_COLS : 2 * ACC_COLS;
+    constexpr uint32_t ACC_COLS = BN <= 32 ? 32 : BN <= 64 ? 64 : BN <= 128 ? 128 : 256, TMEM_COLS = SPLIT ? ACC_COLS : 2 * ACC_COLS;
 
     if (threadIdx.x == 0) {
         asm volatile("prefetch.tensormap [%0];" ::"l"(&map_w) : "memory");
@@ -372,12 +372,13 @@ static int mm_launch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArgs 
     cfg.numAttrs = SPLIT ? 2 : 1;
     return (int)cudaLaunchKernelEx(&cfg, int8_mm_kernel<BN, SPLIT, OUT>, mw, mx, g);
 }
-template <int BN>
+template <int BN, bool CAN_SPLIT = true>
 static int mm_dispatch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArgs &g, int out, cudaStream_t st)
 {
-    if (g.splits > 1)
-        return out == QCC_OUT_BF16 ? mm_launch<BN, true, QCC_OUT_BF16>(mw, mx, g, st)
-               : out == QCC_OUT_F16 ? mm_launch<BN, true, QCC_OUT_F16>(mw, mx, g, st) : mm_launch<BN, true, QCC_OUT_F32>(mw, mx, g, st);
+    if constexpr (CAN_SPLIT)
+        if (g.splits > 1)
+            return out == QCC_OUT_BF16 ? mm_launch<BN, true, QCC_OUT_BF16>(mw, mx, g, st)
+                   : out == QCC_OUT_F16 ? mm_launch<BN, true, QCC_OUT_F16>(mw, mx, g, st) : mm_launch<BN, true, QCC_OUT_F32>(mw, mx, g, st);
     return out == QCC_OUT_BF16 ? mm_launch<BN, false, QCC_OUT_BF16>(mw, mx, g, st)
            : out == QCC_OUT_F16 ? mm_launch<BN, false, QCC_OUT_F16>(mw, mx, g, st) : mm_launch<BN, false, QCC_OUT_F32>(mw, mx, g, st);
 }
@@ -391,12 +392,12 @@ static void mm_choose(int64_t M, int64_t N, int kblocks, int &bn, int &splits)
     const int sms = sm_count();
     double best = 0;
     bn = 0;
-    for (int b = 16; b <= 256; b *= 2) {
-        if (b > 16 && b / 2 >= M) break;
+    for (int b = 16, last = 0; b <= 256; last = b, b += b < 32 ? 16 : 32) {
+        if (last >= M) break;
         const int64_t tiles = (N + MM_BM - 1) / MM_BM * ((M + b - 1) / b);
         const double block = b * 2 > 128 ? (b * 2 > (128 + b) * 2 ? b * 2 : (128 + b) * 2) : (128 + b) * 2;
         for (int s = 1; s <= 8; s *= 2) {
-            if (s > 1 && (kblocks < 2 * s || tiles * s > sms)) break;
+            if (s > 1 && ((b & (b - 1)) || kblocks < 2 * s || tiles * s > sms)) break;
             const int64_t waves = (tiles * s + sms - 1) / sms;
             const double t = waves * ((kblocks + s - 1) / s) * block + 2500 + (waves - 1) * (b * 6.0) + (s > 1 ? 1500 : 0);
             if (bn == 0 || t < best) {
@@ -467,7 +468,11 @@ extern "C" int qcc_int8_scaled_mm(const void *a, const void *b, int64_t M, int64
     case 16: return mm_dispatch<16>(mw, mx, g, out_dtype, st);
     case 32: return mm_dispatch<32>(mw, mx, g, out_dtype, st);
     case 64: return mm_dispatch<64>(mw, mx, g, out_dtype, st);
+    case 96: return mm_dispatch<96, false>(mw, mx, g, out_dtype, st);
     case 128: return mm_dispatch<128>(mw, mx, g, out_dtype, st);
+    case 160: return mm_dispatch<160, false>(mw, mx, g, out_dtype, st);
+    case 192: return mm_dispatch<192, false>(mw, mx, g, out_dtype, st);
+    case 224: return mm_dispatch<224, false>(mw, mx, g, out_dtype, st);
     default: return mm_dispatch<256>(mw, mx, g, out_dtype, st);
     }
 }
