@@ -94,7 +94,8 @@ int qcc_version(void);
  * not ascending multiples of 32 inside M (code 16; the scale buffers then hold zeros only), or a
  * transform matrix that is not diag(+-1) @ H16 / 4 was passed to one of the qcc_*rht* calls (code 17;
  * the outputs then follow the signs of its first column), or a cast tile of qcc_fp8_colwise gave up waiting for the
- * column maxima of its panel (code 18).  Synchronises the device. */
+ * column maxima of its panel (code 18), or a wait for another rank's amax ran out (code 19), or the paged key/value cache was given
+ * page, slot, length, position or query numbers outside their ranges (codes 20 to 22, see there).  Synchronises the device. */
 int qcc_device_error(unsigned int *out);
 
 /* Number of SMs of the current device (cached per device). */
@@ -508,12 +509,13 @@ int qcc_nvfp4_kv_gather(const void *cache, int64_t num_pages, int kv_heads, int 
 
 /* Attention over the cache.  q (rows, q_heads, head_dim) bf16, already rotated; kv_lens[b] (device int32): tokens that the cache
  * holds of sequence b.  Without cu_q every sequence has one query (rows == seqs); with it rows cu_q[b] .. cu_q[b+1] - 1 are the
- * queries of sequence b, its LAST tokens: query i of n sees the keys j <= kv_lens[b] - n + i.  max_q: at least the most
+ * queries of sequence b (ascending from 0), its LAST tokens: query i of n sees the keys j <= kv_lens[b] - n + i.  max_q: at least the most
  * queries of a sequence.  q head h reads kv head h / (q_heads / kv_heads).
  *   out (rows, q_heads, head_dim) bf16 = sum_j softmax_j(scale * q . k_j) v_j;  lse (rows, q_heads) fp32, may be NULL, =
  *   log sum_j exp(scale * q . k_j).  A query that sees no key, and every row behind the last sequence: out = 0, lse = -inf.
  * Sums, maxima and the softmax in fp32; the probabilities are rounded to fp16 before they multiply the values.
- * The result does not depend on what the slots behind a sequence's last token hold.  Two runs on the same inputs give the
+ * The result does not depend on what the slots behind a sequence's last token hold, that of a query not on the tokens behind it,
+ * NaN among them.  Two runs on the same inputs give the
  * same bits.  A sequence whose query offsets descend, leave the rows of q or hold more than max_q rows sets code 22 in the word
  * qcc_device_error reads, and its rows are not written; one that reaches a bad page (code 20) gets a result without meaning.
  * workspace: scratch of qcc_nvfp4_kv_attention_workspace_bytes, 16-byte aligned, any contents; calls that may overlap on the
@@ -530,7 +532,7 @@ typedef struct qcc_kv_attention_args {
     const int32_t *kv_lens, *cu_q;
     int seqs, max_q;
     const float *k_outer, *v_outer;
-    float scale;
+    float scale;                 /* > 0                                                            */
     int q_heads, kv_heads, head_dim, page;
     void *out;
     float *lse;

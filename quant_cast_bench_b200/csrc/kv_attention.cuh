@@ -80,8 +80,9 @@ __device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n
 {
     if (g.cu_q) {
         q0 = __ldg(g.cu_q + b);
-        n = __ldg(g.cu_q + b + 1) - q0;
-        if (q0 < 0 || n < 0 || n > g.max_q || (int64_t)q0 + n > g.rows) {
+        const int64_t end = __ldg(g.cu_q + b + 1), count = end - q0;      // (64 bits: the offsets may be anything)
+        n = (int)count;
+        if (q0 < 0 || count < 0 || count > g.max_q || end > g.rows) {
             atomicMax(&g_qcc_error, QCC_DEVERR_QUERIES);
             q0 = 0;
             n = 0;

@@ -125,7 +125,7 @@ def nvfp4_kv_gather_cuda(cache, block_table, cu_kv, total, head_dim, k_outer, v_
 def nvfp4_kv_attention_cuda(q, cache, block_table, kv_lens, k_outer, v_outer, cu_q=None, max_q=None, scale=None):
     """Attention of q (rows, q_heads, head_dim) bf16, already rotated, over the cache: (out like q, lse (rows, q_heads) fp32).
     block_table (seqs, pages) int32, kv_lens (seqs) int32: the tokens that the cache holds of each sequence.  Without cu_q each sequence has one query;
-    with cu_q (seqs + 1) int32, rows cu_q[b] .. cu_q[b + 1] - 1 are the last tokens of sequence b and attend causally; max_q (a Python int) is at
+    with cu_q (seqs + 1) int32, ascending from 0, rows cu_q[b] .. cu_q[b + 1] - 1 are the last tokens of sequence b and attend causally; max_q (a Python int) is at
     least the most queries of a sequence.  scale defaults to 1 / sqrt(head_dim).  q_heads must be a multiple of kv_heads.
     A query without keys, and a row behind the last sequence, gets zeros and lse -inf."""
     lib = L.load()
@@ -152,12 +152,12 @@ def nvfp4_kv_attention_cuda(q, cache, block_table, kv_lens, k_outer, v_outer, cu
     lse = torch.empty((rows, hq), dtype=torch.float32, device=q.device)
     if rows == 0 or seqs == 0:
         return out.zero_(), lse.fill_(-math.inf)
-    nws = lib.qcc_nvfp4_kv_attention_workspace_bytes(rows, seqs, max_q, hq, heads, D)
-    ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
     a = L.KvAttentionArgs(_p(q), (ctypes.c_int64 * 2)(*q.stride()[:2]), rows, _p(cache), cache.shape[0], _p(block_table), block_table.stride(0),
                           block_table.shape[1], _p(kv_lens), _p(cu_q), seqs, max_q, _p(k_outer), _p(v_outer),
                           1.0 / math.sqrt(D) if scale is None else scale, hq, heads, D, page, _p(out), _p(lse))
     with _on_device(q.device):
+        nws = lib.qcc_nvfp4_kv_attention_workspace_bytes(rows, seqs, max_q, hq, heads, D)
+        ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         L.check(lib.qcc_nvfp4_kv_attention(ctypes.byref(a), _p(ws), nws, _stream(q)), "nvfp4_kv_attention")
-    L.launch_count += 2
+    L.launch_count += 2 if max_q * (hq // heads) <= 32 else 3
     return out, lse

@@ -140,6 +140,14 @@ def test_c_refusals():
     assert attention(seqs=0, rows=0, q=None) == 0 and lib.qcc_nvfp4_kv_attention(None, p, 1, None) == -3
 
 
+def test_c_refuses_a_scale_that_is_not_positive():
+    import ctypes
+    lib, p = L.load(), 1 << 20
+    for scale in (0.0, -0.125, float("nan")):
+        a = L.KvAttentionArgs(p, (ctypes.c_int64 * 2)(512, 64), 4, p, 4, p, 4, 4, p, None, 4, 1, p, p, scale, 4, 2, 64, 16, p, p)
+        assert lib.qcc_nvfp4_kv_attention(ctypes.byref(a), p, 1 << 40, None) == -3
+
+
 def test_native_shapes_without_a_gpu():
     from quant_cast_bench_b200 import build as qbuild
     qbuild.build_torch_binding()
@@ -542,6 +550,56 @@ def test_graph_follows_lengths_and_table_on_the_device():
 
 
 @gpu
+def test_graph_follows_query_offsets_on_the_device():
+    """A captured call for up to 300 rows of new tokens, replayed as they belong to other sequences; two share the pool of one graph."""
+    D, page, hq, heads = 64, 32, 12, 4
+    g = torch.Generator().manual_seed(9)
+    q, cache, _, table, ko, vo = attention_case(D, page, hq, heads, [500, 140, 300], [300, 0, 0], poison=False)
+    lens, cu = torch.tensor([500, 140, 300], dtype=torch.int32).cuda(), torch.tensor([0, 300, 300, 300], dtype=torch.int32).cuda()
+    dev = [t.cuda() for t in (q, cache, table)] + [lens, ko.cuda(), vo.cuda()]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = Q.nvfp4_kv_attention_cuda(*dev, cu_q=cu, max_q=300)
+        again = Q.nvfp4_kv_attention_cuda(*dev, cu_q=cu, max_q=300)
+    for n, offsets in (([500, 140, 300], [0, 300, 300, 300]), ([500, 140, 300], [0, 0, 140, 300]), ([0, 0, 0], [0, 0, 0, 0]), ([90, 0, 7], [0, 100, 130, 137]), ([1, 140, 300], [0, 1, 2, 300])):
+        lens.copy_(torch.tensor(n, dtype=torch.int32))
+        cu.copy_(torch.tensor(offsets, dtype=torch.int32))
+        dev[0].copy_(torch.randn(300, hq, D, generator=g).to(torch.bfloat16))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = Q.nvfp4_kv_attention_cuda(*dev, cu_q=cu, max_q=300)
+        for a, b in zip(first + again, want + want):
+            assert torch.equal(a, b), offsets
+        o, z, tol, ltol = attention_ref(dev[0].cpu()[:offsets[-1]], cache, table, n, [b - a for a, b in zip(offsets, offsets[1:])], ko, vo, 1 / math.sqrt(D))
+        assert bool(((want[0][:offsets[-1]].cpu().double() - o).abs() <= tol).all())
+        assert bool((want[0][offsets[-1]:] == 0).all()) and bool((want[1][offsets[-1]:] == -math.inf).all())
+
+
+@gpu
+def test_many_queries_with_bad_numbers():
+    """The form for many queries: a bad page, offsets and lengths outside their ranges are reported, and the other sequence is right."""
+    D, page, hq, heads, lens, ql = 64, 16, 4, 2, [100, 130], [60, 70]
+    q, cache, _, table, ko, vo = attention_case(D, page, hq, heads, lens, ql, poison=False)
+    L.device_error()
+    want = call(q, cache, table, lens, ql, ko, vo)
+    assert L.device_error() == 0
+    for n in (cache.shape[0], -1, 1 << 30):
+        bad = table.clone()
+        bad[0, 3] = n
+        out, lse = call(q, cache, bad, lens, ql, ko, vo)
+        assert L.device_error() == 20
+        assert torch.equal(out[60:], want[0][60:]) and torch.equal(lse[60:], want[1][60:])
+    call(q, cache, table, [100, 16 * table.shape[1] + 1], ql, ko, vo)
+    assert L.device_error() == 20
+    args = (q.cuda(), cache.cuda(), table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), ko.cuda(), vo.cuda())
+    for cu, mq in (([0, 60, 131], 70), ([0, 60, 50], 70), ([-1, 60, 130], 70), ([0, 60, 130], 69), ([0, 2 ** 31 - 1, -2 ** 31], 70)):
+        Q.nvfp4_kv_attention_cuda(*args, cu_q=torch.tensor(cu, dtype=torch.int32).cuda(), max_q=mq)
+        assert L.device_error() == 22, cu
+    out, lse = call(q, cache, table, lens, ql, ko, vo)
+    assert L.device_error() == 0 and torch.equal(out, want[0]) and torch.equal(lse, want[1])
+
+
+@gpu
 def test_rows_behind_the_last_sequence():
     lens, q_lens = [100, 30], [3, 2]
     q, cache, _, table, ko, vo = attention_case(64, 16, 4, 2, lens, q_lens)
@@ -596,6 +654,9 @@ def test_cache_beyond_4_gib():
     cu = torch.tensor([0, 40], dtype=torch.int32).cuda()
     for a, b in zip(Q.nvfp4_kv_gather_cuda(cache, table.cuda(), cu, 40, D, o.cuda(), o.cuda()), Q.nvfp4_kv_gather_cuda(small, t.cuda(), cu, 40, D, o.cuda(), o.cuda())):
         assert torch.equal(a, b) and bool((a != 0).any())
+    chunk = torch.randn(20, 32, D, generator=g).to(torch.bfloat16)
+    for a, b in zip(call(chunk, cache, table, [40], [20], o, o), call(chunk, small, t, [40], [20], o, o)):
+        assert torch.equal(a, b)
     ref = attention_ref(q, small.cpu(), t, [40], [1], o, o, 1 / math.sqrt(D))
     assert bool(((got[0].cpu().double() - ref[0]).abs() <= ref[2]).all())
 
