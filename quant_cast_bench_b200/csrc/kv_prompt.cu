@@ -24,7 +24,7 @@ namespace qcc {
 // row tiles.  All (unit, tile) pairs are numbered, by a first small kernel, and dealt out evenly to one CTA per SM, whatever the lengths and however
 // many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
 // -------------------------------------------------------------------------------------------------------------------
-constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3;
+constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3, PT_NOTES = 8;
 constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u, PT_MASK = 1024u;      // notes on a tile: the last of its part; both row tiles of its
                                                                                        // unit have rows; some row does not see all its tokens
 constexpr unsigned int PT_ERR = 9u;    // a barrier wait of this kernel ran out
@@ -33,7 +33,7 @@ template <int D> struct PromptCfg {
     static constexpr int BLOCKS = D / 64;                       // 64-element blocks of a row: 128 bytes of fp16
     static constexpr int TILE = BLOCKS * 128 * 128;             // 128 rows of Q, K or V as fp16
     static constexpr int RAW = PT_TOK * kv_row_bytes<D>();      // codes and scales of 128 tokens, keys or values
-    static constexpr int SMEM = 1024 + 6 * TILE + PT_RAW * RAW + 256 + 128 * 8;
+    static constexpr int SMEM = 1024 + 6 * TILE + PT_RAW * RAW + 256 + 128 * 8 + PT_NOTES * (8 + 8 + 48);
 };
 
 // ---- numbering: prefix[p] = tiles of all (sequence, row tile) pairs before p, times the kv heads; pairs[p] = (sequence, row tile)
@@ -182,12 +182,6 @@ __device__ __forceinline__ void next_part(const AttnArgs &g, const PromptPlan &p
     s.first = 0;
     s.last = min(s.tiles, hi - t);
 }
-// for (Part s ...) over the parts of [lo, hi)
-#define QCC_FOR_PARTS(s, t)                                             \
-    Part s;                                                             \
-    int t = lo;                                                         \
-    for (find_part(g, plan, pairs, t, hi, s); t < hi; t += s.last - s.first, t < hi ? next_part(g, plan, t, hi, s) : (void)0)
-
 template <int D> __host__ __device__ constexpr int prompt_part_floats() { return PT_ROWS * (D + 2); }
 
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16])
@@ -242,7 +236,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
     const uint32_t s_q = sm, s_k = sm + 2 * C::TILE, s_v = sm + 4 * C::TILE, s_raw = sm + 6 * C::TILE, bars = s_raw + PT_RAW * C::RAW;
     const uint32_t raw_full = bars, raw_empty = bars + 24, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96, q_full = bars + 112,
                    s_full = bars + 128, p_full = bars + 144, o_done = bars + 160;
-    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_nan = bars + 216, s_ml = bars + 256;      // notes of the last 8 tiles: tokens that exist, PT_LAST, PT_TWO
+    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_nan = bars + 216, s_ml = bars + 256,      // s_info: notes of the last 8 tiles, tokens that exist, PT_LAST, PT_TWO
+                   part_full = s_ml + 128 * 8, part_empty = part_full + 8 * PT_NOTES, s_part = part_empty + 8 * PT_NOTES;      // notes on parts
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
     pdl_trigger();
@@ -279,6 +274,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             mbar_init_at(v_full + 8 * i, 4); mbar_init_at(v_empty + 8 * i, 1);
             mbar_init_at(q_full + 8 * i, 4); mbar_init_at(s_full + 8 * i, 1); mbar_init_at(p_full + 8 * i, 4); mbar_init_at(o_done + 8 * i, 1);
         }
+        for (int i = 0; i < PT_NOTES; i++) { mbar_init_at(part_full + 8 * i, 1); mbar_init_at(part_empty + 8 * i, 8); }
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort), "r"(0u) : "memory");
         sts_u32(s_nan, 0);
         fence_barrier_init();
@@ -296,8 +292,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             uint32_t st = 0, ph = 1, tiles = 0;
             const int pages = PT_TOK / g.page;
             const uint32_t half = (uint32_t)(g.page * RB);
-            QCC_FOR_PARTS(s, t) {
-                if (t == lo && lane == 0) note_seam(g, s.first ? s.unit_first : -1, s.unit_first + s.tiles, total, (int)((int64_t)s.n * g.group), s.q0, s.head, s.qt * PT_ROWS);
+            Part s;
+            find_part(g, plan, pairs, lo, hi, s);
+            for (uint32_t t = lo, k = 0; (int)t < hi; k++) {
+                mbar_wait_at(part_empty + 8 * (k & (PT_NOTES - 1)), (k / PT_NOTES & 1) ^ 1, PT_ERR, abort);
+                if (__any_sync(0xFFFFFFFFu, lds_volatile(abort))) break;      // (the notes that are being read stay)
+                if (lane == 0) {
+                    const uint32_t at = s_part + (k & (PT_NOTES - 1)) * 48;
+                    sts_v4(at, make_uint4(s.b, s.q0, s.n, s.L));
+                    sts_v4(at + 16, make_uint4(s.qt, s.head, s.tiles, s.first));
+                    sts_u32(at + 32, s.last);
+                    mbar_arrive_at(part_full + 8 * (k & (PT_NOTES - 1)));
+                }
+                if (k == 0 && lane == 0) note_seam(g, s.first ? s.unit_first : -1, s.unit_first + s.tiles, total, (int)((int64_t)s.n * g.group), s.q0, s.head, s.qt * PT_ROWS);
                 const int have = (s.L + g.page - 1) / g.page;
                 const int32_t *row = g.table + s.b * g.table_stride;
                 const uint32_t two = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? PT_TWO : 0;
@@ -327,6 +334,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                         if (++st == PT_RAW) { st = 0; ph ^= 1; }
                     }
                 }
+                t += s.last - s.first;
+                if ((int)t < hi) next_part(g, plan, t, hi, s);
             }
         } else if (warp == 1 && elect_one()) {
             // ---- matrix instructions
@@ -495,39 +504,88 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
         const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
         uint32_t sn = 0, on = 0;        // scores, products so far
-        QCC_FOR_PARTS(s, t) {
-            // both row tiles have rows: one for each softmax; one has: both softmaxes take it, and the tiles of tokens in turn
-            const bool two = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128;
-            const int64_t rows = (int64_t)s.n * g.group, r = (int64_t)s.qt * PT_ROWS + (two ? x * 128 : 0) + row;
-            const int first = two ? s.first : s.first + x, step = two ? 1 : 2;
-            const bool live = r < rows, idle = first >= s.last;
-            const int i = live ? (int)(r / g.group) : 0, h = s.head * g.group + (live ? (int)(r - (int64_t)i * g.group) : 0);
-            const int limit = live ? s.L - s.n + i + 1 : 0;
-            float factor = 0.0f;
+        float factor = 0.0f;
+        bool placed = false;            // q of the part is in place already
+        // part k, which starts at tile t, from its note (after a wait has run out: by search)
+        const auto read_note = [&](uint32_t k, int t) {
+            Part s;
+            if (lds_volatile(abort)) {
+                find_part(g, plan, pairs, t, hi, s);
+                return s;
+            }
+            const uint32_t note = s_part + (k & (PT_NOTES - 1)) * 48;
+            const uint4 a = lds_v4(note), b = lds_v4(note + 16);
+            s.b = a.x; s.q0 = a.y; s.n = a.z; s.L = a.w;
+            s.qt = b.x; s.head = b.y; s.tiles = b.z; s.first = b.w;
+            s.last = lds_volatile(note + 32);
+            return s;
+        };
+        const auto read_part = [&](uint32_t k, int t) {
+            mbar_wait_at(part_full + 8 * (k & (PT_NOTES - 1)), k / PT_NOTES & 1, PT_ERR, abort);
+            return read_note(k, t);
+        };
+        // This thread's row of a part.  Both row tiles have rows: one for each softmax; one has: both softmaxes take it, and the
+        // tiles of tokens in turn.
+        struct Rows {
+            bool two, live;
+            int first, i, h, limit;      // first tile; query, head, keys that the row sees
+        };
+        const auto rows_of = [&](const Part &s) {
+            Rows a;
+            const int64_t rows = (int64_t)s.n * g.group, r0 = (int64_t)s.qt * PT_ROWS;
+            a.two = rows - r0 > 128;
+            const int64_t r = r0 + (a.two ? x * 128 : 0) + row;
+            a.first = a.two ? s.first : s.first + x;
+            a.live = r < rows;
+            a.i = a.live ? (int)r / g.group : 0;
+            a.h = s.head * g.group + (a.live ? (int)r - a.i * g.group : 0);
+            a.limit = a.live ? s.L - s.n + a.i + 1 : 0;
+            return a;
+        };
+        // q of this thread's row, into shared memory; its factor score -> log2 units
+        const auto place_q = [&](const Part &s, const Rows &at) {
+            uint4 w[D / 8];
+            uint32_t acc = 0;
+            const uint16_t *src = g.q + (int64_t)(s.q0 + at.i) * g.q_token + at.h * g.q_head;
+#pragma unroll
+            for (int j = 0; j < D / 8; j++) {
+                w[j] = at.live ? ld_v4(src + 8 * j) : make_uint4(0, 0, 0, 0);
+                acc = absmax2_acc(absmax2_acc(absmax2_acc(absmax2_acc(acc, w[j].x), w[j].y), w[j].z), w[j].w);
+            }
+            float mult, back;
+            q_power(f2u(hmax_halves_f32(acc)), mult, back);
+            const uint32_t dst = s_q + x * C::TILE;
+#pragma unroll
+            for (int j = 0; j < D / 8; j++)
+                sts_v4(dst + tile_at(row, j),
+                       make_uint4(pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult), pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult),
+                                  pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult), pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult)));
+            proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(q_full + 8 * x);
+            const float f = back * (g.scale_log2 * k_outer);
+            return f < 1e-37f ? 1e-37f : f;       // not zero: -inf of a hidden key has to stay
+        };
+        for (int t = lo, k = 0; t < hi; k++) {
+            const int t_part = t;
+            int tile, last, step, limit;
+            {
+                const Part s = read_part(k, t);
+                const Rows at = rows_of(s);
+                tile = at.first;
+                last = s.last;
+                step = at.two ? 1 : 2;
+                limit = at.limit;
+                if (tile < last && !placed) factor = place_q(s, at);
+                t += s.last - s.first;
+            }
+            const bool idle = tile >= last;
+            const float scale_in = factor;
             if (!idle) {
-                uint4 w[D / 8];
-                uint32_t acc = 0;
-                const uint16_t *src = g.q + (int64_t)(s.q0 + i) * g.q_token + h * g.q_head;
-#pragma unroll
-                for (int j = 0; j < D / 8; j++) {
-                    w[j] = live ? ld_v4(src + 8 * j) : make_uint4(0, 0, 0, 0);
-                    acc = absmax2_acc(absmax2_acc(absmax2_acc(absmax2_acc(acc, w[j].x), w[j].y), w[j].z), w[j].w);
-                }
-                float mult, back;
-                q_power(f2u(hmax_halves_f32(acc)), mult, back);
-                factor = back * (g.scale_log2 * k_outer);
-                factor = factor < 1e-37f ? 1e-37f : factor;       // not zero: -inf of a hidden key has to stay
-                const uint32_t dst = s_q + x * C::TILE;
-#pragma unroll
-                for (int j = 0; j < D / 8; j++)
-                    sts_v4(dst + tile_at(row, j),
-                           make_uint4(pack_half2(bf16lo(w[j].x) * mult, bf16hi(w[j].x) * mult), pack_half2(bf16lo(w[j].y) * mult, bf16hi(w[j].y) * mult),
-                                      pack_half2(bf16lo(w[j].z) * mult, bf16hi(w[j].z) * mult), pack_half2(bf16lo(w[j].w) * mult, bf16hi(w[j].w) * mult)));
-                proxy_fence();
-                __syncwarp();
-                if (lane == 0) mbar_arrive_at(q_full + 8 * x);
+                placed = false;
+                bool any = false;               // O holds products of this part
                 float m = -INFINITY, l = 0.0f;
-                for (int tile = first; tile < s.last; tile += step) {
+                for (; tile < last; tile += step) {
                     mbar_wait_at(s_full + 8 * (x), sn++ & 1, PT_ERR, abort);
                     tc_fence_after();
                     uint32_t v[4][32];
@@ -549,13 +607,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     for (int j = 2; j < 32; j += 2)
 #pragma unroll
                         for (int c = 0; c < 4; c++) top[c] = max3(top[c], u2f(v[c][j]), u2f(v[c][j + 1]));
-                    const float most = fmaxf(max3(top[0], top[1], top[2]), top[3]) * factor;
+                    const float most = fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale_in;
                     const bool grow = most - m > 8.0f;           // (from -inf: always, once the row sees a key)
                     if (__any_sync(0xFFFFFFFFu, grow)) {
                         const float up = grow ? most : m, a = grow ? ex2(m - up) : 1.0f;
                         m = up;
                         l *= a;
-                        if (tile > first) {
+                        if (any) {
                             mbar_wait_at(o_done + 8 * x, (on - 1) & 1, PT_ERR, abort);
                             tc_fence_after();
 #pragma unroll
@@ -570,14 +628,14 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                         }
                     }
                     const float base = m == -INFINITY ? 0.0f : m;
-                    const uint64_t factor2 = pack2(factor, factor), base2 = pack2(-base, -base);
+                    const uint64_t factor2 = pack2(scale_in, scale_in), base2 = pack2(-base, -base);
                     uint64_t sum[2] = {0, 0};
 #pragma unroll
                     for (int c = 0; c < 4; c++) {
                         uint32_t p[16];
 #pragma unroll
                         for (int j = 0; j < 16; j++) {
-                            // (factor is finite and positive: -inf stays -inf and exp2 gives 0)
+                            // (scale_in is finite and positive: -inf stays -inf and exp2 gives 0)
                             float e0, e1;
                             unpack2(fma2(pack2(u2f(v[c][2 * j]), u2f(v[c][2 * j + 1])), factor2, base2), e0, e1);
                             e0 = ex2(e0);
@@ -597,10 +655,25 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     __syncwarp();
                     if (lane == 0) mbar_arrive_at(p_full + 8 * x);
                     on++;
+                    any = true;
+                }
+                const Part s = read_note(k, t_part);      // (again: it would take up registers that the loop needs)
+                const Rows at = rows_of(s);
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(part_empty + 8 * (k & (PT_NOTES - 1)));
+                const bool whole = s.first == 0 && s.last == s.tiles, join = !at.two && s.last - s.first > 1;
+                if (!join && t < hi) {
+                    // q of the next part, whose first scores are then worked out behind the end of this one (one that joins needs the
+                    // space of q)
+                    const Part n = read_part(k + 1, t);
+                    const Rows to = rows_of(n);
+                    if (to.first < n.last) {
+                        factor = place_q(n, to);
+                        placed = true;
+                    }
                 }
                 mbar_wait_at(o_done + 8 * (x), (on - 1) & 1, PT_ERR, abort);
                 tc_fence_after();
-                const bool whole = s.first == 0 && s.last == s.tiles, join = !two && s.last - s.first > 1;
                 float mine = 1.0f, others = 0.0f;         // weights of this softmax's sums and of the other's
                 if (join) {
                     // the second softmax hands its sums over in Q's place, column by column
@@ -633,8 +706,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                 uint32_t nan = 0;
                 if (lds_volatile(s_nan)) nan = nan_blocks<D>(g, s.b, s.head, max(s.first, prompt_clear(s.n, s.L, s.qt, g.group)) * PT_TOK, min(limit, s.last * PT_TOK));
                 const float scale = l == 0.0f ? 0.0f : __fdividef(v_outer, l);
-                const int64_t at = (int64_t)(s.q0 + i) * g.q_heads + h;
-                float *part = g.part + (size_t)(2 * blockIdx.x + (t == lo ? 0 : 1)) * prompt_part_floats<D>();
+                const int64_t to = (int64_t)(s.q0 + at.i) * g.q_heads + at.h;
+                float *part = g.part + (size_t)(2 * blockIdx.x + (k ? 1 : 0)) * prompt_part_floats<D>();
 #pragma unroll
                 for (int c = 0; c < D; c += 16) {
                     uint32_t o[16];
@@ -655,8 +728,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                             const __nv_bfloat162 b = __floats2bfloat162_rn(l == 0.0f ? 0.0f : u2f(o[2 * j]) * scale, l == 0.0f ? 0.0f : u2f(o[2 * j + 1]) * scale);
                             y[j] = *reinterpret_cast<const uint32_t *>(&b);
                         }
-                        if (live) {
-                            uint4 *dst = reinterpret_cast<uint4 *>(g.out + at * D + c);
+                        if (at.live) {
+                            uint4 *dst = reinterpret_cast<uint4 *>(g.out + to * D + c);
                             dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
                             dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
                         }
@@ -667,9 +740,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     }
                 }
                 if (!whole) reinterpret_cast<float2 *>(part + PT_ROWS * D)[x * 128 + row] = make_float2(m, l);
-                else if (live && g.lse) g.lse[at] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
+                else if (at.live && g.lse) g.lse[to] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
                 tc_fence_before();       // the next unit's products write O
                 if (join) named_barrier(1, 256);
+            } else {
+                __syncwarp();
+                if (lane == 0) mbar_arrive_at(part_empty + 8 * (k & (PT_NOTES - 1)));
             }
         }
     }
