@@ -558,6 +558,7 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     g.table_stride = p->table_stride; g.num_pages = p->num_pages; g.rows = p->rows;
     g.scale_log2 = p->scale * LOG2E;
     g.seqs = p->seqs; g.width = p->table_width; g.q_heads = p->q_heads; g.kv_heads = p->kv_heads; g.group = group; g.page = p->page; g.max_q = max_q;
+    g.wide = 0;
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (many_queries(max_q, group)) return prompt_launch(g, p->head_dim, workspace, st);
     if (p->head_dim == 128)

@@ -225,6 +225,30 @@ __device__ __noinline__ uint32_t nan_blocks(const AttnArgs &g, int b, int head, 
     return bits;
 }
 
+// 32 bytes at once where `wide` (the address is a multiple of 32), else in two pieces.  A thread of the softmax has a row of its own, so
+// each piece of a warp's access is in another line, and a line takes a clock.
+__device__ __forceinline__ void ld_row32(const void *p, bool wide, uint4 &a, uint4 &b)
+{
+    if (wide) {
+        asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+                     : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
+                     : "l"(p));
+    } else {
+        a = ld_v4(p);
+        b = ld_v4(static_cast<const uint8_t *>(p) + 16);
+    }
+}
+__device__ __forceinline__ void st_row32(void *p, bool wide, uint4 a, uint4 b)
+{
+    if (wide) {
+        asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b.x), "r"(b.y), "r"(b.z), "r"(b.w)
+                     : "memory");
+    } else {
+        static_cast<uint4 *>(p)[0] = a;
+        static_cast<uint4 *>(p)[1] = b;
+    }
+}
+
 template <int D>
 __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_constant__ AttnArgs g, const PromptPlan plan)
 {
@@ -548,8 +572,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             uint32_t acc = 0;
             const uint16_t *src = g.q + (int64_t)(s.q0 + at.i) * g.q_token + at.h * g.q_head;
 #pragma unroll
+            for (int j = 0; j < D / 8; j++) w[j] = make_uint4(0, 0, 0, 0);
+            if (at.live) {
+#pragma unroll
+                for (int j = 0; j < D / 8; j += 2) ld_row32(src + 8 * j, g.wide & 1, w[j], w[j + 1]);
+            }
+#pragma unroll
             for (int j = 0; j < D / 8; j++) {
-                w[j] = at.live ? ld_v4(src + 8 * j) : make_uint4(0, 0, 0, 0);
                 acc = absmax2_acc(absmax2_acc(absmax2_acc(absmax2_acc(acc, w[j].x), w[j].y), w[j].z), w[j].w);
             }
             float mult, back;
@@ -729,14 +758,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                             y[j] = *reinterpret_cast<const uint32_t *>(&b);
                         }
                         if (at.live) {
-                            uint4 *dst = reinterpret_cast<uint4 *>(g.out + to * D + c);
-                            dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
-                            dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
+                            st_row32(g.out + to * D + c, g.wide & 2, make_uint4(y[0], y[1], y[2], y[3]), make_uint4(y[4], y[5], y[6], y[7]));
                         }
                     } else {
-                        uint4 *dst = reinterpret_cast<uint4 *>(part + (x * 128 + row) * D + c);
+                        float *dst = part + (x * 128 + row) * D + c;
 #pragma unroll
-                        for (int j = 0; j < 4; j++) dst[j] = make_uint4(o[4 * j], o[4 * j + 1], o[4 * j + 2], o[4 * j + 3]);
+                        for (int j = 0; j < 16; j += 8)
+                            st_row32(dst + j, g.wide & 4, make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]), make_uint4(o[j + 4], o[j + 5], o[j + 6], o[j + 7]));
                     }
                 }
                 if (!whole) reinterpret_cast<float2 *>(part + PT_ROWS * D)[x * 128 + row] = make_float2(m, l);
@@ -764,7 +792,7 @@ bool prompt_fits(int64_t rows, int group, int seqs, int kv_heads, int64_t cached
 }
 size_t prompt_workspace_bytes(int64_t rows, int group, int seqs, int head_dim)
 {
-    return (prompt_plan_bytes(prompt_max_pairs(rows, group, seqs)) + 15) / 16 * 16 + (size_t)2 * sm_count() * (16 + PT_ROWS * (head_dim + 2) * 4);
+    return (prompt_plan_bytes(prompt_max_pairs(rows, group, seqs)) + 31) / 32 * 32 + (size_t)2 * sm_count() * (16 + PT_ROWS * (head_dim + 2) * 4);
 }
 
 template <int D>
@@ -786,8 +814,10 @@ static int launch(AttnArgs g, void *ws, cudaStream_t st)
     const int64_t max_pairs = prompt_max_pairs(g.rows, g.group, g.seqs);
     const PromptPlan plan = prompt_plan(ws, max_pairs);
     const int grid = sm_count();
-    g.seams = reinterpret_cast<int4 *>(static_cast<uint8_t *>(ws) + (prompt_plan_bytes(max_pairs) + 15) / 16 * 16);
+    g.seams = reinterpret_cast<int4 *>(static_cast<uint8_t *>(ws) + (prompt_plan_bytes(max_pairs) + 31) / 32 * 32);
     g.part = reinterpret_cast<float *>(g.seams + 2 * grid);
+    const auto by32 = [](const void *p) { return (reinterpret_cast<uintptr_t>(p) & 31) == 0; };
+    g.wide = (by32(g.q) && g.q_token % 16 == 0 && g.q_head % 16 == 0 ? 1 : 0) | (by32(g.out) ? 2 : 0) | (by32(g.part) ? 4 : 0);
     cudaError_t e = launch_maybe_pdl(kv_prompt_plan_kernel, dim3(1), dim3(1024), 0, st, true, g, plan);
     if (e != cudaSuccess) return (int)e;
     e = launch_maybe_pdl(kv_prompt_kernel<D>, dim3(grid), dim3(PT_THREADS), C::SMEM, st, true, g, plan);
