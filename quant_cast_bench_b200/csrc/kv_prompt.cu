@@ -260,7 +260,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
     const uint32_t s_q = sm, s_k = sm + 2 * C::TILE, s_v = sm + 4 * C::TILE, s_raw = sm + 6 * C::TILE, bars = s_raw + PT_RAW * C::RAW;
     const uint32_t raw_full = bars, raw_empty = bars + 24, k_full = bars + 48, k_empty = bars + 64, v_full = bars + 80, v_empty = bars + 96, q_full = bars + 112,
                    s_full = bars + 128, p_full = bars + 144, o_done = bars + 160;
-    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_nan = bars + 216, s_ml = bars + 256,      // s_info: notes of the last 8 tiles, tokens that exist, PT_LAST, PT_TWO
+    const uint32_t s_info = bars + 176, slot = bars + 208, abort = bars + 212, s_nan = bars + 216, meeting = bars + 224, s_ml = bars + 256,      // s_info: notes of the last 8 tiles, tokens that exist, PT_LAST, PT_TWO
                    part_full = s_ml + 128 * 8, part_empty = part_full + 8 * PT_NOTES, s_part = part_empty + 8 * PT_NOTES;      // notes on parts
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
@@ -300,6 +300,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         }
         for (int i = 0; i < PT_NOTES; i++) { mbar_init_at(part_full + 8 * i, 1); mbar_init_at(part_empty + 8 * i, 8); }
         asm volatile("st.shared.u32 [%0], %1;" ::"r"(abort), "r"(0u) : "memory");
+        mbar_init_at(meeting, 8);
         sts_u32(s_nan, 0);
         fence_barrier_init();
     }
@@ -345,7 +346,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     }
                     const int n = __popc(__ballot_sync(0xFFFFFFFFu, pg >= 0));
                     const uint8_t *src = g.cache + (pg * g.kv_heads + s.head) * (int64_t)(2 * half);
-#pragma unroll
+#pragma unroll 1
                     for (int w = 0; w < 2; w++) {
                         mbar_wait_at(raw_empty + 8 * (st), ph, PT_ERR, abort);
                         if (lane == 0) {
@@ -369,7 +370,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             // rows are tokens, the contracted side, the 16384 bytes between 64-element blocks of a row
             constexpr uint32_t high = 64u | (1u << 14) | (2u << 29);
             const uint32_t dq = (s_q >> 4) | (1u << 16), dk = (s_k >> 4) | (1u << 16), dv = (s_v >> 4) | (1024u << 16);
-            uint32_t kt = 0, vt = 0, qn[2] = {0, 0}, pn[2] = {0, 0};      // tiles of K and V; of each row tile: units, probabilities so far
+            uint32_t kt = 0, vt = 0, qn = 0, pn = 0;      // tiles of K and V; bit x: phase of row tile x's units, probabilities
             const auto scores = [&](int x, uint32_t kb) {
                 const uint32_t a = dq + x * (C::TILE >> 4), b = dk + kb * (C::TILE >> 4);
 #pragma unroll
@@ -409,16 +410,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                         tc_commit_at(k_empty + 8 * (kt & 1));
                         kt++;
                     };
-                    mbar_wait_at(q_full, qn[0]++ & 1, PT_ERR, abort);
+                    mbar_wait_at(q_full, qn & 1, PT_ERR, abort);
+                    qn ^= 1;
                     next(0);
                     if (!(info & PT_LAST)) {
-                        mbar_wait_at(q_full + 8, qn[1]++ & 1, PT_ERR, abort);
+                        mbar_wait_at(q_full + 8, qn >> 1 & 1, PT_ERR, abort);
+                        qn ^= 2;
                         next(1);
                     }
                     for (uint32_t j = 0; vt != kt && !lds_volatile(abort); j++) {
                         const int x = j & 1;
                         mbar_wait_at(v_full + 8 * (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
-                        mbar_wait_at(p_full + 8 * x, pn[x]++ & 1, PT_ERR, abort);
+                        mbar_wait_at(p_full + 8 * x, pn >> x & 1, PT_ERR, abort);
+                        pn ^= 1u << x;
                         tc_fence_after();
                         product(x, vt & 1, j > 1);
                         tc_commit_at(v_empty + 8 * (vt & 1));
@@ -428,8 +432,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     if (lds_volatile(abort)) break;
                     continue;
                 }
+#pragma unroll 1
                 for (int x = 0; x < 2; x++) {
-                    mbar_wait_at(q_full + 8 * (x), qn[x]++ & 1, PT_ERR, abort);
+                    mbar_wait_at(q_full + 8 * x, qn >> x & 1, PT_ERR, abort);
+                    qn ^= 1u << x;
                     tc_fence_after();
                     scores(x, kt & 1);
                 }
@@ -439,8 +445,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     const bool more = !(info & PT_LAST);
                     mbar_wait_at(v_full + 8 * (vt & 1), (vt >> 1) & 1, PT_ERR, abort);
                     if (more) mbar_wait_at(k_full + 8 * (kt & 1), (kt >> 1) & 1, PT_ERR, abort);
+#pragma unroll 1
                     for (int x = 0; x < 2; x++) {
-                        mbar_wait_at(p_full + 8 * (x), pn[x]++ & 1, PT_ERR, abort);
+                        mbar_wait_at(p_full + 8 * x, pn >> x & 1, PT_ERR, abort);
+                        pn ^= 1u << x;
                         tc_fence_after();
                         product(x, vt & 1, o);
                         if (more) scores(x, kt & 1);      // over P: instructions run in order, the product above has read it
@@ -467,7 +475,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         uint32_t st = 0, ph = 0, tiles = 0;
         for (const uint32_t count = hi - lo; tiles < count; tiles++) {
             const uint32_t buf = tiles & 1;
-#pragma unroll
+#pragma unroll 1
             for (int v = 0; v < 2; v++) {
                 {
                     const uint32_t out_full = v ? v_full : k_full, out_empty = v ? v_empty : k_empty, out = v ? s_v : s_k;
@@ -530,13 +538,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         uint32_t sn = 0, on = 0;        // scores, products so far
         float factor = 0.0f;
         bool placed = false;            // q of the part is in place already
-        // part k, which starts at tile t, from its note (after a wait has run out: by search)
-        const auto read_note = [&](uint32_t k, int t) {
+        // the note on part k; after the wait for it, that it is there (not so when some wait has run out)
+        const auto noted = [&](uint32_t k) {
+            mbar_wait_at(part_full + 8 * (k & (PT_NOTES - 1)), k / PT_NOTES & 1, PT_ERR, abort);
+            return (bool)__all_sync(0xFFFFFFFFu, lds_volatile(abort) == 0);
+        };
+        const auto read_note = [&](uint32_t k) {
             Part s;
-            if (lds_volatile(abort)) {
-                find_part(g, plan, pairs, t, hi, s);
-                return s;
-            }
             const uint32_t note = s_part + (k & (PT_NOTES - 1)) * 48;
             const uint4 a = lds_v4(note), b = lds_v4(note + 16);
             s.b = a.x; s.q0 = a.y; s.n = a.z; s.L = a.w;
@@ -544,9 +552,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             s.last = lds_volatile(note + 32);
             return s;
         };
-        const auto read_part = [&](uint32_t k, int t) {
-            mbar_wait_at(part_full + 8 * (k & (PT_NOTES - 1)), k / PT_NOTES & 1, PT_ERR, abort);
-            return read_note(k, t);
+        // both softmaxes meet (a wait with a limit, as all are)
+        uint32_t met = 0;
+        const auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive_at(meeting);
+            mbar_wait_at(meeting, met++ & 1, PT_ERR, abort);
         };
         // This thread's row of a part.  Both row tiles have rows: one for each softmax; one has: both softmaxes take it, and the
         // tiles of tokens in turn.
@@ -596,10 +607,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             return f < 1e-37f ? 1e-37f : f;       // not zero: -inf of a hidden key has to stay
         };
         for (int t = lo, k = 0; t < hi; k++) {
-            const int t_part = t;
+            if (!noted(k)) break;
             int tile, last, step, limit;
             {
-                const Part s = read_part(k, t);
+                const Part s = read_note(k);
                 const Rows at = rows_of(s);
                 tile = at.first;
                 last = s.last;
@@ -645,7 +656,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                         if (any) {
                             mbar_wait_at(o_done + 8 * x, (on - 1) & 1, PT_ERR, abort);
                             tc_fence_after();
-#pragma unroll
+#pragma unroll 1
                             for (int c = 0; c < D; c += 16) {
                                 uint32_t o[16];
                                 tmem_ld16(t_o + c, o);
@@ -686,15 +697,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     on++;
                     any = true;
                 }
-                const Part s = read_note(k, t_part);      // (again: it would take up registers that the loop needs)
+                const Part s = read_note(k);      // (again: it would take up registers that the loop needs)
                 const Rows at = rows_of(s);
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at(part_empty + 8 * (k & (PT_NOTES - 1)));
                 const bool whole = s.first == 0 && s.last == s.tiles, join = !at.two && s.last - s.first > 1;
-                if (!join && t < hi) {
+                if (!join && t < hi && noted(k + 1)) {
                     // q of the next part, whose first scores are then worked out behind the end of this one (one that joins needs the
                     // space of q)
-                    const Part n = read_part(k + 1, t);
+                    const Part n = read_note(k + 1);
                     const Rows to = rows_of(n);
                     if (to.first < n.last) {
                         factor = place_q(n, to);
@@ -706,9 +717,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                 float mine = 1.0f, others = 0.0f;         // weights of this softmax's sums and of the other's
                 if (join) {
                     // the second softmax hands its sums over in Q's place, column by column
-                    named_barrier(1, 256);                // (both are done with Q)
+                    meet();                // (both are done with Q)
                     if (x) {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < D; c += 16) {
                             uint32_t o[16];
                             tmem_ld16(t_o + c, o);
@@ -720,9 +731,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                         sts_u32(s_ml + row * 8 + 4, f2u(l));
                         tc_fence_before();
                     }
-                    named_barrier(1, 256);
+                    meet();
                     if (x) {
-                        named_barrier(1, 256);            // (the sums are read)
+                        meet();            // (the sums are read)
                         continue;
                     }
                     const float m1 = u2f(lds_volatile(s_ml + row * 8)), l1 = u2f(lds_volatile(s_ml + row * 8 + 4)), up = fmaxf(m, m1);
@@ -737,7 +748,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                 const float scale = l == 0.0f ? 0.0f : __fdividef(v_outer, l);
                 const int64_t to = (int64_t)(s.q0 + at.i) * g.q_heads + at.h;
                 float *part = g.part + (size_t)(2 * blockIdx.x + (k ? 1 : 0)) * prompt_part_floats<D>();
-#pragma unroll
+#pragma unroll 1
                 for (int c = 0; c < D; c += 16) {
                     uint32_t o[16];
                     tmem_ld16(t_o + c, o);
@@ -770,7 +781,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                 if (!whole) reinterpret_cast<float2 *>(part + PT_ROWS * D)[x * 128 + row] = make_float2(m, l);
                 else if (at.live && g.lse) g.lse[to] = l == 0.0f ? -INFINITY : (m + log2f(l)) * LN2;
                 tc_fence_before();       // the next unit's products write O
-                if (join) named_barrier(1, 256);
+                if (join) meet();
             } else {
                 __syncwarp();
                 if (lane == 0) mbar_arrive_at(part_empty + 8 * (k & (PT_NOTES - 1)));
