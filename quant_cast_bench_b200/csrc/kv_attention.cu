@@ -503,7 +503,7 @@ static int split_launch(const AttnArgs &g, cudaStream_t st)
     const int grid = sm_count() * C::CTAS;
     cudaError_t e = launch_maybe_pdl(kv_attn_split_kernel<D, NT>, dim3(grid), dim3(SP_THREADS), C::FIXED + (g.seqs + 1) * 4, st, true, g);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_maybe_pdl(kv_join_kernel<D, 4, 8, 8 * D>, dim3(grid, NT), dim3(8 * D), 0, st, true, g, grid, NT * 8);
+    return (int)launch_maybe_pdl(kv_join_kernel<D, 2, 4, 2 * D>, dim3(grid, 2 * NT), dim3(2 * D), 0, st, true, g, grid, NT * 8);
 }
 
 // how the rows of a sequence and kv head are tiled: 8 * nt rows

@@ -833,7 +833,7 @@ static int launch(AttnArgs g, void *ws, cudaStream_t st)
     if (e != cudaSuccess) return (int)e;
     e = launch_maybe_pdl(kv_prompt_kernel<D>, dim3(grid), dim3(PT_THREADS), C::SMEM, st, true, g, plan);
     if (e != cudaSuccess) return (int)e;
-    return (int)launch_maybe_pdl(kv_join_kernel<D, 1, 32, 256>, dim3(grid, PT_ROWS / 32), dim3(256), 0, st, true, g, grid, PT_ROWS);
+    return (int)launch_maybe_pdl(kv_join_kernel<D, 1, 16, 256>, dim3(grid, PT_ROWS / 16), dim3(256), 0, st, true, g, grid, PT_ROWS);
 }
 
 int prompt_launch(const AttnArgs &g, int head_dim, void *ws, cudaStream_t st)
