@@ -23,6 +23,11 @@ namespace qcc {
 // Roles: warp 0 copies, warp 1 issues the matrix instructions, warps 4-7 widen, warps 8-11 and 12-15 are the softmax of the two
 // row tiles.  All (unit, tile) pairs are numbered, by a first small kernel, and dealt out evenly to one CTA per SM, whatever the lengths and however
 // many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
+//
+// Measured, 32 heads over 8 of 128 elements: 4096 queries over 12288 tokens 599 us, 1.15 PFLOP/s (tensor cores 56 % active); 16 prompts of up to 700 tokens
+// 111 us.  A pair of row tiles and a tile of tokens takes about 3000 clocks, of which the exponentials are 1024 and the matrix
+// instructions 1024 by their rates, one after the other for a row tile.  The warps' code is close to what the instruction cache holds: loops
+// that run once a part or are not on the critical path are rolled up (145 -> 111 us for the prompts of 700 tokens).
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3, PT_NOTES = 8;
 constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u, PT_MASK = 1024u;      // notes on a tile: the last of its part; both row tiles of its
