@@ -160,6 +160,14 @@ def test_product_of_the_largest_codes_does_not_overflow(M, N, K):
 
 
 @gpu
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("M,N,K", [(90, 10001, 256), (150, 10001, 272), (190, 10000, 256), (200, 10001, 272), (600, 4096, 2048), (1111, 5003, 272), (2000, 4096, 1040)])
+def test_product_tiles_between_the_powers_of_two(M, N, K, dtype):
+    """Shapes that on 148 SMs take tiles of 96, 160, 192 and 224 tokens, one tile a CTA and several."""
+    check(*make(M, N, K, True, seed=M), dtype=dtype)
+
+
+@gpu
 def test_product_many_tiles_and_rows():
     """More tiles than SMs, several groups of token tiles, both accumulators of the persistent loop."""
     check(*make(2600, 1300, 256, True, seed=9), dtype=torch.bfloat16)

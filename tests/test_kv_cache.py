@@ -396,6 +396,13 @@ def test_decode_many_sequences():
 
 
 @gpu
+def test_most_sequences_a_call_takes():
+    lens = [(i * 37) % 40 for i in range(4096)]
+    check_attention(64, 16, 2, 1, lens, seed=14)
+    check_attention(64, 16, 40, 1, lens, [(i * 5) % 3 for i in range(4096)], seed=15)
+
+
+@gpu
 @pytest.mark.parametrize("page,D,hq,heads", [(16, 128, 8, 2), (128, 64, 6, 6), (32, 128, 16, 1), (64, 64, 40, 8)])
 @pytest.mark.parametrize("lens,q_lens", [([5, 130, 0, 64], [2, 4, 3, 1]), ([300, 17], [7, 17]), ([3], [9]), ([400, 1, 129], [130, 1, 66]), ([700], [257])])
 def test_several_queries(page, D, hq, heads, lens, q_lens):
