@@ -35,8 +35,8 @@ constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ra
 // whatever the lengths; a unit (sequence, head, row tile) that spans CTAs leaves partial sums which a second kernel joins in a
 // fixed order.
 //
-// Measured, 32 heads over 8 of 128 elements: 64 sequences of up to 16384 tokens 138 us, 4.25 TB/s of the cache, 55 % of the issue slots and of the
-// ALU pipe; 2 of 131072 with 64 heads 76 us.  647 warp instructions for 32 tokens, of which the conversions, scalings and nibble merges are
+// Measured, 32 heads over 8 of 128 elements: 64 sequences of up to 16384 tokens 133.5 us, 4.4 TB/s of the cache, 55 % of the issue slots and of the
+// ALU pipe; 2 of 131072 with 64 heads 73 us.  647 warp instructions for 32 tokens, of which the conversions, scalings and nibble merges are
 // 372 and the matrix instructions 32.
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int SP_WARPS = 4, SP_THREADS = SP_WARPS * 32, SP_WTOK = 32, SP_TOK = SP_WTOK * SP_WARPS;
@@ -48,7 +48,8 @@ template <int D, int NT> struct SplitCfg {
     static constexpr int TILE = SP_WTOK * 2 * (D / 2 + D / 16);     // bytes of one warp's tokens, keys and values
     static constexpr int CTAS = split_ctas(D, NT);
     static constexpr int STAGES = (NT == 4 ? 4 : 2) * (D == 64 ? 2 : 1);
-    static constexpr bool QS = NT * D > 256;                        // Q in shared memory: it would not fit the registers beside O
+    // Q in shared memory: it would not fit the registers beside O (NT 1 and 128 elements: it would just, 138 against 133 us for 64 sequences)
+    static constexpr bool QS = NT * D > 256 || (NT == 1 && D == 128);
     static constexpr int QBYTES = QS ? NT * (D / 32) * 32 * 16 : 0;
     static constexpr int RED = SP_WARPS * NT * 8 * (D / 4) * 4;
     static constexpr int ML = SP_WARPS * NT * 8 * 2 * 4;
