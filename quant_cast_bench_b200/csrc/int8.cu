@@ -339,6 +339,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
         // no CTA leaves while another may still read its sums
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
+    settle(abort);
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {

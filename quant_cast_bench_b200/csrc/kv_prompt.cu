@@ -794,6 +794,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         }
     }
     __syncwarp();
+    settle(abort);
     tc_fence_before();
     __syncthreads();
     if (warp == 2) {

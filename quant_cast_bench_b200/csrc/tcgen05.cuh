@@ -67,6 +67,14 @@ __device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsi
     atomicMax(&g_qcc_error, code);
 }
 
+// The end of a kernel in which a wait has run out: copies and matrix instructions that are still under way get a millisecond to end
+// before the CTA's shared and tensor memory are given up.  Before the last barrier of the CTA.
+__device__ __forceinline__ void settle(uint32_t abort)
+{
+    if (threadIdx.x == 0 && lds_volatile(abort))
+        for (int i = 0; i < 1000; i++) __nanosleep(1000);
+}
+
 __device__ __forceinline__ void tma_load_2d_at(uint32_t dst, const CUtensorMap *map, uint32_t bar, int x, int y)
 {
     asm volatile(
