@@ -19,6 +19,7 @@ struct AttnArgs {
     int64_t q_token, q_head, table_stride, num_pages, rows;
     float scale_log2;
     int seqs, width, q_heads, kv_heads, group, page, max_q;
+    int whole;              // kv_attention.cu: units are dealt out whole, none spans CTAs
     int wide;               // kv_prompt.cu: rows of q (1), of out (2), of part (4) lie on 32-byte boundaries
 };
 
