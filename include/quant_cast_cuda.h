@@ -513,7 +513,8 @@ int qcc_nvfp4_kv_gather(const void *cache, int64_t num_pages, int kv_heads, int 
  * queries of a sequence.  q head h reads kv head h / (q_heads / kv_heads).
  *   out (rows, q_heads, head_dim) bf16 = sum_j softmax_j(scale * q . k_j) v_j;  lse (rows, q_heads) fp32, may be NULL, =
  *   log sum_j exp(scale * q . k_j).  A query that sees no key, and every row behind the last sequence: out = 0, lse = -inf.
- * Sums, maxima and the softmax in fp32; the probabilities are rounded to fp16 before they multiply the values.
+ * Sums, maxima and the softmax in fp32; the probabilities are rounded to fp16 before they multiply the values (half a step, 2^-11 of each,
+ * down to 2^-21 of a row's largest; below, 2^-32 of the largest).
  * The result does not depend on what the slots behind a sequence's last token hold, that of a query not on the tokens behind it,
  * NaN among them.  Two runs on the same inputs give the
  * same bits.  A sequence whose query offsets descend, leave the rows of q or hold more than max_q rows sets code 22 in the word

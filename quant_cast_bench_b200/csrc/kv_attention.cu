@@ -27,7 +27,7 @@ constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ra
 //                  are brought side by side before they are widened, which gives the token pairs of the fragment.
 // The queries are on the N side, 8 at a time: no row of the instruction is spent on padding when a group has 8 heads.
 // Codes times block scales are exact in fp16 (2 + 4 significant bits); q is brought to fp16 by a power of two for its row,
-// exact for all elements above 2^-22 of the row's largest; P is rounded to fp16, half a step of 2^-11.  The tensor cores are
+// exact for all elements above 2^-22 of the row's largest; P is rounded to fp16 (see P_LIFT).  The tensor cores are
 // far from busy (tcgen05 would need the widened tiles in shared memory, whose bandwidth that alone would use up).
 //
 // A tile is 128 tokens of one sequence and head, 32 for each warp.  A warp fetches its own tokens by bulk copies into a ring of
@@ -309,8 +309,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                         }
                     }
                 }
-                // exponents of the probabilities, against the running maximum; it moves only when a score is 2^8 above it, so that P
-                // stays below 2^8
+                // exponents of the probabilities, against the running reference
                 const auto seen = [&](int h, int nt, int x) { return !MASKED || tok + (h0 + h) * 16 + gr + (x >> 1) * 8 < limit[nt][x & 1]; };
                 float e[HB][NT][4], most = -INFINITY;
 #pragma unroll
@@ -322,7 +321,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                             e[h][nt][x] = seen(h, nt, x) ? fmaf(sc[h][nt][x], factor[nt][x & 1], -m[nt][x & 1]) : -INFINITY;
                             most = fmaxf(most, e[h][nt][x]);
                         }
-                if (__any_sync(0xFFFFFFFFu, most > 8.0f)) {
+                if (__any_sync(0xFFFFFFFFu, most > P_MOST)) {
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -331,7 +330,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
 #pragma unroll
                             for (int h = 0; h < HB; h++)
 #pragma unroll
-                                for (int y = x; y < 4; y += 2) v = fmaxf(v, seen(h, nt, y) ? sc[h][nt][y] * factor[nt][x] : -INFINITY);
+                                for (int y = x; y < 4; y += 2) v = fmaxf(v, seen(h, nt, y) ? fmaf(sc[h][nt][y], factor[nt][x], -P_LIFT) : -INFINITY);
 #pragma unroll
                             for (int sh = 4; sh < 32; sh <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, sh));
                             const float a = v == -INFINITY ? 1.0f : ex2(m[nt][x] - v);

@@ -7,6 +7,10 @@ namespace qcc {
 constexpr unsigned int QCC_DEVERR_QUERIES = 22u;    // query offsets that are not ascending within the rows of q
 constexpr int KV_MAX_SEQS = 4096;
 constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
+// Probabilities are kept against a reference that is P_LIFT below a row's maximum, in fp16: a row's largest is 2^7 when the reference
+// is set and, as that moves only once a score is P_MOST above it, at most 2^15.  So the upper end of fp16's range is used, and a key's rounding is half a step,
+// 2^-11, down to 2^-21 of the largest; below, half of 2^-24, 2^-32 of the largest.  (All in log2 units; lse has the reference added back.)
+constexpr float P_LIFT = 7.0f, P_MOST = 15.0f;
 
 struct AttnArgs {
     const uint16_t *q;

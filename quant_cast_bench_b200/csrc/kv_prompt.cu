@@ -17,8 +17,8 @@ namespace qcc {
 //   O += P V    P from tensor memory, V in shared memory (its elements contiguous: the N-major form), O in tensor memory.
 // The codes of a page come by bulk copies; four warps widen them to fp16 (codes times block scales: exact) straight into the
 // 128-byte swizzled rows that the instructions read, the same layout for K and V.  That happens once for 256 rows.
-// q is brought to fp16 by a power of two for its row, exact for all elements above 2^-22 of the row's largest; P is rounded to fp16, half a step
-// of 2^-11; sums and maxima stay in fp32.  O is only rescaled when a row's maximum has grown by more than 2^8.
+// q is brought to fp16 by a power of two for its row, exact for all elements above 2^-22 of the row's largest; P is rounded to fp16 (see P_LIFT);
+// sums and maxima stay in fp32.  O is only rescaled when a row's maximum has grown by more than 2^8.
 //
 // Roles: warp 0 copies, warp 1 issues the matrix instructions, warps 4-7 widen, warps 8-11 and 12-15 are the softmax of the two
 // row tiles.  All (unit, tile) pairs are numbered, by a first small kernel, and dealt out evenly to one CTA per SM, whatever the lengths and however
@@ -652,10 +652,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     for (int j = 2; j < 32; j += 2)
 #pragma unroll
                         for (int c = 0; c < 4; c++) top[c] = max3(top[c], u2f(v[c][j]), u2f(v[c][j + 1]));
-                    const float most = fmaxf(max3(top[0], top[1], top[2]), top[3]) * scale_in;
-                    const bool grow = most - m > 8.0f;           // (from -inf: always, once the row sees a key)
+                    const float most = fmaxf(max3(top[0], top[1], top[2]), top[3]);
+                    const bool grow = fmaf(most, scale_in, -m) > P_MOST;      // (from -inf: always, once the row sees a key; one rounding, as below)
                     if (__any_sync(0xFFFFFFFFu, grow)) {
-                        const float up = grow ? most : m, a = grow ? ex2(m - up) : 1.0f;
+                        const float up = grow ? fmaf(most, scale_in, -P_LIFT) : m, a = grow ? ex2(m - up) : 1.0f;
                         m = up;
                         l *= a;
                         if (any) {

@@ -764,3 +764,31 @@ def test_a_decoder_step():
         want = (oq.cpu().double() @ wo.cpu().double().T) * os_.cpu().double() * wos.cpu().double().T
         assert bool(((y.cpu().double() - want).abs() <= 3.01 * 2.0 ** -24 * want.abs() + want.abs() * 2.0 ** -24).all())
     assert L.device_error() == 0
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hq,q_len", [(4, 1), (16, 1), (32, 1), (8, 10), (8, 40)])      # each form of the kernels
+@pytest.mark.parametrize("every,ratio", [(32, 1.5 * 2.0 ** -24), (32, 1.3 * 2.0 ** -26), (32, 2.0 ** -19), (4096, 1.5 * 2.0 ** -24)])
+def test_a_flat_tail_keeps_its_weight_beside_dominant_keys(D, hq, q_len, every, ratio):
+    """Dominant keys, `every` tokens apart, whose values are zero, over a tail of keys of one score whose values are one: the output is the
+    tail's share.  All keys of the tail are rounded alike, so nothing averages out.  A probability is rounded by half a step of fp16, 2^-11, or
+    below fp16's normal numbers by half of 2^-24 where a dominant one is at least 2^7: 2^-32 of it.  Scores: see the module's docstring."""
+    n, page = 4096, 64
+    table = torch.randperm(n // page, generator=torch.Generator().manual_seed(D)).to(torch.int32).view(1, -1)
+    cache = torch.zeros(n // page, 1, 2, page * 9 * D // 16, dtype=torch.uint8)
+    codes, scales = planes(cache, D)
+    scales.fill_(0x38)                                        # 1.0
+    at = torch.arange(n)
+    loud = at % every == 0
+    codes[table[0, at // page].long(), 0, 0, at % page] = (loud * 0x22).to(torch.uint8).view(-1, 1).expand(-1, D // 2)
+    codes[table[0, at // page].long(), 0, 1, at % page] = (~loud * 0x22).to(torch.uint8).view(-1, 1).expand(-1, D // 2)
+    scale = float(torch.tensor(-math.log(ratio) / D))
+    q, one = torch.ones(q_len, hq, D, dtype=torch.bfloat16), torch.ones(1)
+    out, lse = call(q, cache, table, [n], [q_len], one, one, scale, decode=q_len == 1)
+    o, z, _, ltol = attention_ref(q, cache, table, [n], [q_len], one, one, scale)
+    e = (D + 2) * 2.0 ** -23 * scale * D
+    tol = (2 * e + 2.0 ** -11 + (n + 64) * 2.0 ** -23 + 2.0 ** -8) * o + every * 2.0 ** -32
+    err = (out.cpu().double() - o).abs()
+    assert bool((err <= tol * 1.01).all()), f"off by {float((err / o).max())} of the tail, {float((tol / o).max())} allowed"
+    assert bool(((lse.cpu().double() - z).abs() <= ltol).all()) and L.device_error() == 0
