@@ -339,9 +339,9 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
         // no CTA leaves while another may still read its sums
         asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
     }
-    settle(abort);
     tc_fence_before();
     __syncthreads();
+    settle(abort);
     if (warp == 2) {
         tc_fence_after();
         tmem_free(tmem, TMEM_COLS);

@@ -794,9 +794,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         }
     }
     __syncwarp();
-    settle(abort);
     tc_fence_before();
     __syncthreads();
+    settle(abort);
     if (warp == 2) {
         tc_fence_after();
         tmem_free(tmem, 512);

@@ -68,10 +68,10 @@ __device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsi
 }
 
 // The end of a kernel in which a wait has run out: copies and matrix instructions that are still under way get a millisecond to end
-// before the CTA's shared and tensor memory are given up.  Before the last barrier of the CTA.
+// before the CTA's shared and tensor memory are given up.  By all threads, after the last barrier of the CTA: by then nobody issues any more.
 __device__ __forceinline__ void settle(uint32_t abort)
 {
-    if (threadIdx.x == 0 && lds_volatile(abort))
+    if (lds_volatile(abort))
         for (int i = 0; i < 1000; i++) __nanosleep(1000);
 }
 
