@@ -202,11 +202,12 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
     if (warp == 0) {
         if (elect_one()) {
             uint32_t s = 0, ph = 1;
-            for (int t = t0; t < total; t += step) {
+            bool go = true;
+            for (int t = t0; go && t < total; t += step) {
                 int tn, tm;
                 mm_tile(g, t, tn, tm);
                 for (int kb = kb0; kb < kb1; kb++) {
-                    mbar_wait_at(empty + 8 * s, ph, MM_ERR, abort);
+                    if (!(go = mbar_reached(empty + 8 * s, ph, MM_ERR, abort))) break;
                     const uint32_t p = stages + s * C::STAGE, bar = full + 8 * s;
                     mbar_expect_at(bar, C::STAGE);
                     tma_load_2d_at(p, &map_w, bar, kb * MM_BK, tn * MM_BM);
@@ -220,12 +221,13 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
             constexpr uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(MM_BM >> 4) << 24);
             constexpr uint32_t high = 64u | (1u << 14) | (2u << 29);      // high words of the descriptors: 8 rows are 1024 bytes, 128-byte swizzle
             uint32_t s = 0, ph = 0, n = 0;
-            for (int t = t0; t < total; t += step, n++) {
+            bool go = true;
+            for (int t = t0; go && t < total; t += step, n++) {
                 const uint32_t acc = SPLIT ? 0 : n & 1, aph = SPLIT ? 0 : (n >> 1) & 1;
-                mbar_wait_at(acc_empty + 8 * acc, aph ^ 1, MM_ERR, abort);
+                if (!mbar_reached(acc_empty + 8 * acc, aph ^ 1, MM_ERR, abort)) break;
                 tc_fence_after();
                 for (int kb = kb0; kb < kb1; kb++) {
-                    mbar_wait_at(full + 8 * s, ph, MM_ERR, abort);
+                    if (!(go = mbar_reached(full + 8 * s, ph, MM_ERR, abort))) break;
                     tc_fence_after();
                     const uint32_t da = ((stages + s * C::STAGE) >> 4) | (1u << 16), db = da + (MM_BM * MM_BK >> 4);
 #pragma unroll

@@ -49,7 +49,9 @@ __device__ __forceinline__ uint32_t lds_volatile(uint32_t addr)
     asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsigned int code, uint32_t abort)
+// Whether the phase was reached.  Who arms a barrier or issues copies or matrix instructions behind the wait has to leave where it was not:
+// arming a barrier again whose phase is incomplete is undefined.
+[[nodiscard]] __device__ __forceinline__ bool mbar_reached(uint32_t bar, uint32_t parity, unsigned int code, uint32_t abort)
 {
     for (uint32_t it = 0; it < (1u << 22); it++) {
         uint32_t done;
@@ -60,12 +62,15 @@ __device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsi
             : "=r"(done)
             : "r"(bar), "r"(parity)
             : "memory");
-        if (done) return;
-        if ((it & 63u) == 63u && lds_volatile(abort)) return;
+        if (done) return true;
+        if ((it & 63u) == 63u && lds_volatile(abort)) return false;
     }
     asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(abort), "r"(1u) : "memory");
     atomicMax(&g_qcc_error, code);
+    return false;
 }
+// the same for who only reads what the phase brings, or looks at the abort word later
+__device__ __forceinline__ void mbar_wait_at(uint32_t bar, uint32_t parity, unsigned int code, uint32_t abort) { (void)mbar_reached(bar, parity, code, abort); }
 
 // The end of a kernel in which a wait has run out: copies and matrix instructions that are still under way get a millisecond to end
 // before the CTA's shared and tensor memory are given up.  By all threads, after the last barrier of the CTA: by then nobody issues any more.

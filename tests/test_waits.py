@@ -20,3 +20,18 @@ def test_copies_settle_after_the_last_barrier(name):
     assert len(re.findall(r"\bsettle\(", text)) == 1
     at = text.index("settle(")
     assert text[:at].rstrip().endswith("__syncthreads();") and "tmem_free(" in text[at:at + 200]
+
+
+def loops_that_arm(text):
+    """The bodies of the innermost loops that arm a transaction barrier."""
+    for m in re.finditer(r"\bmbar_expect_at\(", text):
+        start = text.rindex("for (", 0, m.start())
+        yield text[start:m.end()]
+
+
+@pytest.mark.parametrize("name", ["int8.cu"])
+def test_no_barrier_is_armed_behind_a_wait_that_ran_out(name):
+    loops = list(loops_that_arm(source(name)))
+    assert loops
+    for body in loops:
+        assert "mbar_reached(" in body and "mbar_wait_at(" not in body and "break;" in body
