@@ -324,7 +324,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
             const uint32_t half = (uint32_t)(g.page * RB);
             Part s;
             find_part(g, plan, pairs, lo, hi, s);
-            for (uint32_t t = lo, k = 0; (int)t < hi; k++) {
+            bool go = true;
+            for (uint32_t t = lo, k = 0; go && (int)t < hi; k++) {
                 mbar_wait_at(part_empty + 8 * (k & (PT_NOTES - 1)), (k / PT_NOTES & 1) ^ 1, PT_ERR, abort);
                 if (__any_sync(0xFFFFFFFFu, lds_volatile(abort))) break;      // (the notes that are being read stay)
                 if (lane == 0) {
@@ -339,7 +340,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                 const int32_t *row = g.table + s.b * g.table_stride;
                 const uint32_t two = (int64_t)s.n * g.group - (int64_t)s.qt * PT_ROWS > 128 ? PT_TWO : 0;
                 const int clear = prompt_clear(s.n, s.L, s.qt, g.group);
-                for (int tile = s.first; tile < s.last; tile++, tiles++) {
+                for (int tile = s.first; go && tile < s.last; tile++, tiles++) {
                     const int p = tile * pages + lane;
                     int64_t pg = -1;
                     if (lane < pages && p < have) {
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     const uint8_t *src = g.cache + (pg * g.kv_heads + s.head) * (int64_t)(2 * half);
 #pragma unroll 1
                     for (int w = 0; w < 2; w++) {
-                        mbar_wait_at(raw_empty + 8 * (st), ph, PT_ERR, abort);
+                        if (!(go = __all_sync(0xFFFFFFFFu, mbar_reached(raw_empty + 8 * (st), ph, PT_ERR, abort)))) break;
                         if (lane == 0) {
                             if (w == 0)
                                 sts_u32(s_info + 4 * (tiles & 7), (uint32_t)min(max(s.L - tile * PT_TOK, 0), PT_TOK) | (tile + 1 == s.last ? PT_LAST : 0) | (tile >= clear ? PT_MASK : 0) | two);

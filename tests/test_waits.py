@@ -29,7 +29,7 @@ def loops_that_arm(text):
         yield text[start:m.end()]
 
 
-@pytest.mark.parametrize("name", ["int8.cu"])
+@pytest.mark.parametrize("name", ["int8.cu", "kv_prompt.cu"])
 def test_no_barrier_is_armed_behind_a_wait_that_ran_out(name):
     loops = list(loops_that_arm(source(name)))
     assert loops
