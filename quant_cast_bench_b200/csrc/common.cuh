@@ -460,8 +460,9 @@ __device__ __forceinline__ void mbar_expect_at(uint32_t bar, uint32_t bytes)
 }
 // Wait for phase `parity` with an iteration cap; on timeout record the code and carry on (the caller
 // then works on whatever is in shared memory, but never hangs).
-__device__ __forceinline__ void mbar_wait_addr(uint32_t a, uint32_t parity, unsigned int err_code)
+__device__ __forceinline__ void mbar_wait(uint64_t *bar, uint32_t parity, unsigned int err_code)
 {
+    uint32_t a = smem_u32(bar);
     for (uint32_t it = 0; it < (1u << 24); it++) {
         uint32_t done;
         asm volatile(
@@ -475,7 +476,6 @@ __device__ __forceinline__ void mbar_wait_addr(uint32_t a, uint32_t parity, unsi
     }
     atomicMax(&g_qcc_error, err_code);
 }
-__device__ __forceinline__ void mbar_wait(uint64_t *bar, uint32_t parity, unsigned int err_code) { mbar_wait_addr(smem_u32(bar), parity, err_code); }
 __device__ __forceinline__ void fence_barrier_init()
 {
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");

@@ -5,6 +5,7 @@
 // over the keys j that a query sees: query i of the n of a sequence with L cached tokens sees j <= L - n + i.  A query that
 // sees none gets o = 0 and lse = -inf.  One pass over the cache with the running maximum and sum of the softmax in fp32.
 #include "kv_attention.cuh"
+#include "tcgen05.cuh"      // settle()
 
 #include <type_traits>
 
@@ -62,6 +63,24 @@ struct Segment {
     int b, q0, n, L, head, first, last, unit_last;   // first, last: tiles of the unit; unit_last: flat number of the tile behind it
 };
 
+// Whether the copies of phase `parity` have come within `polls` polls.  (No look at an abort word, as elsewhere: that alone took 3 % of a
+// long decode.)
+__device__ __forceinline__ bool copied(uint32_t bar, uint32_t parity, uint32_t polls)
+{
+    for (uint32_t it = 0; it < polls; it++) {
+        uint32_t done;
+        asm volatile(
+            "{\n.reg .pred p;\n"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+            "selp.u32 %0, 1, 0, p;\n}\n"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+    }
+    return false;
+}
+
 // the segment that starts at flat tile t: its unit's tiles [first, last) within hi
 __device__ __forceinline__ void find_segment(const AttnArgs &g, const int32_t *prefix, int t, int hi, Segment &s)
 {
@@ -93,10 +112,14 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     uint64_t *full = reinterpret_cast<uint64_t *>(ml + C::ML / 8) + warp * C::STAGES;
     int32_t *prefix = reinterpret_cast<int32_t *>(reinterpret_cast<uint64_t *>(ml + C::ML / 8) + SP_WARPS * C::STAGES);
     __shared__ int32_t wsum[SP_WARPS];
+    __shared__ uint32_t out_of_time;      // a wait for a copy has run out
 
     if (lane == 0)
         for (int i = 0; i < C::STAGES; i++) mbar_init(full + i, 1);
-    if (threadIdx.x == 0) prefix[0] = 0;
+    if (threadIdx.x == 0) {
+        prefix[0] = 0;
+        out_of_time = 0;
+    }
     fence_barrier_init();
     pdl_trigger();
     pdl_wait();
@@ -161,6 +184,9 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     // ---- fetching: the warp's tokens of tile after tile, C::STAGES ahead of their use.  The pages of the next fetch are looked up
     // one fetch early.  Pages of 32 tokens and more: four copies (codes and scales, keys and values), by a lane each; pages of 16:
     // two of a whole (page, head) block.  What a lane copies, and to where, is the same for every tile.
+    //
+    // A lane whose wait has run out (SP_LATE in its f_stage) copies, arms and waits no more: arming a barrier whose phase is incomplete is
+    // undefined.  It goes on through the instructions of its warp, with whatever the stages hold; the host reads the error.
     const int shift = 31 - __clz(g.page), copies = shift == 4 ? 2 : 4;
     const uint32_t block_bytes = (uint32_t)g.page * 2 * RB, page_bytes = block_bytes * g.kv_heads, num_pages = (uint32_t)min(g.num_pages, (int64_t)0x7FFFFFFF);
     const uint32_t in_page = (warp * SP_WTOK) & (g.page - 1), scales_of = lane & 1;
@@ -169,6 +195,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     const uint32_t lane_bytes = shift == 4 ? C::TILE / 2 : scales_of ? SP_WTOK * D / 16 : SP_WTOK * D / 2;
     const uint32_t bar0 = smem_u32(full);
     int f_t = lo, f_left = 0, f_tok = 0, f_L = 0, f_page = -1;      // next segment; tiles left of this one; this lane's first token, and its page
+    constexpr uint32_t SP_LATE = 1u << 31;
     uint32_t f_stage = 0;
     const int32_t *f_row = nullptr;
     const uint8_t *f_base = nullptr;
@@ -190,10 +217,10 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     };
     const auto fetch = [&]() {
         if (f_left <= 0) return;
-        const bool ok = (uint32_t)f_page < num_pages;
-        if (!ok && lane < copies && f_tok < f_L) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
+        const bool on_time = !(f_stage & SP_LATE), ok = (uint32_t)f_page < num_pages && on_time;
+        if ((uint32_t)f_page >= num_pages && lane < copies && f_tok < f_L) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
         const uint32_t bytes = __popc(__ballot_sync(0xFFFFFFFFu, ok)) * (shift == 4 ? C::TILE / 2 : C::TILE / 4), bar = bar0 + f_stage * 8;
-        if (lane == 0) mbar_expect_at(bar, bytes);
+        if (lane == 0 && on_time) mbar_expect_at(bar, bytes);
         __syncwarp();
         if (ok) bulk_load_at(lane_dst + f_stage * C::TILE, f_base + (uint64_t)(uint32_t)f_page * page_bytes, lane_bytes, bar);
         f_stage = f_stage + 1 == C::STAGES ? 0 : f_stage + 1;
@@ -422,7 +449,11 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         const int clear = s.L - s.n + 1;      // keys that every row sees
 
         for (int tile = s.first; tile < end; tile++) {
-            mbar_wait_addr(bar0 + stage * 8, phase, KV_ATTN_ERR);
+            if (!copied(bar0 + stage * 8, phase, f_stage & SP_LATE ? 0 : 1u << 24)) {
+                f_stage |= SP_LATE;
+                out_of_time = 1;
+                atomicMax(&g_qcc_error, KV_ATTN_ERR);
+            }
             const int tok = tile * SP_TOK + warp * SP_WTOK;
             if (tok + SP_WTOK <= clear) step(std::false_type(), tok);
             else if (tok < s.L) step(std::true_type(), tok);
@@ -500,6 +531,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         }
         t += s.last - s.first;
     }
+    settle(smem_u32(&out_of_time));      // (the last unit ended with a barrier)
 }
 
 template <int D, int NT>

@@ -35,3 +35,17 @@ def test_no_barrier_is_armed_behind_a_wait_that_ran_out(name):
     assert loops
     for body in loops:
         assert "mbar_reached(" in body and "mbar_wait_at(" not in body and "break;" in body
+
+
+def test_few_queries_a_lane_whose_wait_ran_out_stops_copying():
+    """kv_attention.cu arms and copies in fetch(), both only in lanes whose waits were met; and a CTA settles behind its last unit."""
+    text = source("kv_attention.cu")
+    assert "mbar_wait" not in text
+    fetch = text[text.index("const auto fetch"):text.index("seek();", text.index("const auto fetch"))]
+    assert "on_time = !(f_stage & SP_LATE)" in fetch
+    assert re.findall(r"if \(([^\n]*)\) mbar_expect_at\(", text) == ["lane == 0 && on_time"]
+    assert re.findall(r"if \(([^\n]*)\) bulk_load_at\(", text) == ["ok"] and "num_pages && on_time;" in fetch
+    waits = re.findall(r"if \(!copied\(.*?\n            \}", text, re.S)
+    assert len(waits) == len(re.findall(r"\bcopied\(", text)) - 1 == 1 and "f_stage |= SP_LATE;" in waits[0] and "out_of_time = 1;" in waits[0]
+    end = text.index("settle(smem")
+    assert text.rindex("named_barrier(", 0, end) > text.rindex("fetch()", 0, end)
