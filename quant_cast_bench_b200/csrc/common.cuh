@@ -526,6 +526,21 @@ __device__ __forceinline__ uint4 ld_nc_v4(const void *p)
                  : "l"(p));
     return r;
 }
+// The same by the coherent path.  The non-coherent one (ld.global.nc, __ldg, const __restrict__) is for data that nothing writes
+// while the kernel lives; a kernel launched under a predecessor that still writes it (see pdl_wait) reads what that wrote by plain loads.
+__device__ __forceinline__ uint4 ld_once_v4(const void *p)
+{
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+    return r;
+}
+// a 4-byte number by the coherent path
+__device__ __forceinline__ int32_t ld_i32(const int32_t *p)
+{
+    int32_t r;
+    asm volatile("ld.global.s32 %0, [%1];" : "=r"(r) : "l"(p));
+    return r;
+}
 // 16-byte load that allocates in L1: for threads that read several neighbouring 16-byte pieces of the
 // same sectors with separate instructions (measured +9 % on the 64-bytes-per-thread streams)
 __device__ __forceinline__ uint4 ld_v4(const void *p)

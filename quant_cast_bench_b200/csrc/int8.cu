@@ -45,8 +45,8 @@ __device__ __forceinline__ uint32_t int8x4(uint32_t w0, uint32_t w1, float inv)
 // One CTA per row.  The row stays in registers (CH 16-byte pieces a thread) between its maximum and the cast, so x is read
 // once; CH = 0: rows too long for that, or not a multiple of 8 elements, are read twice (the second time from L2).
 template <int CH>
-__global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t *__restrict__ x, int64_t N, uint8_t *__restrict__ q,
-                                                                  float *__restrict__ scale, int recip_div)
+__global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t *x, int64_t N, uint8_t *q,
+                                                                  float *scale, int recip_div)
 {
     pdl_trigger();
     pdl_wait();
@@ -60,7 +60,7 @@ __global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t
 #pragma unroll
         for (int c = 0; c < CH; c++) {
             const int64_t k = threadIdx.x + (int64_t)c * I8_THREADS;
-            v[c] = k < nchunk ? ld_nc_v4(reinterpret_cast<const uint4 *>(xr) + k) : make_uint4(0, 0, 0, 0);
+            v[c] = k < nchunk ? ld_once_v4(reinterpret_cast<const uint4 *>(xr) + k) : make_uint4(0, 0, 0, 0);
         }
 #pragma unroll
         for (int c = 0; c < CH; c++) acc = absmax2_nan(absmax2_nan(absmax2_nan(absmax2_nan(acc, v[c].x), v[c].y), v[c].z), v[c].w);

@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
         }
     }
     if (g.cu_q) {
-        const int64_t first = max(__ldg(g.cu_q + g.seqs), 0);
+        const int64_t first = max(g.cu_q[g.seqs], 0);
         fill_rows<D>(g, first, g.rows - first, blockIdx.x, gridDim.x);
     }
     if ((int)blockIdx.x >= ctas) {
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
             f_row = g.table + s.b * g.table_stride + (f_tok >> shift);
             f_base = g.cache + s.head * (int64_t)block_bytes + lane_src;
         }
-        f_page = f_left > 0 && lane < copies && f_tok < f_L ? __ldg(f_row) : -1;
+        f_page = f_left > 0 && lane < copies && f_tok < f_L ? ld_i32(f_row) : -1;
     };
     const auto fetch = [&]() {
         if (f_left <= 0) return;
@@ -235,7 +235,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
 
     // ---- 32 tokens of every tile each
     const int gr = lane >> 2, c = lane & 3;
-    const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
+    const float k_outer = ld_cg_f32(g.k_outer), v_outer = ld_cg_f32(g.v_outer);
     uint32_t stage = 0, phase = 0;
     for (int t = lo; t < hi;) {
         Segment s;

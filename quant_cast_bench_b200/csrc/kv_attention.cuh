@@ -85,8 +85,8 @@ __device__ __forceinline__ void bulk_load_at(uint32_t dst, const void *src, uint
 __device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n, int &L)
 {
     if (g.cu_q) {
-        q0 = __ldg(g.cu_q + b);
-        const int64_t end = __ldg(g.cu_q + b + 1), count = end - q0;      // (64 bits: the offsets may be anything)
+        q0 = ld_i32(g.cu_q + b);
+        const int64_t end = ld_i32(g.cu_q + b + 1), count = end - q0;      // (64 bits: the offsets may be anything)
         n = (int)count;
         if (q0 < 0 || count < 0 || count > g.max_q || end > g.rows) {
             atomicMax(&g_qcc_error, QCC_DEVERR_QUERIES);
@@ -97,7 +97,7 @@ __device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n
         q0 = b;
         n = 1;
     }
-    L = max(__ldg(g.kv_lens + b), 0);
+    L = max(ld_i32(g.kv_lens + b), 0);
     if (L > (int64_t)g.width * g.page) {
         atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
         L = g.width * g.page;
@@ -149,7 +149,7 @@ __global__ void __launch_bounds__(THREADS) kv_join_kernel(const AttnArgs g, int 
     pdl_wait();
     const int c = blockIdx.x;
     const int4 s0 = g.seams[2 * c], s1 = g.seams[2 * c + 1];
-    const float v_outer = __ldg(g.v_outer);
+    const float v_outer = *g.v_outer;
     if (s0.x < 0) return;
     const int total = s0.z, ctas = min(grid, total), i0 = owner_of(s0.x, ctas, total);
     if (i0 != c - 1) return;

@@ -115,12 +115,12 @@ __device__ __forceinline__ void append_rows(const AppendArgs &g, float *lut, int
         }
         const bool second = live && (KV || 2 * it.part + 1 < g.q_heads);
         const uint4 none = make_uint4(0, 0, 0, 0);
-        it.x[0][0] = live ? ld_nc_v4(p0 + 8 * ca) : none;
-        it.x[0][1] = live ? ld_nc_v4(p0 + 8 * cb) : none;
-        it.x[1][0] = second ? ld_nc_v4(p1 + 8 * ca) : none;
-        it.x[1][1] = second ? ld_nc_v4(p1 + 8 * cb) : none;
-        it.slot = live ? __ldg(g.slots + it.token) : -1;
-        it.pos = live && g.rot > 0 ? __ldg(g.positions + it.token) : 0;
+        it.x[0][0] = live ? ld_once_v4(p0 + 8 * ca) : none;
+        it.x[0][1] = live ? ld_once_v4(p0 + 8 * cb) : none;
+        it.x[1][0] = second ? ld_once_v4(p1 + 8 * ca) : none;
+        it.x[1][1] = second ? ld_once_v4(p1 + 8 * cb) : none;
+        it.slot = live ? g.slots[it.token] : -1;
+        it.pos = live && g.rot > 0 ? g.positions[it.token] : 0;
     };
     const int64_t stride = (int64_t)blocks * GROUPS, first = (int64_t)block * GROUPS + threadIdx.x / TPR, d_token = stride / per_token;
     const int d_part = (int)(stride - d_token * per_token);
@@ -129,8 +129,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs &g, float *lut, int
     load(next);
     float k_outer = 1.0f, v_outer = 1.0f;
     if (KV) {
-        k_outer = __ldg(g.k_outer);
-        v_outer = __ldg(g.v_outer);
+        k_outer = *g.k_outer;
+        v_outer = *g.v_outer;
         nvfp4_fill_recip_lut(lut, __fdiv_rn(1.0f, k_outer));
         nvfp4_fill_recip_lut(lut + 128, __fdiv_rn(1.0f, v_outer));
         __syncthreads();
@@ -152,8 +152,8 @@ __device__ __forceinline__ void append_rows(const AppendArgs &g, float *lut, int
             const float *cs = g.cos_sin + (live && placed ? cur.pos : 0) * g.rot;
             const int half = g.rot / 2, at = turn_halves ? 8 * t : 4 * ca, more = turn_halves ? 4 : 4 * (cb - ca);
             const bool both = turn_halves || turn_b;
-            const float4 c0 = __ldg(reinterpret_cast<const float4 *>(cs + at)), s0 = __ldg(reinterpret_cast<const float4 *>(cs + half + at));
-            const float4 c1 = both ? __ldg(reinterpret_cast<const float4 *>(cs + at + more)) : c0, s1 = both ? __ldg(reinterpret_cast<const float4 *>(cs + half + at + more)) : s0;
+            const float4 c0 = *reinterpret_cast<const float4 *>(cs + at), s0 = *reinterpret_cast<const float4 *>(cs + half + at);
+            const float4 c1 = both ? *reinterpret_cast<const float4 *>(cs + at + more) : c0, s1 = both ? *reinterpret_cast<const float4 *>(cs + half + at + more) : s0;
             c[0] = c0.x; c[1] = c0.y; c[2] = c0.z; c[3] = c0.w; c[4] = c1.x; c[5] = c1.y; c[6] = c1.z; c[7] = c1.w;
             s[0] = s0.x; s[1] = s0.y; s[2] = s0.z; s[3] = s0.w; s[4] = s1.x; s[5] = s1.y; s[6] = s1.z; s[7] = s1.w;
         }
@@ -251,19 +251,20 @@ __global__ void __launch_bounds__(KV_THREADS) kv_gather_kernel(const GatherArgs 
     const int64_t row = (int64_t)blockIdx.x * TOKENS + threadIdx.x / TPR;
     const int head = blockIdx.y;
     if (row >= g.total) return;
+    const float outer[2] = {*g.k_outer, *g.v_outer};
     // sequence of the row: the last b with cu[b] <= row
     int lo = 0, hi = g.seqs;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(g.cu + mid) <= row) lo = mid; else hi = mid - 1;
+        if (g.cu[mid] <= row) lo = mid; else hi = mid - 1;
     }
     const int side = g.page * kv_row_bytes<D>();
     const uint8_t *base = nullptr;
     int off = 0;
-    if (lo < g.seqs && row >= __ldg(g.cu)) {
+    if (lo < g.seqs && row >= *g.cu) {
         const int shift = 31 - __clz(g.page);
-        const int64_t i = row - __ldg(g.cu + lo), pi = i >> shift;
-        const int64_t pg = pi < g.width ? __ldg(g.table + lo * g.table_stride + pi) : -1;
+        const int64_t i = row - g.cu[lo], pi = i >> shift;
+        const int64_t pg = pi < g.width ? g.table[lo * g.table_stride + pi] : -1;
         off = (int)(i & (g.page - 1));
         if (pg < 0 || pg >= g.num_pages) atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
         else base = g.cache + (pg * g.kv_heads + head) * (int64_t)(2 * side);
@@ -275,14 +276,13 @@ __global__ void __launch_bounds__(KV_THREADS) kv_gather_kernel(const GatherArgs 
 #pragma unroll
             for (int c = 0; c < 2; c++) {
                 const uint8_t *p = base + w * side;
-                codes[w][c] = __ldg(reinterpret_cast<const uint32_t *>(p + off * kv_row_codes<D>()) + t + c * TPR);
-                scales[w][c] = __ldg(p + g.page * kv_row_codes<D>() + off * kv_row_scales<D>() + ((t + c * TPR) >> 1));
+                codes[w][c] = reinterpret_cast<const uint32_t *>(p + off * kv_row_codes<D>())[t + c * TPR];
+                scales[w][c] = p[g.page * kv_row_codes<D>() + off * kv_row_scales<D>() + ((t + c * TPR) >> 1)];
             }
     }
     const size_t at = ((size_t)row * g.kv_heads + head) * D;
 #pragma unroll
     for (int w = 0; w < 2; w++) {
-        const float outer = __ldg(w ? g.v_outer : g.k_outer);
         uint4 *dst = reinterpret_cast<uint4 *>((w ? g.v : g.k) + at) + t;
 #pragma unroll
         for (int c = 0; c < 2; c++) {
@@ -293,7 +293,7 @@ __global__ void __launch_bounds__(KV_THREADS) kv_gather_kernel(const GatherArgs 
             for (int j = 0; j < 4; j++) {
                 const uint32_t p = hmul2_bits(v[j], sc);       // exact: 2 + 4 significant bits
                 const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&p));
-                const __nv_bfloat162 b = __floats2bfloat162_rn(__fmul_rn(f.x, outer), __fmul_rn(f.y, outer));
+                const __nv_bfloat162 b = __floats2bfloat162_rn(__fmul_rn(f.x, outer[w]), __fmul_rn(f.y, outer[w]));
                 o[j] = base ? *reinterpret_cast<const uint32_t *>(&b) : 0;
             }
             dst[c * TPR] = make_uint4(o[0], o[1], o[2], o[3]);

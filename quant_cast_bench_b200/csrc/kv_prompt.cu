@@ -222,10 +222,10 @@ __device__ __noinline__ uint32_t nan_blocks(const AttnArgs &g, int b, int head, 
     uint32_t bits = 0;
     for (int t = from; t < to; t++) {
         const int p = t / g.page, off = t - p * g.page;
-        const int64_t pg = __ldg(g.table + b * g.table_stride + p);
+        const int64_t pg = ld_i32(g.table + b * g.table_stride + p);
         if (pg < 0 || pg >= g.num_pages) continue;
         const uint8_t *sc = g.cache + ((pg * g.kv_heads + head) * 2 + 1) * ((int64_t)g.page * kv_row_bytes<D>()) + g.page * (D / 2) + off * (D / 16);
-        for (int i = 0; i < D / 16; i++) bits |= (uint32_t)((__ldg(sc + i) & 0x7Fu) == 0x7Fu) << i;
+        for (int i = 0; i < D / 16; i++) bits |= (uint32_t)((sc[i] & 0x7Fu) == 0x7Fu) << i;
     }
     return bits;
 }
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         }
     }
     if (g.cu_q) {
-        const int64_t first = max(__ldg(g.cu_q + g.seqs), 0);
+        const int64_t first = max(g.cu_q[g.seqs], 0);
         fill_rows<D>(g, first, g.rows - first, blockIdx.x, gridDim.x);
     }
     if ((int)blockIdx.x >= ctas) {
@@ -344,7 +344,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     const int p = tile * pages + lane;
                     int64_t pg = -1;
                     if (lane < pages && p < have) {
-                        pg = __ldg(row + p);
+                        pg = ld_i32(row + p);
                         if (pg < 0 || pg >= g.num_pages) {
                             atomicMax(&g_qcc_error, QCC_DEVERR_PAGE);
                             pg = -1;
@@ -540,7 +540,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         // ---- softmax of row tile x, one thread a row
         const int x = (warp - 8) >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21, t_s = tmem + lanes + x * 128, t_o = tmem + lanes + 256 + x * 128;
-        const float k_outer = __ldg(g.k_outer), v_outer = __ldg(g.v_outer);
+        const float k_outer = *g.k_outer, v_outer = *g.v_outer;
         uint32_t sn = 0, on = 0;        // scores, products so far
         float factor = 0.0f;
         bool placed = false;            // q of the part is in place already

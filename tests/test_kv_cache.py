@@ -792,3 +792,65 @@ def test_a_flat_tail_keeps_its_weight_beside_dominant_keys(D, hq, q_len, every, 
     err = (out.cpu().double() - o).abs()
     assert bool((err <= tol * 1.01).all()), f"off by {float((err / o).max())} of the tail, {float((tol / o).max())} allowed"
     assert bool(((lse.cpu().double() - z).abs() <= ltol).all()) and L.device_error() == 0
+
+
+@pytest.mark.parametrize("name", ["int8.cu", "kv_cache.cuh", "kv_cache.cu", "kv_attention.cuh", "kv_attention.cu", "kv_prompt.cu"])
+def test_overlapped_kernels_load_by_the_coherent_path(name):
+    """These kernels start under their predecessor, which may still write what they read: no load that takes its data for constant."""
+    import os
+    import re
+    with open(os.path.join(os.path.dirname(L.LIB_PATH), "..", "csrc", name)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    assert not re.findall(r"__ldg\b|ld_nc_v4|\.nc\b|__restrict__", text)
+
+
+@gpu
+@pytest.mark.parametrize("captured", [False, True])
+def test_steps_in_a_row_read_what_the_last_one_wrote(captured):
+    """A projection into one buffer, an append to the same slots, a read-back and an attention, twelve times without a synchronisation
+    between: each step sees the keys and values of its own."""
+    D, page, heads, qh, tokens, steps = 128, 16, 2, 8, 48, 12
+    g = torch.Generator().manual_seed(6)
+    w, ws = Q.rowwise_int8_cuda(torch.randn((qh + 2 * heads) * D, 256, generator=g).to(torch.bfloat16).cuda())
+    x = torch.randn(steps, tokens, 256, generator=g).to(torch.bfloat16).cuda()
+    rope, slots, pos = rotation_table(tokens, D).cuda(), torch.randperm(tokens, generator=g).cuda(), torch.arange(tokens).cuda()
+    one = torch.tensor([0.02]).cuda()
+    table = torch.tensor([[2, 0, 1]], dtype=torch.int32).cuda()
+    cu, n = torch.tensor([0, tokens], dtype=torch.int32).cuda(), torch.tensor([tokens], dtype=torch.int32).cuda()
+
+    def run(cache, synchronise):
+        got = []
+        for i in range(steps):
+            calls = []
+            for call in range(5):
+                if call == 0:
+                    calls.append(Q.rowwise_int8_cuda(x[i]))
+                elif call == 1:
+                    calls.append(Q.int8_scaled_mm_cuda(calls[0][0], w, calls[0][1], ws).view(tokens, qh + 2 * heads, D))
+                elif call == 2:
+                    q, k, v = calls[1].split([qh, heads, heads], 1)
+                    calls.append(Q.nvfp4_kv_append_cuda(k, v, cache, slots, one, one, positions=pos, cos_sin=rope, q=q))
+                elif call == 3:
+                    calls.append(Q.nvfp4_kv_gather_cuda(cache, table, cu, tokens, D, one, one))
+                else:
+                    calls.append(Q.nvfp4_kv_attention_cuda(calls[2], cache, table, n, one, one, cu_q=cu, max_q=tokens) if i % 2 else
+                                 Q.nvfp4_kv_attention_cuda(calls[2][-1:], cache, table, n, one, one))
+                if synchronise:
+                    torch.cuda.synchronize()
+            got += [calls[2], *calls[3], *calls[4]]
+        return got
+    want = run(torch.zeros(3, heads, 2, page * 72, dtype=torch.uint8, device="cuda"), True)
+    cache = torch.zeros(3, heads, 2, page * 72, dtype=torch.uint8, device="cuda")
+    if captured:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(cache, False)
+        graph.replay()
+        graph.replay()
+    else:
+        got = run(cache, False)
+    torch.cuda.synchronize()
+    assert not any(torch.equal(a, b) for a, b in zip(got[:-5], got[5:]))        # the steps do differ
+    for a, b in zip(got, want):
+        assert torch.equal(a, b)
+    assert L.device_error() == 0
