@@ -512,10 +512,13 @@ std::tuple<at::Tensor, at::Tensor> nvfp4_kv_gather_cuda(const at::Tensor &cache,
     return {k, v};
 }
 
+void check_scale(const std::optional<double> &scale) { TORCH_CHECK(!scale || *scale > 0, "quant_cast_cuda: scale must be positive, got ", *scale); }
+
 std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_cuda(const at::Tensor &q, const at::Tensor &cache, const at::Tensor &block_table, const at::Tensor &kv_lens,
                                                            const at::Tensor &k_outer, const at::Tensor &v_outer, const std::optional<at::Tensor> &cu_q,
-                                                           int64_t max_q, double scale)
+                                                           int64_t max_q, std::optional<double> scale)
 {
+    check_scale(scale);
     TORCH_CHECK(q.dim() == 3, "quant_cast_cuda: q must be (rows, q_heads, head_dim)");
     const int64_t rows = q.size(0), hq = q.size(1), D = q.size(2), seqs = block_table.size(0);
     const CacheShape c = check_cache(cache, D);
@@ -554,7 +557,7 @@ std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_cuda(const at::Tensor &q, 
     a.cu_q = cu_q ? cu_q->data_ptr<int32_t>() : nullptr;
     a.seqs = (int)std::min<int64_t>(seqs, 1 << 20);
     a.max_q = (int)max_q;
-    a.scale = scale > 0 ? (float)scale : (float)(1.0 / std::sqrt((double)D));
+    a.scale = (float)(scale ? *scale : 1.0 / std::sqrt((double)D));
     a.q_heads = (int)hq;
     a.kv_heads = c.heads;
     a.head_dim = (int)D;
@@ -694,8 +697,9 @@ std::tuple<at::Tensor, at::Tensor> nvfp4_kv_gather_meta(const at::Tensor &cache,
     return {like(cache, {total, cache.size(1), head_dim}, at::kBFloat16), like(cache, {total, cache.size(1), head_dim}, at::kBFloat16)};
 }
 std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_meta(const at::Tensor &q, const at::Tensor &, const at::Tensor &, const at::Tensor &, const at::Tensor &,
-                                                           const at::Tensor &, const std::optional<at::Tensor> &, int64_t, double)
+                                                           const at::Tensor &, const std::optional<at::Tensor> &, int64_t, std::optional<double> scale)
 {
+    check_scale(scale);
     TORCH_CHECK(q.dim() == 3, "quant_cast_cuda: q must be (rows, q_heads, head_dim)");
     return {like(q, q.sizes().vec(), at::kBFloat16), like(q, {q.size(0), q.size(1)}, at::kFloat)};
 }
@@ -725,7 +729,7 @@ TORCH_LIBRARY(quant_cast_cuda_native, m)
           "Tensor? cos_sin=None, bool interleaved=False, Tensor? q=None, bool recip_div=False) -> Tensor");
     m.def("nvfp4_kv_gather(Tensor cache, Tensor block_table, Tensor cu_kv, int total, int head_dim, Tensor k_outer, Tensor v_outer) -> (Tensor, Tensor)");
     m.def("nvfp4_kv_attention(Tensor q, Tensor cache, Tensor block_table, Tensor kv_lens, Tensor k_outer, Tensor v_outer, Tensor? cu_q=None, "
-          "int max_q=1, float scale=0.) -> (Tensor, Tensor)");
+          "int max_q=1, float? scale=None) -> (Tensor, Tensor)");
     m.def("sr_f32_to_bf16(Tensor x, Tensor key, int global_row=0, int global_col=0, int num_col=-1) -> Tensor");
 }
 

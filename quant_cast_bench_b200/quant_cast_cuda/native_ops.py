@@ -182,7 +182,7 @@ def nvfp4_kv_gather_native(cache, block_table, cu_kv, total, head_dim, k_outer, 
 def nvfp4_kv_attention_native(q, cache, block_table, kv_lens, k_outer, v_outer, cu_q=None, max_q=None, scale=None):
     if scale is not None and not scale > 0:
         raise ValueError(f"scale must be positive, got {scale}")
-    return _kv_attention(q, cache, block_table, kv_lens, k_outer, v_outer, cu_q, max_q or 0 if cu_q is not None else 1, scale or 0.0)
+    return _kv_attention(q, cache, block_table, kv_lens, k_outer, v_outer, cu_q, max_q or 0 if cu_q is not None else 1, scale)
 
 
 # (gold function name in the golden vectors, operator-backed function, aux input): the other recipe families

@@ -854,3 +854,22 @@ def test_steps_in_a_row_read_what_the_last_one_wrote(captured):
     for a, b in zip(got, want):
         assert torch.equal(a, b)
     assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("device", ["meta", pytest.param("cuda", marks=gpu)])
+def test_the_registered_operator_refuses_a_scale_that_is_not_positive(device):
+    from quant_cast_bench_b200 import build as qbuild
+    qbuild.build_torch_binding()
+    from quant_cast_bench_b200.quant_cast_cuda import native_ops  # noqa: F401  (loads the operators)
+    op = torch.ops.quant_cast_cuda_native.nvfp4_kv_attention
+
+    def zeros(*shape, dtype=torch.bfloat16):
+        return torch.zeros(*shape, dtype=dtype, device=device)
+    o = zeros(1, dtype=torch.float32) + 1
+    args = (zeros(1, 4, 64), zeros(1, 2, 2, 16 * 36, dtype=torch.uint8), zeros(1, 1, dtype=torch.int32), zeros(1, dtype=torch.int32) + 3, o, o)
+    for scale in (0.0, -1.0, float("nan")):
+        with pytest.raises(RuntimeError, match="scale must be positive"):
+            op(*args, scale=scale)
+    assert all(a.shape == b.shape for a, b in zip(op(*args), op(*args, scale=0.125)))
+    if device == "cuda":
+        assert all(torch.equal(a, b) for a, b in zip(op(*args), op(*args, scale=0.125)))
