@@ -539,6 +539,8 @@ typedef struct qcc_kv_attention_args {
     float *lse;
 } qcc_kv_attention_args;
 size_t qcc_nvfp4_kv_attention_workspace_bytes(int64_t rows, int seqs, int max_q, int q_heads, int kv_heads, int head_dim);
+/* Kernels that a call with these (valid) arguments launches, on the current device: 0 to 3. */
+int qcc_nvfp4_kv_attention_launches(const qcc_kv_attention_args *args);
 int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *args, void *workspace, size_t workspace_bytes, void *stream);
 
 /* ---------------------------------------------------------------------------------------------

@@ -559,6 +559,14 @@ static int row_tiles_of(int64_t rows) { return rows <= 8 ? 1 : rows <= 16 ? 2 : 
 // 32 over 8000 247 against 246, with 64-element heads 57 against 81; 16 rows over 8000 tokens 79 against 144.  Only 32 rows over 100 tokens are
 // behind (19 against 15).
 static bool many_queries(int max_q, int group) { return (int64_t)max_q * group > 32; }
+// Units are dealt out whole, with nothing to join and one launch less, where the longest that the table allows is short, or where it is not long (16 tiles of
+// 8 rows) and there are enough of them for the GPU.  One sequence of 250 tokens 9.1 against 9.0 us and the launch, 64 of 1000 25.8 against 31.8, 150 of up to
+// 2000 73 against 82, 300 of up to 1000 86 against 94; the worst met, 80 of 1000 (640 units for 592 CTAs), 41 against 37.
+static bool dealt_out_whole(const qcc_kv_attention_args *p, int nt)
+{
+    const int64_t most = nt * (((int64_t)p->table_width * p->page + SP_TOK - 1) / SP_TOK);
+    return most <= 2 || (most <= 16 && (int64_t)p->seqs * p->kv_heads * 4 >= 3 * sm_count() * split_ctas(p->head_dim, nt));
+}
 
 }  // namespace qcc
 
@@ -572,6 +580,14 @@ extern "C" size_t qcc_nvfp4_kv_attention_workspace_bytes(int64_t rows, int seqs,
     if (many_queries(max_q, q_heads / kv_heads)) return prompt_workspace_bytes(rows, q_heads / kv_heads, seqs, head_dim);
     const int nt = row_tiles_of((int64_t)max_q * (q_heads / kv_heads));
     return (size_t)sm_count() * split_ctas(head_dim, nt) * 2 * (16 + nt * 8 * (head_dim + 2) * 4);
+}
+
+extern "C" int qcc_nvfp4_kv_attention_launches(const qcc_kv_attention_args *p)
+{
+    if (!p || p->kv_heads < 1 || p->seqs <= 0 || p->rows <= 0) return 0;
+    const int group = p->q_heads / p->kv_heads, max_q = p->cu_q ? p->max_q : 1;
+    if (many_queries(max_q, group)) return 3;
+    return dealt_out_whole(p, row_tiles_of((int64_t)max_q * group)) ? 1 : 2;
 }
 
 extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *workspace, size_t workspace_bytes, void *stream)
@@ -608,11 +624,7 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     g.scale_log2 = p->scale * LOG2E;
     g.seqs = p->seqs; g.width = p->table_width; g.q_heads = p->q_heads; g.kv_heads = p->kv_heads; g.group = group; g.page = p->page; g.max_q = max_q;
     g.wide = 0;
-    // Units are dealt out whole, with nothing to join and one launch less, where the longest that the table allows is short, or where it is not long (16 tiles of
-    // 8 rows) and there are enough of them for the GPU.  One sequence of 250 tokens 9.1 against 9.0 us and the launch, 64 of 1000 25.8 against 31.8, 150 of up to
-    // 2000 73 against 82, 300 of up to 1000 86 against 94; the worst met, 80 of 1000 (640 units for 592 CTAs), 41 against 37.
-    const int64_t most = nt * ((cached + SP_TOK - 1) / SP_TOK);
-    g.whole = most <= 2 || (most <= 16 && (int64_t)p->seqs * p->kv_heads * 4 >= 3 * sm_count() * split_ctas(p->head_dim, nt));
+    g.whole = dealt_out_whole(p, nt);
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     if (many_queries(max_q, group)) return prompt_launch(g, p->head_dim, workspace, st);
     if (p->head_dim == 128)

@@ -86,6 +86,7 @@ SIGNATURES = {
     "qcc_nvfp4_kv_append": (_int, [_vp, _vp]),
     "qcc_nvfp4_kv_gather": (_int, [_vp, _i64, _int, _int, _int, _vp, _i64, _int, _vp, _int, _i64, _vp, _vp, _vp, _vp, _vp]),
     "qcc_nvfp4_kv_attention_workspace_bytes": (_sz, [_i64, _int, _int, _int, _int, _int]),
+    "qcc_nvfp4_kv_attention_launches": (_int, [_vp]),
     "qcc_nvfp4_kv_attention": (_int, [_vp, _vp, _sz, _vp]),
     "qcc_hadamard_rht": (_int, [_vp, _i64, _i64, _vp, _vp, _vp]),
     "qcc_nvfp4_rht_amax": (_int, [_vp, _i64, _i64, _vp, _int, _vp, _vp]),

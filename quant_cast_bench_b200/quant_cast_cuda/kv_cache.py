@@ -159,5 +159,5 @@ def nvfp4_kv_attention_cuda(q, cache, block_table, kv_lens, k_outer, v_outer, cu
         nws = lib.qcc_nvfp4_kv_attention_workspace_bytes(rows, seqs, max_q, hq, heads, D)
         ws = torch.empty(nws, dtype=torch.uint8, device=q.device)
         L.check(lib.qcc_nvfp4_kv_attention(ctypes.byref(a), _p(ws), nws, _stream(q)), "nvfp4_kv_attention")
-    L.launch_count += 2 if max_q * (hq // heads) <= 32 else 3
+        L.launch_count += lib.qcc_nvfp4_kv_attention_launches(ctypes.byref(a))
     return out, lse

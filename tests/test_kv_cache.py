@@ -873,3 +873,21 @@ def test_the_registered_operator_refuses_a_scale_that_is_not_positive(device):
     assert all(a.shape == b.shape for a, b in zip(op(*args), op(*args, scale=0.125)))
     if device == "cuda":
         assert all(torch.equal(a, b) for a, b in zip(op(*args), op(*args, scale=0.125)))
+
+
+@gpu
+@pytest.mark.parametrize("lens,q_lens,hq", [([100, 30], None, 4), ([300] * 300, None, 4), ([5000, 20], None, 4), ([5000, 20], [8, 3], 4), ([200, 90], [70, 4], 4), ([200], None, 80)])
+def test_launch_count_is_what_a_call_launches(lens, q_lens, hq):
+    """The binding's counter against the kernels of the captured call: units dealt out whole, joined, many queries."""
+    import ctypes
+    ql = q_lens or [1] * len(lens)
+    q, cache, _, table, ko, vo = (t.cuda() for t in attention_case(64, 16, hq, 2, lens, ql, poison=False))
+    kw = {} if q_lens is None else dict(cu_q=torch.tensor([0] + ql).cumsum(0).to(torch.int32).cuda(), max_q=max(ql))
+    n = torch.tensor(lens, dtype=torch.int32).cuda()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    before = L.launch_count
+    with torch.cuda.graph(graph):
+        Q.nvfp4_kv_attention_cuda(q, cache, table, n, ko, vo, **kw)
+    count = ctypes.c_size_t(0)
+    assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(count)) == 0
+    assert L.launch_count - before == count.value
