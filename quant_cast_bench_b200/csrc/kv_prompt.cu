@@ -69,13 +69,15 @@ __device__ __forceinline__ int prompt_tiles(int n, int L, int qt, int group)
 // the first of them that its first row does not see whole
 __device__ __forceinline__ int prompt_clear(int n, int L, int qt, int group) { return max(L - n + (int)((int64_t)qt * PT_ROWS / group) + 1, 0) / PT_TOK; }
 
+// Sums of numbers that are not negative, 2^31 - 1 at most.  (Offsets that overlap, an error of the caller, can claim more pairs than that.)
+__device__ __forceinline__ int sum_limited(int a, int b) { return (int)min((uint32_t)a + (uint32_t)b, 0x7FFFFFFFu); }
 __device__ __forceinline__ int block_scan(int v, int32_t *wsum, int &all)     // inclusive; 1024 threads
 {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int u = __shfl_up_sync(0xFFFFFFFFu, v, o);
-        if (lane >= o) v += u;
+        if (lane >= o) v = sum_limited(v, u);
     }
     if (lane == 31) wsum[warp] = v;
     __syncthreads();
@@ -84,13 +86,13 @@ __device__ __forceinline__ int block_scan(int v, int32_t *wsum, int &all)     //
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int x = __shfl_up_sync(0xFFFFFFFFu, u, o);
-            if (lane >= o) u += x;
+            if (lane >= o) u = sum_limited(u, x);
         }
         wsum[lane] = u;
     }
     __syncthreads();
     all = wsum[31];
-    const int r = v + (warp ? wsum[warp - 1] : 0);
+    const int r = sum_limited(v, warp ? wsum[warp - 1] : 0);
     __syncthreads();
     return r;
 }
@@ -105,9 +107,9 @@ __global__ void __launch_bounds__(1024) kv_prompt_plan_kernel(const AttnArgs g, 
         const int b = b0 + threadIdx.x;
         int q0, n = 0, L, all;
         if (b < g.seqs) seq_of(g, b, q0, n, L);
-        const int v = block_scan((int)(((int64_t)n * g.group + PT_ROWS - 1) / PT_ROWS), wsum, all);
-        if (b < g.seqs) start[b + 1] = carry + v;
-        carry += all;
+        const int v = block_scan((int)min(((int64_t)n * g.group + PT_ROWS - 1) / PT_ROWS, (int64_t)0x7FFFFFFF), wsum, all);
+        if (b < g.seqs) start[b + 1] = sum_limited(carry, v);
+        carry = sum_limited(carry, all);
     }
     if (threadIdx.x == 0) start[0] = 0;
     __syncthreads();

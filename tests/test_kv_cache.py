@@ -891,3 +891,23 @@ def test_launch_count_is_what_a_call_launches(lens, q_lens, hq):
     count = ctypes.c_size_t(0)
     assert ctypes.CDLL("libcudart.so.12").cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(count)) == 0
     assert L.launch_count - before == count.value
+
+
+@gpu
+def test_overlapping_offsets_that_claim_more_rows_than_31_bits_number():
+    """Every second sequence claims all rows of q, the others' offsets descend: 2048 times 2^20 and one blocks of 256 rows, which a 32-bit sum cannot
+    hold.  The offsets are reported; all sequences are empty, so every row is zero."""
+    rows, hq, D, seqs = (1 << 22) + 4, 64, 64, 4096
+    assert seqs // 2 * -(-rows * hq // 256) > 1 << 31
+    if torch.cuda.mem_get_info()[0] < 60 << 30:
+        pytest.skip("36 GB of results")
+    q = torch.zeros(1, 1, D, dtype=torch.bfloat16, device="cuda").expand(rows, hq, D)
+    cache, one = Q.nvfp4_kv_cache_cuda(1, 1, 16, D), torch.ones(1, device="cuda")
+    cu = (torch.arange(seqs + 1, device="cuda") % 2 * rows).to(torch.int32)
+    L.device_error()
+    out, lse = Q.nvfp4_kv_attention_cuda(q, cache, torch.zeros(seqs, 1, dtype=torch.int32, device="cuda"), torch.zeros(seqs, dtype=torch.int32, device="cuda"),
+                                         one, one, cu_q=cu, max_q=rows)
+    assert L.device_error() == 22
+    assert out.view(torch.int16).amax() == 0 and out.view(torch.int16).amin() == 0 and lse.amax() == -math.inf
+    del out, lse
+    torch.cuda.empty_cache()
