@@ -531,7 +531,8 @@ std::tuple<at::Tensor, at::Tensor> nvfp4_kv_attention_cuda(const at::Tensor &q, 
     a.v_outer = outer_of(v_outer, cache, "v_outer");
     if (cu_q) {
         check_numbers(*cu_q, at::kInt, seqs + 1, cache, "cu_q");
-        TORCH_CHECK(max_q >= 1 && max_q <= 0x7FFFFFFF, "quant_cast_cuda: cu_q needs max_q >= 1");
+        TORCH_CHECK(max_q >= 1, "quant_cast_cuda: cu_q needs max_q >= 1");
+        max_q = std::min<int64_t>(max_q, 0x7FFFFFFF);
     } else {
         TORCH_CHECK(rows == seqs, "quant_cast_cuda: ", rows, " query rows for ", seqs, " sequences: several queries a sequence need cu_q");
         max_q = 1;

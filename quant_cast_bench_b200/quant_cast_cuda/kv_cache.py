@@ -146,6 +146,7 @@ def nvfp4_kv_attention_cuda(q, cache, block_table, kv_lens, k_outer, v_outer, cu
     else:
         _check_numbers(cu_q, "cu_q", torch.int32, (seqs + 1,), cache)
         assert max_q is not None and max_q >= 1, "cu_q needs max_q"
+        max_q = min(max_q, 0x7FFFFFFF)      # (more rows than that there are not; a C int)
     if scale is not None and not scale > 0:
         raise ValueError(f"scale must be positive, got {scale}")
     out = torch.empty((rows, hq, D), dtype=torch.bfloat16, device=q.device)

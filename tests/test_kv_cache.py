@@ -911,3 +911,26 @@ def test_overlapping_offsets_that_claim_more_rows_than_31_bits_number():
     assert out.view(torch.int16).amax() == 0 and out.view(torch.int16).amin() == 0 and lse.amax() == -math.inf
     del out, lse
     torch.cuda.empty_cache()
+
+
+@gpu
+def test_max_q_may_be_any_bound():
+    """max_q is at least the most queries of a sequence: numbers that a C int does not hold among them."""
+    import sys
+    from quant_cast_bench_b200 import build as qbuild
+    qbuild.build_torch_binding()
+    from quant_cast_bench_b200.quant_cast_cuda import native_ops as N
+    lens, q_lens = [100, 30], [30, 20]
+    q, cache, _, table, ko, vo = (t.cuda() for t in attention_case(64, 16, 4, 2, lens, q_lens, poison=False))
+    args = (q, cache, table, torch.tensor(lens, dtype=torch.int32).cuda(), ko, vo)
+    cu = torch.tensor([0, 30, 50], dtype=torch.int32).cuda()
+    want = Q.nvfp4_kv_attention_cuda(*args, cu_q=cu, max_q=30)
+    for fn in (Q.nvfp4_kv_attention_cuda, N.nvfp4_kv_attention_native):
+        for max_q in (2 ** 31 - 1, 2 ** 31, 2 ** 32 + 1, sys.maxsize):
+            out, lse = fn(*args, cu_q=cu, max_q=max_q)
+            assert L.device_error() == 0 and torch.equal(out, want[0]) and torch.equal(lse, want[1]), (fn, max_q)
+    for max_q in (0, -5):
+        with pytest.raises((AssertionError, RuntimeError)):
+            Q.nvfp4_kv_attention_cuda(*args, cu_q=cu, max_q=max_q)
+        with pytest.raises((AssertionError, RuntimeError)):
+            N.nvfp4_kv_attention_native(*args, cu_q=cu, max_q=max_q)
