@@ -464,7 +464,8 @@ int qcc_nvfp4_both(const void *x, int64_t M, int64_t N, const float *outer, int 
  * head: the e2m1 codes of its tokens, (page, head_dim / 2) bytes with the even element in the low nibble, then their e4m3
  * block scales, (page, head_dim / 16) bytes.  value = code * scale * outer, with one fp32 outer scale for keys and one for
  * values (device; finite and > 0).  head_dim 64 or 128; page 16, 32, 64 or 128 tokens.  Nothing needs to be initialised:
- * a slot is read only once a sequence's length says that it holds a token.
+ * a slot is read only once a sequence's length says that it holds a token.  cache may be NULL where num_pages is 0, and a table
+ * where it has no entries: sequences without tokens need neither.
  *
  * Sequences are rows of a block table of int32 page numbers: token i of sequence b is token i % page of page
  * table[b * table_stride + i / page].  Slot numbers are page * page_number + offset.  Page, slot and position numbers live on

@@ -601,7 +601,7 @@ extern "C" int qcc_nvfp4_kv_attention(const qcc_kv_attention_args *p, void *work
     if (p->seqs == 0 || p->rows == 0) return 0;
     if (!p->cu_q && p->rows != p->seqs) return QCC_ERR_SHAPE;
     if (!(p->scale > 0.0f)) return QCC_ERR_ARG;
-    if (!p->q || !p->cache || !p->kv_lens || !p->k_outer || !p->v_outer || !p->out || (!p->table && p->table_width > 0)) return QCC_ERR_ARG;
+    if (!p->q || (!p->cache && p->num_pages > 0) || !p->kv_lens || !p->k_outer || !p->v_outer || !p->out || (!p->table && p->table_width > 0)) return QCC_ERR_ARG;
     if (!aligned16(p->q) || !aligned16(p->cache) || !aligned16(p->out) || (p->q_stride[0] | p->q_stride[1]) % 8 != 0) return QCC_ERR_ALIGN;
     const int group = p->q_heads / p->kv_heads, max_q = p->cu_q ? p->max_q : 1, nt = row_tiles_of((int64_t)max_q * group);
     const int64_t cached = (int64_t)p->table_width * p->page;

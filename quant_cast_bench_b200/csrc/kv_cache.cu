@@ -325,7 +325,7 @@ extern "C" int qcc_nvfp4_kv_append(const qcc_kv_append_args *p, void *stream)
     if (p->kv_heads < 1 || p->kv_heads > 4096 || p->q_heads < 0 || p->q_heads > 4096 || !page_ok(p->page) || p->tokens < 0 || p->num_pages < 0) return QCC_ERR_SHAPE;
     if (p->rot < 0 || p->rot > p->head_dim || p->rot % 32 != 0 || p->max_pos < 0) return QCC_ERR_SHAPE;
     if (p->tokens == 0) return 0;
-    if (!p->k || !p->v || !p->cache || !p->slots || !p->k_outer || !p->v_outer) return QCC_ERR_ARG;
+    if (!p->k || !p->v || (!p->cache && p->num_pages > 0) || !p->slots || !p->k_outer || !p->v_outer) return QCC_ERR_ARG;
     if (p->rot > 0 && (!p->positions || !p->cos_sin || p->max_pos < 1)) return QCC_ERR_ARG;
     if (p->q_heads > 0 && (!p->q || !p->q_out)) return QCC_ERR_ARG;
     if (!aligned16(p->k) || !aligned16(p->v) || !aligned16(p->cache) || (p->rot > 0 && !aligned16(p->cos_sin))) return QCC_ERR_ALIGN;
@@ -368,7 +368,7 @@ extern "C" int qcc_nvfp4_kv_gather(const void *cache, int64_t num_pages, int kv_
         table_width < 0 || table_stride < 0)
         return QCC_ERR_SHAPE;
     if (total == 0) return 0;
-    if (!cache || !cu_kv || !k_outer || !v_outer || !k || !v || (!table && table_width > 0)) return QCC_ERR_ARG;
+    if ((!cache && num_pages > 0) || !cu_kv || !k_outer || !v_outer || !k || !v || (!table && table_width > 0 && seqs > 0)) return QCC_ERR_ARG;
     if (!aligned16(cache) || !aligned16(k) || !aligned16(v)) return QCC_ERR_ALIGN;
     const GatherArgs g = {static_cast<const uint8_t *>(cache), table, cu_kv, k_outer, v_outer, static_cast<uint16_t *>(k), static_cast<uint16_t *>(v),
                           total, table_stride, num_pages, seqs, table_width, kv_heads, page};

@@ -934,3 +934,44 @@ def test_max_q_may_be_any_bound():
             Q.nvfp4_kv_attention_cuda(*args, cu_q=cu, max_q=max_q)
         with pytest.raises((AssertionError, RuntimeError)):
             N.nvfp4_kv_attention_native(*args, cu_q=cu, max_q=max_q)
+
+
+@gpu
+def test_empty_batches_and_caches():
+    """A batch without sequences, and a cache without pages: tensors that have no address.  Rows without tokens are zeros, a slot is reported."""
+    from quant_cast_bench_b200 import build as qbuild
+    qbuild.build_torch_binding()
+    from quant_cast_bench_b200.quant_cast_cuda import native_ops as N
+    D, one = 64, torch.ones(1, device="cuda")
+
+    def ints(*v):
+        return torch.tensor(v, dtype=torch.int32, device="cuda")
+    none, page = Q.nvfp4_kv_cache_cuda(0, 2, 16, D), Q.nvfp4_kv_cache_cuda(1, 2, 16, D)
+    x = torch.ones(3, 2, D, dtype=torch.bfloat16, device="cuda")
+    L.device_error()
+    for gather, attention, append in ((Q.nvfp4_kv_gather_cuda, Q.nvfp4_kv_attention_cuda, Q.nvfp4_kv_append_cuda),
+                                      (N.nvfp4_kv_gather_native, N.nvfp4_kv_attention_native, N.nvfp4_kv_append_native)):
+        for cache in (none, page):
+            empty = torch.empty(0, 4, dtype=torch.int32, device="cuda")
+            for t in gather(cache, empty, ints(0), 5, D, one, one) + gather(cache, torch.empty(2, 0, dtype=torch.int32, device="cuda"), ints(0, 0, 0), 5, D, one, one):
+                assert t.shape == (5, 2, D) and not t.any()
+            for kw, lens in ((dict(), ints(0, 0, 0)), (dict(cu_q=ints(0, 2, 2), max_q=2), ints(0, 0)), (dict(cu_q=ints(0, 3), max_q=40), ints(0))):
+                for width in (0, 2):
+                    out, lse = attention(x, cache, torch.zeros(lens.shape[0], width, dtype=torch.int32, device="cuda"), lens, one, one, **kw)
+                    assert not out.any() and bool((lse == -math.inf).all())
+            assert append(x, x, cache, torch.full((3,), -1, device="cuda"), one, one, q=x).equal(x)
+        assert L.device_error() == 0
+        append(x, x, none, torch.tensor([-1, 0, -1], device="cuda"), one, one)
+        assert L.device_error() == 20
+        gather(none, ints(0).view(1, 1), ints(0, 3), 3, D, one, one)
+        assert L.device_error() == 20
+        attention(x[:1], none, ints(0).view(1, 1), ints(3), one, one)
+        assert L.device_error() == 20
+        attention(x, none, ints(0).view(1, 1), ints(3), one, one, cu_q=ints(0, 3), max_q=40)
+        assert L.device_error() == 20
+
+
+def test_c_takes_no_cache_without_pages():
+    lib, p = L.load(), 1 << 20
+    assert lib.qcc_nvfp4_kv_gather(None, 4, 2, 16, 64, p, 4, 4, p, 1, 4, p, p, p, p, None) == -3
+    assert lib.qcc_nvfp4_kv_gather(p, 4, 2, 16, 64, None, 4, 4, p, 1, 4, p, p, p, p, None) == -3
