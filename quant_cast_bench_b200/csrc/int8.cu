@@ -389,10 +389,11 @@ static int mm_dispatch(const CUtensorMap &mw, const CUtensorMap &mx, const MmArg
            : out == QCC_OUT_F16 ? mm_launch<BN, false, QCC_OUT_F16>(mw, mx, g, st) : mm_launch<BN, false, QCC_OUT_F32>(mw, mx, g, st);
 }
 
-// Tokens a tile and shares of K for a product: the pair with the least estimated time.  A block of K takes the longer of its matrix
-// instructions (2 clocks a token, 128 at least: the weights' tile is read at 128 bytes a clock) and of its way from L2 (64 bytes a
-// clock and SM); a tile has a start and an end of about 2500 clocks, of which all but the first overlap with other tiles; adding up
-// over a cluster costs about 1500.  The widths between the powers of two are there for the last wave: 600 x 4096 x 4096 16.4 -> 12.6 us (160
+// Tokens a tile and shares of K for a product: the pair with the least estimated time.  A block of K counts by its way from L2, 128 rows of the
+// weights and b of the tokens at 64 bytes a clock and SM (the matrix instructions take less by this estimate, 2 clocks a token and 128 at
+// least); a tile has a start and an end of about 2500 clocks, of which all but the first overlap with other tiles; adding up
+// over a cluster costs about 1500.  It ranks the choices and is no forecast: wide tiles share what they read, 8192^3 is estimated at 710 000
+// clocks and takes 501 000.  The widths between the powers of two are there for the last wave: 600 x 4096 x 4096 16.4 -> 12.6 us (160
 // tokens), 2000 x 4096 x 7168 43.3 -> 38.9 (224); of 7 sizes tried the choice was the best width in each but for 2 %.
 static void mm_choose(int64_t M, int64_t N, int kblocks, int &bn, int &splits)
 {
@@ -402,7 +403,7 @@ static void mm_choose(int64_t M, int64_t N, int kblocks, int &bn, int &splits)
     for (int b = 16, last = 0; b <= 256; last = b, b += b < 32 ? 16 : 32) {
         if (last >= M) break;
         const int64_t tiles = (N + MM_BM - 1) / MM_BM * ((M + b - 1) / b);
-        const double block = b * 2 > 128 ? (b * 2 > (128 + b) * 2 ? b * 2 : (128 + b) * 2) : (128 + b) * 2;
+        const double block = (MM_BM + b) * 2;
         for (int s = 1; s <= 8; s *= 2) {
             if (s > 1 && ((b & (b - 1)) || kblocks < 2 * s || tiles * s > sms)) break;
             const int64_t waves = (tiles * s + sms - 1) / sms;
