@@ -12,34 +12,7 @@ __device__ __forceinline__ bool elect_one()
     return p != 0;
 }
 
-__device__ __forceinline__ void mbar_arrive(uint64_t *bar)
-{
-    asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
-
-// Wait for phase `parity`.  The wait is bounded: when it runs out it records `code` in the device error word and raises
-// `*abort` (shared memory), which makes every later wait of the CTA return at once, so that the kernel ends soon, with
-// its tensor memory freed, and the host reads the error.
-__device__ __forceinline__ void mbar_wait_abort(uint64_t *bar, uint32_t parity, unsigned int code, volatile uint32_t *abort)
-{
-    const uint32_t a = smem_u32(bar);
-    for (uint32_t it = 0; it < (1u << 22); it++) {
-        uint32_t done;
-        asm volatile(
-            "{\n.reg .pred p;\n"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-            "selp.u32 %0, 1, 0, p;\n}\n"
-            : "=r"(done)
-            : "r"(a), "r"(parity)
-            : "memory");
-        if (done) return;
-        if ((it & 63u) == 63u && *abort) return;
-    }
-    *abort = 1u;
-    atomicMax(&g_qcc_error, code);
-}
-
-// The same by shared-memory address (32 bits: a kernel with many barriers then keeps one base register, the rest are immediates)
+// Barriers by shared-memory address (32 bits: a kernel with many of them then keeps one base register, the rest are immediates)
 __device__ __forceinline__ void mbar_init_at(uint32_t bar, uint32_t count) { asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count)); }
 __device__ __forceinline__ void mbar_arrive_at(uint32_t bar) { asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory"); }
 __device__ __forceinline__ void sts_u32(uint32_t addr, uint32_t v) { asm volatile("st.shared.u32 [%0], %1;" ::"r"(addr), "r"(v) : "memory"); }
@@ -49,7 +22,9 @@ __device__ __forceinline__ uint32_t lds_volatile(uint32_t addr)
     asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
     return v;
 }
-// Whether the phase was reached.  Who arms a barrier or issues copies or matrix instructions behind the wait has to leave where it was not:
+// Wait for phase `parity`: whether it was reached.  The wait is bounded: when it runs out it records `code` in the device error word and
+// raises `abort` (shared memory), which makes every later wait of the CTA return soon, so that the kernel ends, with its tensor memory freed,
+// and the host reads the error.  Who arms a barrier or issues copies or matrix instructions behind the wait has to leave where it was not:
 // arming a barrier again whose phase is incomplete is undefined.
 [[nodiscard]] __device__ __forceinline__ bool mbar_reached(uint32_t bar, uint32_t parity, unsigned int code, uint32_t abort)
 {
@@ -95,7 +70,6 @@ __device__ __forceinline__ void tmem_alloc_at(uint32_t slot, uint32_t cols)
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(slot), "r"(cols) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
 }
-__device__ __forceinline__ void tmem_alloc(uint32_t *slot, uint32_t cols) { tmem_alloc_at(smem_u32(slot), cols); }
 __device__ __forceinline__ void tmem_free(uint32_t addr, uint32_t cols)
 {
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(addr), "r"(cols));
@@ -105,10 +79,6 @@ __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 // arrives on `bar` once every matrix instruction issued by this thread so far has finished
-__device__ __forceinline__ void tc_commit(uint64_t *bar)
-{
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
-}
 __device__ __forceinline__ void tc_commit_at(uint32_t bar)
 {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
@@ -132,13 +102,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, uint32_t (&r)[16])
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr));
-}
-
-// Shared-memory descriptor of a K-major operand whose rows are 128 bytes, swizzled in 128-byte atoms of 8 rows (1024 bytes,
-// 1024-byte aligned).  Stepping K by 32 bytes inside the atom adds 2 (16-byte units) to the descriptor.
-__device__ __forceinline__ uint64_t desc_kmajor_sw128(uint32_t smem_addr)
-{
-    return (uint64_t)((smem_addr >> 4) & 0x3FFFu) | (1ull << 16) | (64ull << 32) | (1ull << 46) | (2ull << 61);
 }
 
 }  // namespace qcc
