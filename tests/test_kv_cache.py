@@ -975,3 +975,52 @@ def test_c_takes_no_cache_without_pages():
     lib, p = L.load(), 1 << 20
     assert lib.qcc_nvfp4_kv_gather(None, 4, 2, 16, 64, p, 4, 4, p, 1, 4, p, p, p, p, None) == -3
     assert lib.qcc_nvfp4_kv_gather(p, 4, 2, 16, 64, None, 4, 4, p, 1, 4, p, p, p, p, None) == -3
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hq,q_len,longest", [(16, 1, 1000), (48, 1, 900), (8, 7, 1000), (80, 1, 500), (16, 8, 400)])      # 4, 12, 14, 20 and 32 rows
+def test_many_short_units_are_dealt_out_whole(D, hq, q_len, longest):
+    """Several whole units a CTA, one after the other; q of each in turn, where it is kept in shared memory, and idle slots between."""
+    g = torch.Generator().manual_seed(hq)
+    lens = [longest] + [0 if i % 16 == 3 else int(n) for i, n in enumerate(torch.randint(1, longest + 1, (169,), generator=g))]
+    q_lens = None if q_len == 1 else [q_len if i % 3 else int(i % q_len) for i in range(170)]
+    before = L.launch_count
+    check_attention(D, 32, hq, 4, lens, q_lens, seed=hq + D)
+    assert L.launch_count - before == 1
+
+
+@gpu
+def test_the_operators_trace_under_torch_compile():
+    """A decoder step in one graph: the append writes the cache, an argument, and the reads behind it see that."""
+    from quant_cast_bench_b200 import build as qbuild
+    qbuild.build_torch_binding()
+    from quant_cast_bench_b200.quant_cast_cuda import native_ops as N
+    D, page, heads, qh, tokens = 64, 16, 2, 8, 20
+    g = torch.Generator().manual_seed(3)
+    w, ws = Q.rowwise_int8_cuda(torch.randn((qh + 2 * heads) * D, 256, generator=g).to(torch.bfloat16).cuda())
+    x = torch.randn(tokens, 256, generator=g).to(torch.bfloat16).cuda()
+    rope, slots, pos = rotation_table(tokens, D).cuda(), torch.arange(tokens).cuda(), torch.arange(tokens).cuda()
+    one, table = torch.tensor([0.02]).cuda(), torch.tensor([[1, 0]], dtype=torch.int32).cuda()
+    cu, n = torch.tensor([0, tokens], dtype=torch.int32).cuda(), torch.tensor([tokens], dtype=torch.int32).cuda()
+
+    def step(x, cache):
+        a, s = N.rowwise_int8_native(x * 2.0)
+        q, k, v = N.int8_scaled_mm_native(a, w, s, ws).view(tokens, qh + 2 * heads, D).split([qh, heads, heads], 1)
+        q = N.nvfp4_kv_append_native(k, v, cache, slots, one, one, positions=pos, cos_sin=rope, q=q)
+        kb, vb = N.nvfp4_kv_gather_native(cache, table, cu, tokens, D, one, one)
+        out, lse = N.nvfp4_kv_attention_native(q, cache, table, n, one, one, cu_q=cu, max_q=tokens)
+        last, last_lse = N.nvfp4_kv_attention_native(q[-1:], cache, table, n, one, one, scale=0.1)
+        return q, kb, vb, out * 1.0, lse, last, last_lse
+
+    caches = [torch.zeros(2, heads, 2, page * 36, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    slots = (table[0].long()[slots // page] * page + slots % page).contiguous()
+    want = step(x, caches[0])
+    got = torch.compile(step, fullgraph=True)(x, caches[1])
+    assert torch.equal(*caches) and bool(caches[0].any())
+    for a, b in zip(got, want):
+        assert a.dtype == b.dtype and torch.equal(a, b)
+    for op, args in ((N.ops.nvfp4_kv_append, (want[1], want[2], caches[0], slots, one, one)), (N.ops.int8_rowwise, (x,)),
+                     (N.ops.int8_scaled_mm, (*N.rowwise_int8_native(x)[:1], w, N.rowwise_int8_native(x)[1], ws)),
+                     (N.ops.nvfp4_kv_gather, (caches[0], table, cu, tokens, D, one, one)), (N.ops.nvfp4_kv_attention, (want[0][-1:], caches[0], table, n, one, one))):
+        torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
