@@ -43,7 +43,7 @@ __device__ __forceinline__ uint32_t int8x4(uint32_t w0, uint32_t w1, float inv)
 }
 
 // One CTA per row.  The row stays in registers (CH 16-byte pieces a thread) between its maximum and the cast, so x is read
-// once; CH = 0: rows too long for that, or not a multiple of 8 elements, are read twice (the second time from L2).
+// once; CH = 0: rows too long for that, or not a multiple of 8 elements, are read twice (the second time from L2), an element at a time.
 template <int CH>
 __global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t *x, int64_t N, uint8_t *q,
                                                                   float *scale, int recip_div)
@@ -98,8 +98,8 @@ __global__ void __launch_bounds__(I8_THREADS) int8_rowwise_kernel(const uint16_t
 // Where there are fewer tiles than SMs, the CTAs of a cluster share out K and add their sums up through each other's shared
 // memory; whole numbers, so in any order the same.
 //
-// Measured: 8192^3 359 us, 3.06 POP/s, tensor cores 93 % active; 2000 x 4096 x 7168 39 us, 3.0 POP/s; 64 x 14336 x 4096 10.7 us, weights at 5.6 TB/s.  Rows
-// of K that are no multiple of 128 bytes cost a second line a row: K = 2064 21 us where 2048 takes 14.
+// Measured: 8192^3 351 us, 3.13 POP/s, tensor cores 92 % active; 2000 x 4096 x 7168 39 us, 3.0 POP/s; 64 x 14336 x 4096 9.7 us, again and again on the
+// same weights (59 MB, less than L2).  Rows of K that are no multiple of 128 bytes cost a second line a row: K = 2064 21 us where 2048 takes 14.
 constexpr int MM_BM = 128, MM_BK = 128, MM_THREADS = 384;
 constexpr unsigned int MM_ERR = 7;   // a barrier wait of the product ran out
 

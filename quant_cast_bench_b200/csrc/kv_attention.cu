@@ -36,8 +36,8 @@ constexpr unsigned int KV_ATTN_ERR = 8u;            // a wait for a bulk copy ra
 // whatever the lengths; a unit (sequence, head, row tile) that spans CTAs leaves partial sums which a second kernel joins in a
 // fixed order.  Short units are dealt out whole instead, where there are many.
 //
-// Measured, 32 heads over 8 of 128 elements: 64 sequences of up to 16384 tokens 133.5 us, 4.4 TB/s of the cache, 55 % of the issue slots and of the
-// ALU pipe; 2 of 131072 with 64 heads 73 us.  647 warp instructions for 32 tokens, of which the conversions, scalings and nibble merges are
+// Measured, 32 heads over 8 of 128 elements: 64 sequences of up to 16384 tokens 132.5 us, 4.4 TB/s of the cache, 56 % of the issue slots and of the
+// ALU pipe; 2 of 131072 with 64 heads 72.3 us.  647 warp instructions for 32 tokens, of which the conversions, scalings and nibble merges are
 // 372 and the matrix instructions 32.
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int SP_WARPS = 4, SP_THREADS = SP_WARPS * 32, SP_WTOK = 32, SP_TOK = SP_WTOK * SP_WARPS;

@@ -98,7 +98,7 @@ __device__ __forceinline__ void seq_of(const AttnArgs &g, int b, int &q0, int &n
 }
 
 // The power of two that brings a row of q to fp16, its largest magnitude (fp32 bits) to [2^7, 2^8), and its inverse; 1 for a row
-// with an infinity or a NaN, which stay what they are.  2^70 at most: rows that are smaller still score 0 to all 24 bits of exp.
+// with an infinity.  Infinities and NaN stay what they are.  2^70 at most: rows that are smaller still score 0 to all 24 bits of exp.
 __device__ __forceinline__ void q_power(uint32_t largest, float &mult, float &back)
 {
     uint32_t e = largest >> 23;

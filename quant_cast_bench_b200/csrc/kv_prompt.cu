@@ -24,10 +24,11 @@ namespace qcc {
 // row tiles.  All (unit, tile) pairs are numbered, by a first small kernel, and dealt out evenly to one CTA per SM, whatever the lengths and however
 // many tiles the causal mask leaves a unit; a unit that spans CTAs leaves partial sums, which a third kernel joins in a fixed order.
 //
-// Measured, 32 heads over 8 of 128 elements: 4096 queries over 12288 tokens 599 us, 1.15 PFLOP/s (tensor cores 56 % active); 16 prompts of up to 700 tokens
-// 111 us.  A pair of row tiles and a tile of tokens takes about 3000 clocks, of which the exponentials are 1024 and the matrix
-// instructions 1024 by their rates, one after the other for a row tile.  The warps' code is close to what the instruction cache holds: loops
-// that run once a part or are not on the critical path are rolled up (145 -> 111 us for the prompts of 700 tokens).
+// Measured, 32 heads over 8 of 128 elements: 4096 queries over 12288 tokens 600 us, 1.15 PFLOP/s (tensor cores 56 % active, exponential unit 55 %; 651 us
+// and 1.60 GHz under the profiler, 1 044 000 clocks both); 16 prompts of up to 700 tokens 114 us.  A pair of row tiles and a tile of tokens takes
+// about 3750 clocks, in which the exponentials and the matrix instructions of both need 2048 each by their rates; those of one row tile
+// follow one another, and the two row tiles do not overlap fully.  The warps' code is close to what the instruction cache holds: loops
+// that run once a part or are not on the critical path are rolled up (145 -> 111 us for the prompts of 700 tokens, when it was done).
 // -------------------------------------------------------------------------------------------------------------------
 constexpr int PT_THREADS = 512, PT_TOK = 128, PT_ROWS = 256, PT_RAW = 3, PT_NOTES = 8;
 constexpr uint32_t PT_LAST = 256u, PT_TWO = 512u, PT_MASK = 1024u;      // notes on a tile: the last of its part; both row tiles of its
