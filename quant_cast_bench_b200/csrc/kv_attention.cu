@@ -353,14 +353,14 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int x = 0; x < 2; x++) {
-                            float v = m[nt][x];
+                            float top = -INFINITY;
 #pragma unroll
                             for (int h = 0; h < HB; h++)
 #pragma unroll
-                                for (int y = x; y < 4; y += 2) v = fmaxf(v, seen(h, nt, y) ? fmaf(sc[h][nt][y], factor[nt][x], -P_LIFT) : -INFINITY);
+                                for (int y = x; y < 4; y += 2) top = fmaxf(top, seen(h, nt, y) ? sc[h][nt][y] : -INFINITY);
 #pragma unroll
-                            for (int sh = 4; sh < 32; sh <<= 1) v = fmaxf(v, __shfl_xor_sync(0xFFFFFFFFu, v, sh));
-                            const float a = v == -INFINITY ? 1.0f : ex2(m[nt][x] - v);
+                            for (int sh = 4; sh < 32; sh <<= 1) top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, sh));
+                            const float v = fmaxf(m[nt][x], reference_of(top, factor[nt][x])), a = v == -INFINITY ? 1.0f : ex2(m[nt][x] - v);
                             m[nt][x] = v;
                             l[nt][x] *= a;
 #pragma unroll

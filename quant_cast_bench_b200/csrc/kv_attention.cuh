@@ -11,6 +11,13 @@ constexpr float LOG2E = 1.4426950408889634f, LN2 = 0.6931471805599453f;
 // is set and, as that moves only once a score is P_MOST above it, at most 2^15.  So the upper end of fp16's range is used, and a key's rounding is half a step,
 // 2^-11, down to 2^-21 of the largest; below, half of 2^-24, 2^-32 of the largest.  (All in log2 units; lse has the reference added back.)
 constexpr float P_LIFT = 7.0f, P_MOST = 15.0f;
+// the reference for a row's largest score; scores beyond 2^28 are multiples of 32, and one whose reference was rounded down that far would leave
+// fp16's range: there the next number up
+__device__ __forceinline__ float reference_of(float score, float factor)
+{
+    const float r = fmaf(score, factor, -P_LIFT);
+    return fmaf(score, factor, -r) > P_MOST ? u2f(f2u(r) + (r > 0.0f ? 1u : 0xFFFFFFFFu)) : r;
+}
 
 struct AttnArgs {
     const uint16_t *q;

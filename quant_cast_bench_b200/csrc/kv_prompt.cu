@@ -659,7 +659,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
                     const float most = fmaxf(max3(top[0], top[1], top[2]), top[3]);
                     const bool grow = fmaf(most, scale_in, -m) > P_MOST;      // (from -inf: always, once the row sees a key; one rounding, as below)
                     if (__any_sync(0xFFFFFFFFu, grow)) {
-                        const float up = grow ? fmaf(most, scale_in, -P_LIFT) : m, a = grow ? ex2(m - up) : 1.0f;
+                        const float up = grow ? reference_of(most, scale_in) : m, a = grow ? ex2(m - up) : 1.0f;
                         m = up;
                         l *= a;
                         if (any) {

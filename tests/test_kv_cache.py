@@ -1024,3 +1024,24 @@ def test_the_operators_trace_under_torch_compile():
                      (N.ops.int8_scaled_mm, (*N.rowwise_int8_native(x)[:1], w, N.rowwise_int8_native(x)[1], ws)),
                      (N.ops.nvfp4_kv_gather, (caches[0], table, cu, tokens, D, one, one)), (N.ops.nvfp4_kv_attention, (want[0][-1:], caches[0], table, n, one, one))):
         torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("hq,q_len", [(4, 1), (16, 1), (32, 1), (8, 10), (8, 40)])      # each form of the kernels
+def test_scores_that_leave_no_bits_for_a_difference(D, hq, q_len):
+    """Keys of one score, up to 2^29 in log2 units, where fp32 numbers are 32 apart: each has the same weight all the same."""
+    n, page = 200, 64
+    cache = torch.zeros(4, 1, 2, page * 9 * D // 16, dtype=torch.uint8)
+    codes, scales = planes(cache, D)
+    scales.fill_(0x38)                                        # 1.0
+    codes.fill_(0x22)                                         # 1.0 in every element of keys and values, but 37 twos in a key:
+    codes[:, :, 0, :, :18], codes[:, :, 0, :, 18] = 0x44, 0x24      # a product of score and factor has more than 24 bits
+    dot = D + 37
+    table, one, q = torch.arange(4, dtype=torch.int32).view(1, 4), torch.ones(1), torch.ones(q_len, hq, D, dtype=torch.bfloat16)
+    for log2 in [1.0, 1e3, 1e6] + [2.0 ** 27 * x for x in (1.1, 1.37, 1.73)] + [2.0 ** 28 * x for x in (1.03, 1.13, 1.27, 1.37, 1.49, 1.6, 1.72, 1.83, 1.91, 1.97)]:
+        scale = float(torch.tensor(log2 * math.log(2) / dot))
+        out, lse = call(q, cache, table, [n], [q_len], one, one, scale, decode=q_len == 1)
+        assert bool(((out.cpu().double() - 1).abs() <= 2.0 ** -8 + 2.0 ** -11).all()), log2
+        want = scale * dot + torch.log(torch.arange(n - q_len + 1, n + 1).double()).view(-1, 1)
+        assert bool(((lse.cpu().double() - want).abs() <= 2.0 ** -21 * want).all()), log2
