@@ -497,6 +497,9 @@ __device__ __forceinline__ void named_barrier(int id, int threads)
 // flagged launch begin as soon as every CTA of the earlier kernel has started.  Both are no-ops in launches that are
 // not part of such a pair.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// Copies by the async proxy (bulk and TMA copies) are not ordered by that wait alone: who issues them behind it, and may read what the
+// predecessor stored, calls this in between.
+__device__ __forceinline__ void pdl_copies_fence() { asm volatile("fence.proxy.async.global;" ::: "memory"); }
 __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 // a per-tensor scalar that an overlapped predecessor wrote: read past L1 (which may hold what an earlier kernel saw)
 __device__ __forceinline__ float ld_cg_f32(const float *p)

@@ -201,6 +201,7 @@ __global__ void __launch_bounds__(MM_THREADS, 1) int8_mm_kernel(const __grid_con
 
     if (warp == 0) {
         if (elect_one()) {
+            pdl_copies_fence();
             uint32_t s = 0, ph = 1;
             bool go = true;
             for (int t = t0; go && t < total; t += step) {

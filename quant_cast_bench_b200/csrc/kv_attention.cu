@@ -229,6 +229,7 @@ __global__ void __launch_bounds__(SP_THREADS, (SplitCfg<D, NT>::CTAS)) kv_attn_s
     // where a stage has codes and scales of keys and values, and the distance from the first 16 tokens to the second
     const uint32_t k_scales = shift == 4 ? 8 * D : SP_WTOK * D / 2, v_codes = shift == 4 ? 16 * RB : C::TILE / 2, v_scales = v_codes + k_scales;
     const uint32_t next_codes = shift == 4 ? C::TILE / 2 : 8 * D, next_scales = shift == 4 ? C::TILE / 2 : D;
+    pdl_copies_fence();
     seek();
 #pragma unroll 1
     for (int i = 0; i < C::STAGES; i++) fetch();

@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) kv_prompt_kernel(const __grid_c
         asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
         if (warp == 0) {
             // ---- copies: a tile's keys, then its values
+            pdl_copies_fence();
             uint32_t st = 0, ph = 1, tiles = 0;
             const int pages = PT_TOK / g.page;
             const uint32_t half = (uint32_t)(g.page * RB);

@@ -49,3 +49,14 @@ def test_few_queries_a_lane_whose_wait_ran_out_stops_copying():
     assert len(waits) == len(re.findall(r"\bcopied\(", text)) - 1 == 1 and "f_stage |= SP_LATE;" in waits[0] and "out_of_time = 1;" in waits[0]
     end = text.index("settle(smem")
     assert text.rindex("named_barrier(", 0, end) > text.rindex("fetch()", 0, end)
+
+
+@pytest.mark.parametrize("name", ["int8.cu", "kv_attention.cu", "kv_prompt.cu"])
+def test_copies_are_ordered_behind_the_overlapped_predecessor(name):
+    """Between the wait for the predecessor's end and the first copy by the async proxy stands a fence between the proxies."""
+    text = source(name)
+    fences = [m.start() for m in re.finditer(r"\bpdl_copies_fence\(\)", text)]
+    kernel = text.index("__grid_constant__ CUtensorMap map_w") if name == "int8.cu" else text.index("kv_attn_split_kernel(" if name == "kv_attention.cu" else "kv_prompt_kernel(const")
+    wait = text.index("pdl_wait()", kernel)
+    issue = text.index({"int8.cu": "tma_load_2d_at(", "kv_prompt.cu": "bulk_load_at(", "kv_attention.cu": "fetch();"}[name], kernel)
+    assert len(fences) == 1 and wait < fences[0] < issue
